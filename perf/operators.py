@@ -327,7 +327,7 @@ def _grow(s, seqs, n_new):
     need = want - have + copy
     upto = torch.cumsum(need, 0)
     free = torch.sort((refs > 0).int(), stable=True).indices
-    ok = upto <= (refs == 0).sum()
+    ok = (upto <= (refs == 0).sum()) | (need == 0)
     col = torch.arange(t.shape[1], device="cuda")[None, :]
     is_new = ok[:, None] & (col >= have[:, None]) & (col < want[:, None])
     is_copy = (ok & copy)[:, None] & (col == have[:, None] - 1)
