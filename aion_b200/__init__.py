@@ -69,6 +69,13 @@ class Opts(ctypes.Structure):
                 ("reserved", ctypes.c_int32 * 6)]
 
 
+class KV8(ctypes.Structure):
+    """aion_kv8: the view of an 8-bit paged K/V cache."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k", "v", "k_scale", "v_scale", "tables", "lens", "refs", "work")] + \
+               [(n, ctypes.c_int32) for n in ("device", "n_layers", "n_pages", "n_kv_heads", "page_tokens", "head_size",
+                                              "max_seqs", "max_pages")]
+
+
 _lib = None
 
 
@@ -118,6 +125,18 @@ def lib() -> ctypes.CDLL:
         "aion_quantize_buffer_dev": (I32, [VP, VP, VP, I64, VP]),
         "aion_tp_connect": (I32, [VP, VP]),
         "aion_quantize_activations": (I32, [VP, VP, VP, I64, VP]),
+        "aion_kv8_create": (I32, [P(KV8), P(KV8)]),
+        "aion_kv8_destroy": (I32, [P(KV8)]),
+        "aion_kv8_reset": (I32, [VP, VP]),
+        "aion_kv8_grow": (I32, [VP, VP, VP, I32, VP, VP]),
+        "aion_kv8_fork": (I32, [VP, VP, VP, VP, I32, VP]),
+        "aion_kv8_trim": (I32, [VP, VP, VP, I32, VP]),
+        "aion_kv8_compact": (I32, [VP, VP, VP]),
+        "aion_kv8_append": (I32, [VP, I32, VP, VP, I32, I64, I64, VP, VP, VP, I32, I32, VP]),
+        "aion_kv8_read": (I32, [VP, I32, VP, VP, I32, I64, I64, VP, VP, VP, I32, I32, VP]),
+        "aion_kv8_attention": (I32, [VP, I32, VP, VP, I32, I32, I64, I64, F, VP, VP, VP, I32, I32, VP, I64, VP]),
+        "aion_kv8_attention_workspace": (I64, [VP, I32, I32, I32]),
+        "aion_kv8_status": (I32, [VP, VP]),
         "aion_quantize_buffer": (None, [VP, VP, VP, I64]),
         "aion_checkpoint_bytes": (I64, [P(I32), ctypes.c_int]),
         "aion_quantize_file": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_char_p, ctypes.c_int, ctypes.c_char_p,
@@ -437,5 +456,224 @@ def quantize_activations(x, qx, xs, stream=None) -> None:
                                            _dev_ptr(xs, "torch.float32", n // 32), n, _stream_ptr(stream)))
 
 
-__all__ = ["AionError", "Config", "Model", "QMatrix", "checkpoint_bytes", "lib", "quantize_activations",
+class KV8Cache:
+    """An 8-bit paged K/V cache (aion_kv8 of include/aion.h): int8 K and V rows
+    in pages of page_tokens tokens with one fp32 scale per (layer, page, K/V
+    head), a page table for each of max_seqs slots, and a count of the slots
+    that hold each page.
+
+    The arrays are torch tensors on one CUDA device: k, v [n_layers][n_pages]
+    [n_kv_heads][page_tokens][head_size] int8; k_scale, v_scale [n_layers]
+    [n_pages][n_kv_heads] fp32; tables [max_seqs][max_pages], lens [max_seqs]
+    and refs [n_pages] int32.  All calls are asynchronous on `stream` (default:
+    torch's current stream of that device); seqs, pos0, n_new, keep, src, dst
+    and cu are int32 CUDA tensors.  status() waits and raises what the calls
+    could only see on the device.
+    """
+
+    def __init__(self, n_layers: int, n_pages: int, n_kv_heads: int, head_size: int, max_seqs: int, max_pages: int,
+                 page_tokens: int = 64, device: int = 0):
+        import torch
+        dev = torch.device("cuda", device)
+        pool, sc = (n_layers, n_pages, n_kv_heads, page_tokens, head_size), (n_layers, n_pages, n_kv_heads)
+        self._bind(torch.zeros(pool, dtype=torch.int8, device=dev), torch.zeros(pool, dtype=torch.int8, device=dev),
+                   torch.zeros(sc, device=dev), torch.zeros(sc, device=dev),
+                   torch.full((max_seqs, max_pages), -1, dtype=torch.int32, device=dev),
+                   torch.zeros(max_seqs, dtype=torch.int32, device=dev),
+                   torch.zeros(n_pages, dtype=torch.int32, device=dev))
+
+    @classmethod
+    def wrap(cls, k, v, k_scale, v_scale, tables, lens, refs) -> "KV8Cache":
+        """A cache over arrays that exist already (contiguous CUDA tensors)."""
+        self = cls.__new__(cls)
+        self._bind(k, v, k_scale, v_scale, tables, lens, refs)
+        return self
+
+    def _bind(self, k, v, k_scale, v_scale, tables, lens, refs) -> None:
+        import torch
+        if k.dim() != 5 or tables.dim() != 2:
+            raise ValueError("k must be [layer][page][head][token][head_size], tables [slot][page]")
+        n_layers, n_pages, n_kv, page, hd = k.shape
+        max_seqs, max_pages = tables.shape
+        for name, t, dtype, shape in (("k", k, torch.int8, k.shape), ("v", v, torch.int8, k.shape),
+                                      ("k_scale", k_scale, torch.float32, k.shape[:3]),
+                                      ("v_scale", v_scale, torch.float32, k.shape[:3]),
+                                      ("tables", tables, torch.int32, tables.shape),
+                                      ("lens", lens, torch.int32, (max_seqs,)), ("refs", refs, torch.int32, (n_pages,))):
+            if not t.is_cuda or t.device != k.device or not t.is_contiguous() or t.dtype != dtype or \
+                    tuple(t.shape) != tuple(shape):
+                raise ValueError(f"{name}: expected a contiguous {dtype} tensor of shape {tuple(shape)} on {k.device}, "
+                                 f"got {t.dtype} {tuple(t.shape)} on {t.device}")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.tables, self.lens, self.refs = tables, lens, refs
+        self.work = torch.zeros(4 + 3 * n_pages, dtype=torch.int32, device=k.device)
+        torch.cuda.current_stream(k.device).synchronize()   # the arrays are ready for calls on any stream
+        self.device = k.device
+        self.n_layers, self.n_pages, self.n_kv_heads, self.page_tokens, self.head_size = n_layers, n_pages, n_kv, page, hd
+        self.max_seqs, self.max_pages = max_seqs, max_pages
+        self._c = KV8(*[t.data_ptr() for t in (k, v, k_scale, v_scale, tables, lens, refs, self.work)],
+                      k.device.index, n_layers, n_pages, n_kv, page, hd, max_seqs, max_pages)
+        self._p = ctypes.addressof(self._c)
+        self._types = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+        self._ws = {}   # bytes of workspace by (heads, sequences, rows)
+        if lib().aion_kv8_attention_workspace(self._p, n_kv, 1, 1) < 0:
+            _check(3)
+
+    # -- arguments ----------------------------------------------------------
+    def _stream(self, stream):
+        if stream is None:
+            import torch
+            return torch.cuda.current_stream(self.device).cuda_stream
+        return getattr(stream, "cuda_stream", stream)
+
+    def _empty(self, shape, dtype, stream):
+        """A new tensor that belongs to the stream the call runs on."""
+        import torch
+        if stream is None:
+            return torch.empty(shape, dtype=dtype, device=self.device)
+        if isinstance(stream, int):
+            stream = torch.cuda.ExternalStream(stream, device=self.device)
+        with torch.cuda.stream(stream):
+            return torch.empty(shape, dtype=dtype, device=self.device)
+
+    def _ints(self, name: str, t, n: int) -> int:
+        if t.dtype != self.tables.dtype or t.device != self.device or not t.is_contiguous() or t.numel() < n:
+            raise ValueError(f"{name}: expected a contiguous int32 tensor with >= {n} elements on {self.device}")
+        return t.data_ptr()
+
+    def _rows(self, name: str, t, n: int, heads: int):
+        """(pointer, row stride) of an [n][heads][head_size] tensor whose rows are dense."""
+        if t.dtype not in self._types or t.device != self.device:
+            raise ValueError(f"{name}: expected an fp32, fp16 or bf16 tensor on {self.device}")
+        if tuple(t.shape) != (n, heads, self.head_size):
+            raise ValueError(f"{name}: expected shape {(n, heads, self.head_size)}, got {tuple(t.shape)}")
+        st = t.stride()
+        if (st[2] != 1 and self.head_size > 1) or (heads > 1 and st[1] != self.head_size):
+            raise ValueError(f"{name}: the values of one token must be dense (strides {st})")
+        return t.data_ptr(), st[0]
+
+    def _seqs(self, seqs, pos0, cu, n_tok: int):
+        n = seqs.numel()
+        if cu is None and n != n_tok:
+            raise ValueError(f"without cu every sequence has one row: {n} sequences, {n_tok} rows")
+        return (self._ints("seqs", seqs, n), self._ints("pos0", pos0, n),
+                None if cu is None else self._ints("cu", cu, n + 1), n)
+
+    # -- rows ---------------------------------------------------------------
+    def append(self, layer: int, k, v, seqs, pos0, cu=None, stream=None) -> None:
+        """Writes k, v [n_tok][n_kv_heads][head_size] at positions pos0[i].. of
+        slots seqs[i]; sequence i has rows cu[i]..cu[i+1]-1 (cu None: one each)
+        (aion_kv8_append)."""
+        n_tok = k.shape[0]
+        kp, ks = self._rows("k", k, n_tok, self.n_kv_heads)
+        vp, vs = self._rows("v", v, n_tok, self.n_kv_heads)
+        if k.dtype != v.dtype:
+            raise ValueError("k and v differ in type")
+        sp, pp, cp, n = self._seqs(seqs, pos0, cu, n_tok)
+        st = lib().aion_kv8_append(self._p, layer, kp, vp, self._types[k.dtype], ks, vs, sp, pp, cp, n, n_tok,
+                                   self._stream(stream))
+        if st:
+            _check(st)
+
+    def read(self, layer: int, seqs, pos0, n_tok: int, cu=None, dtype=None, out=None, stream=None):
+        """The K and V rows at those positions as the cache holds them: a pair of
+        [n_tok][n_kv_heads][head_size] tensors (`out`, or new ones of `dtype`,
+        default fp32) (aion_kv8_read)."""
+        if out is None:
+            shape, dtype = (n_tok, self.n_kv_heads, self.head_size), dtype or self.k_scale.dtype
+            out = self._empty(shape, dtype, stream), self._empty(shape, dtype, stream)
+        k, v = out
+        kp, ks = self._rows("k", k, n_tok, self.n_kv_heads)
+        vp, vs = self._rows("v", v, n_tok, self.n_kv_heads)
+        if k.dtype != v.dtype:
+            raise ValueError("k and v differ in type")
+        sp, pp, cp, n = self._seqs(seqs, pos0, cu, n_tok)
+        st = lib().aion_kv8_read(self._p, layer, kp, vp, self._types[k.dtype], ks, vs, sp, pp, cp, n, n_tok,
+                                 self._stream(stream))
+        if st:
+            _check(st)
+        return k, v
+
+    def attention(self, layer: int, q, seqs, pos0, cu=None, scale: float | None = None, out=None, stream=None):
+        """Attention of q [n_tok][n_heads][head_size]: the row at position p of
+        slot seqs[i] sees positions 0..p (aion_kv8_attention).  Returns `out`
+        (default: a new tensor like q)."""
+        n_tok, n_heads = q.shape[0], q.shape[1]
+        qp, qs = self._rows("q", q, n_tok, n_heads)
+        if out is None:
+            out = self._empty((n_tok, n_heads, self.head_size), q.dtype, stream)
+        elif out.dtype != q.dtype:
+            raise ValueError("q and out differ in type")
+        op, os_ = self._rows("out", out, n_tok, n_heads)
+        sp, pp, cp, n = self._seqs(seqs, pos0, cu, n_tok)
+        if scale is None:
+            scale = 0.0
+        elif scale == 0.0:
+            raise ValueError("a scale of 0 stands for the default: pass None")
+        key = (n_heads, n, n_tok)
+        ws = self._ws.get(key)
+        if ws is None:
+            if len(self._ws) > 4096:   # ragged serving meets many shapes
+                self._ws.clear()
+            ws = self._ws[key] = lib().aion_kv8_attention_workspace(self._p, *key)
+            if ws < 0:
+                _check(3)
+        buf = self._empty((ws,), self.k.dtype, stream) if ws else None
+        st = lib().aion_kv8_attention(self._p, layer, qp, op, self._types[q.dtype], n_heads, qs, os_, scale, sp, pp, cp,
+                                      n, n_tok, buf.data_ptr() if ws else None, ws, self._stream(stream))
+        if st:
+            _check(st)
+        return out
+
+    # -- pages --------------------------------------------------------------
+    def grow(self, seqs, n_new, pos0=None, stream=None):
+        """Makes room for n_new[i] more tokens in slot seqs[i]; returns pos0, the
+        position of each one's first new token or -1 where it was refused
+        (aion_kv8_grow)."""
+        n = seqs.numel()
+        if pos0 is None:
+            pos0 = self._empty((n,), seqs.dtype, stream)
+        st = lib().aion_kv8_grow(self._p, self._ints("seqs", seqs, n), self._ints("n_new", n_new, n), n,
+                                 self._ints("pos0", pos0, n), self._stream(stream))
+        if st:
+            _check(st)
+        return pos0
+
+    def fork(self, src, dst, keep=None, stream=None) -> None:
+        """Slot dst[i] shares the pages of slot src[i]'s first keep[i] tokens
+        (None: all of them) (aion_kv8_fork)."""
+        n = src.numel()
+        st = lib().aion_kv8_fork(self._p, self._ints("src", src, n), self._ints("dst", dst, n),
+                                 None if keep is None else self._ints("keep", keep, n), n, self._stream(stream))
+        if st:
+            _check(st)
+
+    def trim(self, seqs, keep=None, stream=None) -> None:
+        """Slot seqs[i] keeps its first keep[i] tokens (None: none)
+        (aion_kv8_trim)."""
+        n = seqs.numel()
+        st = lib().aion_kv8_trim(self._p, self._ints("seqs", seqs, n),
+                                 None if keep is None else self._ints("keep", keep, n), n, self._stream(stream))
+        if st:
+            _check(st)
+
+    def compact(self, n_used=None, stream=None) -> None:
+        """Moves pages until those in use come first; n_used (int32, one element)
+        receives their number (aion_kv8_compact)."""
+        st = lib().aion_kv8_compact(self._p, None if n_used is None else self._ints("n_used", n_used, 1),
+                                    self._stream(stream))
+        if st:
+            _check(st)
+
+    def reset(self, stream=None) -> None:
+        """Empties every slot and frees every page."""
+        _check(lib().aion_kv8_reset(self._p, self._stream(stream)))
+
+    def status(self, stream=None) -> None:
+        """Waits for the stream; raises AionError for what the calls before it
+        refused on the device (aion_kv8_status)."""
+        _check(lib().aion_kv8_status(self._p, self._stream(stream)))
+
+
+__all__ = ["AionError", "Config", "KV8Cache", "Model", "QMatrix", "checkpoint_bytes", "lib", "quantize_activations",
            "quantize_buffer", "quantize_file", "synth_checkpoint", "MODE_W4A16", "MODE_W4A8"]

@@ -29,7 +29,7 @@ NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC,-fvisibilit
 CC_FLAGS = ["-O2", "-std=gnu11", "-fPIC", "-fvisibility=hidden", "-ffp-contract=off", "-pthread", "-Wall",
             "-Wno-unused-result"]
 
-CUDA_SOURCES = ["aion_runtime.cu"]
+CUDA_SOURCES = ["aion_runtime.cu", "aion_kv8.cu"]
 C_SOURCES = ["aion_ckpt.c", "aion_tok.c"]
 
 

@@ -30,6 +30,7 @@
 #include "decode_batch.cuh"
 #include "decode_step.cuh"
 #include "gemm_tc.cuh"
+#include "kv8.h"
 #include "prefill.cuh"
 
 using namespace aion;
@@ -46,6 +47,15 @@ static void set_err(std::string* dst, const char* fmt, ...) {
     vsnprintf(buf, sizeof(buf), fmt, ap);
     va_end(ap);
     if (dst) *dst = buf;
+    g_thread_err = buf;
+}
+
+void aion_thread_error(const char* fmt, ...) {
+    char buf[512];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof(buf), fmt, ap);
+    va_end(ap);
     g_thread_err = buf;
 }
 

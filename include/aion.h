@@ -314,6 +314,135 @@ AION_API aion_status aion_quantize_activations(const float* x_dev, int8_t* qx_de
                                                void* stream);
 
 /* ---------------------------------------------------------------------------
+ * 8-bit paged K/V cache (no counterpart in the reference, whose cache is one
+ * fp32 array per sequence, src/kernel_simd.c:1006-1007).
+ *
+ * A cache holds the K and V rows of many sequences ("slots") in pages of
+ * page_tokens tokens, int8 values with one fp32 scale per (layer, page, K/V
+ * head): value = q * scale.  A slot's table lists its pages in order; a page
+ * may be held by several slots (refs counts them) and is then never written.
+ *
+ * The struct is a view: its pointers are device memory of the caller, or of
+ * aion_kv8_create.  Every call below is enqueued on `stream` and returns at
+ * once; the calls that change a cache, and a call that reads it after them,
+ * have to be ordered (one stream, or events).  Reads (aion_kv8_read,
+ * aion_kv8_attention) of one cache may run at the same time.  All calls but
+ * _create, _destroy and _status can be captured into a CUDA graph.  The
+ * current device is left as it was.
+ *
+ * seqs, pos0, n_new, keep, src, dst and cu are int32 arrays in device memory.
+ * What the host cannot see in them is checked on the device: an entry whose
+ * slot or count is out of range, or whose slot a changing call has met
+ * earlier in its list, is skipped (the first one counts), as is a row whose
+ * page is missing, and the cache's status word records it for
+ * aion_kv8_status.  Nothing out of bounds is read or written.
+ * ------------------------------------------------------------------------- */
+typedef struct aion_kv8 {
+    int8_t *k, *v;             /* [n_layers][n_pages][n_kv_heads][page_tokens][head_size], 16-byte aligned */
+    float *k_scale, *v_scale;  /* [n_layers][n_pages][n_kv_heads]                                          */
+    int32_t* tables;           /* [max_seqs][max_pages] page ids; entries behind a slot's last page: -1    */
+    int32_t* lens;             /* [max_seqs] tokens of each slot                                           */
+    int32_t* refs;             /* [n_pages] slots that hold the page; 0: free                              */
+    int32_t* work;             /* [4 + 3 * n_pages]: status word, page lists of the call in flight; zeroed
+                                  before the first call                                                    */
+    int32_t device;
+    int32_t n_layers, n_pages, n_kv_heads;
+    int32_t page_tokens;       /* 16, 32, 64 or 128                                                        */
+    int32_t head_size;         /* a multiple of 16, at most 128                                            */
+    int32_t max_seqs;          /* slots, at most 4096                                                      */
+    int32_t max_pages;         /* pages of one slot                                                        */
+} aion_kv8;
+
+/* Element types of the rows that go in and come out. */
+enum { AION_F32 = 0, AION_F16 = 1, AION_BF16 = 2 };
+
+/* Allocates a cache of the shape in *shape (its int32 fields; the pointers
+ * are ignored) in one device allocation, empty, and fills *out.  Waits for
+ * the device memory to be cleared. */
+AION_API aion_status aion_kv8_create(const aion_kv8* shape, aion_kv8* out);
+/* Frees a cache that aion_kv8_create made; clears *kv. */
+AION_API aion_status aion_kv8_destroy(aion_kv8* kv);
+/* Empties every slot and frees every page. */
+AION_API aion_status aion_kv8_reset(const aion_kv8* kv, void* stream);
+
+/* Makes room for n_new[i] more tokens in slot seqs[i], i < n (n <= 1024):
+ * pos0[i] = the position of the first of them (the slot's length before),
+ * lens[slot] += n_new[i], and the table gets the pages that are missing.  A
+ * last page that is not full and that other slots hold too is replaced by a
+ * copy of its own.  Pages are taken lowest id first, in list order, and an
+ * entry gets all of its pages or none: entry i is refused (pos0[i] = -1, the
+ * slot unchanged) when it needs pages and those that entries 0..i ask for
+ * exceed the free ones, or when its arguments are bad. */
+AION_API aion_status aion_kv8_grow(const aion_kv8* kv, const int32_t* seqs, const int32_t* n_new, int32_t n,
+                                   int32_t* pos0, void* stream);
+/* Slot dst[i] gives up what it holds and shares the pages of the first
+ * keep[i] tokens (keep NULL: all; never more than the slot has) of slot
+ * src[i], i < n (n <= 1024).  A slot that is written must not be read in the
+ * same call (no dst[i] among src). */
+AION_API aion_status aion_kv8_fork(const aion_kv8* kv, const int32_t* src, const int32_t* dst, const int32_t* keep,
+                                   int32_t n, void* stream);
+/* Slot seqs[i] keeps its first keep[i] tokens (keep NULL: none) and gives up
+ * the pages behind them, i < n (n <= 1024). */
+AION_API aion_status aion_kv8_trim(const aion_kv8* kv, const int32_t* seqs, const int32_t* keep, int32_t n,
+                                   void* stream);
+/* Moves pages until the U pages in use are pages 0..U-1: the i-th used page
+ * at or behind U goes to the i-th free page before U; every table follows.
+ * *n_used (device memory, may be NULL) receives U. */
+AION_API aion_status aion_kv8_compact(const aion_kv8* kv, int32_t* n_used, void* stream);
+
+/* Writes the K and V rows of n_tok tokens of n_seq sequences into `layer`.
+ * Sequence i has the rows cu[i] .. cu[i+1]-1 (cu NULL: one row each, n_tok =
+ * n_seq) and they stand at positions pos0[i], pos0[i]+1, ... of slot seqs[i],
+ * which has pages for them (aion_kv8_grow); pos0[i] < 0 skips the sequence.
+ * Rows are [n_kv_heads][head_size] of `type`, k_stride / v_stride elements
+ * apart.  Per page and head the scale is
+ *   s = max|x| / 127                       for a page that starts here,
+ *   s = s0                                 where max|x| / 127 <= s0,
+ *   s = max(max|x| / 127, 1.25 s0)         else, and the page's earlier
+ *                                          values become rint(q (s0 / s)),
+ * in fp32, and q = the integer nearest to x / s (ties to even) within
+ * +-127.  The step of 1.25 bounds what the repeated roundings of one value
+ * add up to at 2.5 scales.  A value that is not finite makes the page's
+ * scale NaN, and so every result that reads the page for that head.  What
+ * the page holds behind the last row written is left as it was. */
+AION_API aion_status aion_kv8_append(const aion_kv8* kv, int32_t layer, const void* k, const void* v, int32_t type,
+                                     int64_t k_stride, int64_t v_stride, const int32_t* seqs, const int32_t* pos0,
+                                     const int32_t* cu, int32_t n_seq, int32_t n_tok, void* stream);
+
+/* The K and V rows at those positions as the cache holds them, q * s rounded
+ * to `type` (k or v may be NULL).  Rows of a skipped sequence or of a page
+ * that is missing are zero; rows from cu[n_seq] on are left as they were. */
+AION_API aion_status aion_kv8_read(const aion_kv8* kv, int32_t layer, void* k, void* v, int32_t type,
+                                   int64_t k_stride, int64_t v_stride, const int32_t* seqs, const int32_t* pos0,
+                                   const int32_t* cu, int32_t n_seq, int32_t n_tok, void* stream);
+
+/* Attention of n_tok query rows over the cache (src/kernel_simd.c:1099-1117
+ * over the pages): the query of row r of sequence i stands at position p =
+ * pos0[i] + r - cu[i] and sees positions 0..p of slot seqs[i]; head h reads
+ * K/V head h / (n_heads / n_kv_heads).  q and out are [n_heads][head_size]
+ * rows of `type`, q_stride / out_stride elements apart, and do not overlap.
+ * scale 0: 1 / sqrt(head_size).  A sequence with pos0[i] < 0 gets zeros;
+ * positions whose page is missing are left out; rows from cu[n_seq] on are
+ * left as they were.  Scores, softmax and sums are exact integer dots of
+ * fixed-point digits (24 bits for fp32 rows, 16 for 16-bit rows, relative to
+ * the largest of a row) joined in fp32; out is rounded once.
+ * `workspace`: aion_kv8_attention_workspace bytes of device memory, 16-byte
+ * aligned, that no other call in flight uses (NULL when that is 0). */
+AION_API aion_status aion_kv8_attention(const aion_kv8* kv, int32_t layer, const void* q, void* out, int32_t type,
+                                        int32_t n_heads, int64_t q_stride, int64_t out_stride, float scale,
+                                        const int32_t* seqs, const int32_t* pos0, const int32_t* cu, int32_t n_seq,
+                                        int32_t n_tok, void* workspace, int64_t workspace_bytes, void* stream);
+/* Workspace bytes of such a call; -1 when the shape is not supported. */
+AION_API int64_t aion_kv8_attention_workspace(const aion_kv8* kv, int32_t n_heads, int32_t n_seq, int32_t n_tok);
+
+/* Waits for `stream`, then reports and clears what the calls enqueued before
+ * it recorded: AION_ERR_ARG (an entry was out of range or a slot appeared
+ * twice), AION_ERR_STATE (a page was missing, or an append met a page that
+ * several slots hold), AION_ERR_OOM (aion_kv8_grow refused an entry for want
+ * of pages); the first of these that applies. */
+AION_API aion_status aion_kv8_status(const aion_kv8* kv, void* stream);
+
+/* ---------------------------------------------------------------------------
  * Checkpoint tools (host)
  * ------------------------------------------------------------------------- */
 
