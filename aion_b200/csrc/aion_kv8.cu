@@ -6,6 +6,8 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <atomic>
+#include <utility>
 
 #include "kv8.h"
 #include "kv8.cuh"
@@ -347,11 +349,37 @@ extern "C" AION_API aion_status aion_kv8_read(const aion_kv8* kv, int32_t layer,
 // ---------------------------------------------------------------------------
 // Attention
 // ---------------------------------------------------------------------------
+// Blocks of k_kv_attention: one an SM with 128-dimension slots, two with 64.
+static int attention_blocks(const aion_kv8* kv) { return sm_count(kv->device) * (kv->head_size <= 64 ? 2 : 1); }
+// Units of at most this many groups of 64 keys go to one block whole: no join
+// launch.
+constexpr int kWholeGroups = 8;
+static bool attention_whole(const aion_kv8* kv) {
+    return (int64_t)kv->max_pages * kv->page_tokens <= kWholeGroups * kKvaT;
+}
+
 extern "C" AION_API int64_t aion_kv8_attention_workspace(const aion_kv8* kv, int32_t n_heads, int32_t n_seq,
                                                          int32_t n_tok) {
     if (check_shape(kv, "aion_kv8_attention_workspace") != AION_OK) return -1;
     if (n_heads < 1 || n_heads % kv->n_kv_heads || n_seq < 0 || n_tok < 0) return -1;
-    return 0;
+    return attention_whole(kv) ? 0 : (int64_t)attention_blocks(kv) * 2 * sizeof(KvPart);
+}
+
+template <typename T, int HDP, int D>
+static cudaError_t launch_attention(const KvAttnArgs& a, int blocks, int dev, cudaStream_t st) {
+    static std::atomic<uint64_t> opted{0};   // devices whose shared-memory limit is raised
+    const uint64_t bit = dev >= 0 && dev < 64 ? 1ull << dev : 0;
+    if (!bit || !(opted.load() & bit)) {
+        const cudaError_t e = cudaFuncSetAttribute(k_kv_attention<T, HDP, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                   KvaSmem<HDP>::kTotal);
+        if (e != cudaSuccess) return e;
+        opted.fetch_or(bit);
+    }
+    k_kv_attention<T, HDP, D><<<blocks, kKvaThreads, KvaSmem<HDP>::kTotal, st>>>(a);
+    cudaError_t e = cudaGetLastError();
+    if (e == cudaSuccess && !a.whole && blocks > 1)
+        e = launch_pdl(k_kv_attention_join<T>, dim3(blocks - 1), dim3(kKvJoinThreads), 0, st, a, blocks);
+    return e;
 }
 
 extern "C" AION_API aion_status aion_kv8_attention(const aion_kv8* kv, int32_t layer, const void* q, void* out,
@@ -393,12 +421,24 @@ extern "C" AION_API aion_status aion_kv8_attention(const aion_kv8* kv, int32_t l
     a.q_stride = q_stride;
     a.out_stride = out_stride;
     a.scale = (scale == 0.0f ? 1.0f / sqrtf((float)kv->head_size) : scale) * 1.4426950408889634f;
-    const dim3 grid(n_tok, (n_heads + kKvAttnThreads / 32 - 1) / (kKvAttnThreads / 32));
+    a.vec_q = vectors(q, q_stride, type);
+    a.vec_out = vectors(out, out_stride, type);
+    a.whole = attention_whole(kv);
+    a.parts = (KvPart*)workspace;
+    const int blocks = attention_blocks(kv);
     const cudaStream_t st = (cudaStream_t)stream;
-    if (type == AION_F32) k_kv_attention<float><<<grid, kKvAttnThreads, 0, st>>>(a);
-    else if (type == AION_F16) k_kv_attention<__half><<<grid, kKvAttnThreads, 0, st>>>(a);
-    else k_kv_attention<__nv_bfloat16><<<grid, kKvAttnThreads, 0, st>>>(a);
-    KV_CUDA(cudaGetLastError());
+    const bool wide = kv->head_size > 64;
+    cudaError_t e;
+    if (type == AION_F32)
+        e = wide ? launch_attention<float, 128, 3>(a, blocks, kv->device, st)
+                 : launch_attention<float, 64, 3>(a, blocks, kv->device, st);
+    else if (type == AION_F16)
+        e = wide ? launch_attention<__half, 128, 2>(a, blocks, kv->device, st)
+                 : launch_attention<__half, 64, 2>(a, blocks, kv->device, st);
+    else
+        e = wide ? launch_attention<__nv_bfloat16, 128, 2>(a, blocks, kv->device, st)
+                 : launch_attention<__nv_bfloat16, 64, 2>(a, blocks, kv->device, st);
+    KV_CUDA(e);
     return AION_OK;
 }
 
