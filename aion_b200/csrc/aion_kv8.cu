@@ -12,6 +12,7 @@
 #include "kv8.h"
 #include "kv8.cuh"
 #include "kv8_attention.cuh"
+#include "kv8_prompt.cuh"
 
 using namespace aion;
 
@@ -349,6 +350,11 @@ extern "C" AION_API aion_status aion_kv8_read(const aion_kv8* kv, int32_t layer,
 // ---------------------------------------------------------------------------
 // Attention
 // ---------------------------------------------------------------------------
+// Rows of a K/V head (tokens x query heads) from which a sequence, on average,
+// goes to the tiles of 128 rows.
+constexpr int kTileRows = 32;
+static bool attention_tiles(int n_seq, int n_tok, int group) { return (int64_t)n_tok * group >= (int64_t)kTileRows * n_seq; }
+
 // Blocks of k_kv_attention: one an SM with 128-dimension slots, two with 64.
 static int attention_blocks(const aion_kv8* kv) { return sm_count(kv->device) * (kv->head_size <= 64 ? 2 : 1); }
 // Units of at most this many groups of 64 keys go to one block whole: no join
@@ -362,6 +368,7 @@ extern "C" AION_API int64_t aion_kv8_attention_workspace(const aion_kv8* kv, int
                                                          int32_t n_tok) {
     if (check_shape(kv, "aion_kv8_attention_workspace") != AION_OK) return -1;
     if (n_heads < 1 || n_heads % kv->n_kv_heads || n_seq < 0 || n_tok < 0) return -1;
+    if (attention_tiles(n_seq, n_tok, n_heads / kv->n_kv_heads)) return 0;
     return attention_whole(kv) ? 0 : (int64_t)attention_blocks(kv) * 2 * sizeof(KvPart);
 }
 
@@ -382,6 +389,21 @@ static cudaError_t launch_attention(const KvAttnArgs& a, int blocks, int dev, cu
     return e;
 }
 
+template <typename T, int NQ>
+static cudaError_t launch_prompt(const KvAttnArgs& a, int dev, cudaStream_t st) {
+    static std::atomic<uint64_t> opted{0};
+    const uint64_t bit = dev >= 0 && dev < 64 ? 1ull << dev : 0;
+    if (!bit || !(opted.load() & bit)) {
+        const cudaError_t e =
+            cudaFuncSetAttribute(k_kv_prompt<T, NQ>, cudaFuncAttributeMaxDynamicSharedMemorySize, kKvpSmem);
+        if (e != cudaSuccess) return e;
+        opted.fetch_or(bit);
+    }
+    const int64_t places = (int64_t)a.r.n_tok * a.group / (128 * NQ) + a.r.n_seq;
+    k_kv_prompt<T, NQ><<<dim3((unsigned)places, a.c.nkv), kKvpThreads, kKvpSmem, st>>>(a);
+    return cudaGetLastError();
+}
+
 extern "C" AION_API aion_status aion_kv8_attention(const aion_kv8* kv, int32_t layer, const void* q, void* out,
                                                    int32_t type, int32_t n_heads, int64_t q_stride, int64_t out_stride,
                                                    float scale, const int32_t* seqs, const int32_t* pos0,
@@ -390,8 +412,8 @@ extern "C" AION_API aion_status aion_kv8_attention(const aion_kv8* kv, int32_t l
     const char* what = "aion_kv8_attention";
     aion_status s = check_rows(kv, layer, type, seqs, pos0, cu, n_seq, n_tok, what);
     if (s != AION_OK) return s;
-    if (n_heads < 1 || n_heads % kv->n_kv_heads || n_heads > 65535) {
-        aion_thread_error("%s: %d query heads for %d K/V heads", what, n_heads, kv->n_kv_heads);
+    if (n_heads < 1 || n_heads % kv->n_kv_heads || (int64_t)n_tok * (n_heads / kv->n_kv_heads) > (1 << 30)) {
+        aion_thread_error("%s: %d query heads for %d K/V heads, %d rows", what, n_heads, kv->n_kv_heads, n_tok);
         return AION_ERR_SHAPE;
     }
     const int64_t width = (int64_t)n_heads * kv->head_size;
@@ -425,8 +447,14 @@ extern "C" AION_API aion_status aion_kv8_attention(const aion_kv8* kv, int32_t l
     a.vec_out = vectors(out, out_stride, type);
     a.whole = attention_whole(kv);
     a.parts = (KvPart*)workspace;
-    const int blocks = attention_blocks(kv);
     const cudaStream_t st = (cudaStream_t)stream;
+    if (attention_tiles(n_seq, n_tok, a.group)) {
+        if (type == AION_F32) KV_CUDA((launch_prompt<float, 1>(a, kv->device, st)));
+        else if (type == AION_F16) KV_CUDA((launch_prompt<__half, 2>(a, kv->device, st)));
+        else KV_CUDA((launch_prompt<__nv_bfloat16, 2>(a, kv->device, st)));
+        return AION_OK;
+    }
+    const int blocks = attention_blocks(kv);
     const bool wide = kv->head_size > 64;
     cudaError_t e;
     if (type == AION_F32)
@@ -453,8 +481,9 @@ extern "C" AION_API aion_status aion_kv8_status(const aion_kv8* kv, void* stream
     KV_CUDA(cudaMemsetAsync(kv->work, 0, 4, (cudaStream_t)stream));
     KV_CUDA(cudaStreamSynchronize((cudaStream_t)stream));
     if (!word) return AION_OK;
-    aion_thread_error("%s:%s%s%s", what, word & KV_BAD_ARG ? " an entry was out of range or a slot appeared twice;" : "",
+    aion_thread_error("%s:%s%s%s%s", what, word & KV_TIMEOUT ? " a bounded device-side wait gave up: its result is invalid;" : "",
+                      word & KV_BAD_ARG ? " an entry was out of range or a slot appeared twice;" : "",
                       word & KV_BAD_PAGE ? " a page was missing, or an append met a page that is not its slot's alone;" : "",
                       word & KV_NO_PAGES ? " not enough free pages for an entry of aion_kv8_grow;" : "");
-    return word & KV_BAD_ARG ? AION_ERR_ARG : word & KV_BAD_PAGE ? AION_ERR_STATE : AION_ERR_OOM;
+    return word & KV_TIMEOUT ? AION_ERR_TIMEOUT : word & KV_BAD_ARG ? AION_ERR_ARG : word & KV_BAD_PAGE ? AION_ERR_STATE : AION_ERR_OOM;
 }

@@ -27,7 +27,7 @@
 #include <cuda_bf16.h>
 #include <stdint.h>
 
-#include "common.cuh"
+#include "tcgen05.cuh"
 
 namespace aion {
 
@@ -40,13 +40,6 @@ constexpr int kGemmStageBytes = kGemmABytes + kGemmBBytes;
 constexpr int kGemmSmem = kGemmStages * kGemmStageBytes + 1024;   // + room to align to 1024
 constexpr uint32_t kGemmWaitLimit = 1u << 26;
 
-// UMMA shared-memory matrix descriptor, K-major with the 128-byte swizzle:
-// rows of 128 bytes, 8-row groups 1024 bytes apart (SBO), version 1.
-__device__ __forceinline__ uint64_t umma_desc_sw128(uint32_t saddr) {
-    return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) |
-           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
-}
-
 // Instruction descriptor: bf16 A and B (K-major), fp32 D, M 128, N 256.
 constexpr uint32_t kGemmIdesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(kGemmBN >> 3) << 17) |
                                 ((uint32_t)(kGemmBM >> 4) << 24);
@@ -56,36 +49,6 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map
         "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
         ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar)
         : "memory");
-}
-
-__device__ __forceinline__ void umma_bf16(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
-                                          uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}"
-        ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(0), "r"(0), "r"(0), "r"(0)
-        : "memory");
-}
-
-__device__ __forceinline__ void umma_commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
-                 : "memory");
-}
-
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
-    uint32_t r[16];
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(taddr));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-    for (int i = 0; i < 16; i++) v[i] = __uint_as_float(r[i]);
 }
 
 constexpr int kGemmGroupM = 16;   // row tiles per rasterisation group
@@ -193,7 +156,7 @@ k_gemm_bf16_tn(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                 const uint64_t adesc = umma_desc_sw128(sa), bdesc = umma_desc_sw128(sa + kGemmABytes);
 #pragma unroll
                 for (int k = 0; k < kGemmBK / 16; k++)   // 32 bytes of K per step inside the swizzle atom
-                    umma_bf16(acc, adesc + 2 * k, bdesc + 2 * k, kGemmIdesc, (kb | k) != 0);
+                    umma_f16(acc, adesc + 2 * k, bdesc + 2 * k, kGemmIdesc, (kb | k) != 0);
                 umma_commit(smem_addr(&empty_bar[s]));
             }
             if (!ok) break;

@@ -16,7 +16,7 @@ constexpr int kKvMaxList = 1024;    // entries of one page call: one thread each
 constexpr int kKvMaxHead = 128;
 
 // Bits of the status word (work[0]).
-enum KvStatus : int32_t { KV_NO_PAGES = 1, KV_BAD_ARG = 2, KV_BAD_PAGE = 4 };
+enum KvStatus : int32_t { KV_NO_PAGES = 1, KV_BAD_ARG = 2, KV_BAD_PAGE = 4, KV_TIMEOUT = 8 };
 
 // The cache as kernels take it (aion_kv8 of include/aion.h).
 struct KvView {

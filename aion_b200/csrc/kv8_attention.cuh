@@ -57,6 +57,13 @@ struct KvAttnArgs {
 // ---------------------------------------------------------------------------
 constexpr int kKvaWarps = 8, kKvaThreads = 32 * kKvaWarps, kKvaT = 64, kKvaRows = 8;
 
+// 2^x to about 2^-22; 0 below the normal range.
+__device__ __forceinline__ float kv_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 // Softmax state of one unit over a stretch of its keys.
 struct alignas(16) KvPart {
     long long begin, end, at;    // the unit's groups in the line; the block's first group
@@ -513,8 +520,8 @@ __global__ void __launch_bounds__(kKvaThreads, HDP == 64 ? 2 : 1) k_kv_attention
                 mg[e] = fmaxf(mg[e], __shfl_xor_sync(0xffffffffu, mg[e], 8));
                 mg[e] = fmaxf(mg[e], __shfl_xor_sync(0xffffffffu, mg[e], 16));
                 const float mn = fmaxf(m[e], mg[e]);
-                alpha[e] = m[e] == -INFINITY ? 0.0f : exp2f(m[e] - mn);
-                wt[e] = mg[e] == -INFINITY ? 0.0f : exp2f(mg[e] - mn);
+                alpha[e] = m[e] == -INFINITY ? 0.0f : kv_exp2(m[e] - mn);
+                wt[e] = mg[e] == -INFINITY ? 0.0f : kv_exp2(mg[e] - mn);
                 m[e] = mn;
             }
             uint32_t* fx = reinterpret_cast<uint32_t*>(ks);   // [row][68]: the K slot is read
@@ -526,7 +533,7 @@ __global__ void __launch_bounds__(kKvaThreads, HDP == 64 ? 2 : 1) k_kv_attention
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     const bool none = p[j][e] == -INFINITY;
-                    const float w = none ? 0.0f : exp2f(p[j][e] - mg[e & 1]);
+                    const float w = none ? 0.0f : kv_exp2(p[j][e] - mg[e & 1]);
                     sum[e & 1] += !none && vs[j] != vs[j] ? vs[j] : w;   // a NaN scale reaches the rows that see it
                     fx[(2 * t + (e & 1)) * 68 + 16 * j + g + 8 * (e >> 1)] = __float2uint_rn(w * ratio);
                 }
@@ -647,7 +654,7 @@ __global__ void __launch_bounds__(kKvaThreads, HDP == 64 ? 2 : 1) k_kv_attention
             for (int i = first; i < 2 * kKvaWarps; i++) {
                 if (!info[i].valid || info[i].begin != f.begin) continue;
                 const float* p = piece(i);
-                const float pm = p[kKvaRows * HDP + r], wgt = pm == -INFINITY ? 0.0f : exp2f(pm - mx);
+                const float pm = p[kKvaRows * HDP + r], wgt = pm == -INFINITY ? 0.0f : kv_exp2(pm - mx);
                 ls += wgt * p[kKvaRows * HDP + kKvaRows + r];
 #pragma unroll
                 for (int e = 0; e < HDP / 32; e++) os[e] += wgt * p[r * HDP + (HDP / 32) * lane + e];
@@ -694,7 +701,7 @@ __global__ void __launch_bounds__(kKvJoinThreads) k_kv_attention_join(const KvAt
         float4 os = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         for (int i = b - 1; i < end; i++) {
             const KvPart* p = i < b ? head : a.parts + 2 * (size_t)i;
-            const float pm = p->m[r], wgt = pm == -INFINITY ? 0.0f : exp2f(pm - mx);
+            const float pm = p->m[r], wgt = pm == -INFINITY ? 0.0f : kv_exp2(pm - mx);
             const float4 x = *reinterpret_cast<const float4*>(&p->o[r][4 * lane]);
             ls += wgt * p->l[r];
             os.x += wgt * x.x;

@@ -1,0 +1,562 @@
+// Attention over the 8-bit paged K/V cache (kv8.cuh) for many query rows a
+// sequence: prompts and chunks of prompts, on the 5th-generation tensor cores.
+#pragma once
+
+#include <type_traits>
+
+#include "kv8_attention.cuh"
+#include "tcgen05.cuh"
+
+namespace aion {
+
+// ---------------------------------------------------------------------------
+// A block takes one K/V head and 256 rows (two tiles of 128; one of 128 for
+// fp32 rows) of a sequence: the rows of a K/V head are its tokens times the
+// query heads that read it, so grouped heads share every key.  Keys come in
+// tiles of 128:
+//   warps 0-3, 4-7   softmax of row tile 0, 1: one thread a row;
+//   warps 8-11       bring K and V from int8 to fp16, which holds each value
+//                    exactly, into 128-byte-swizzled shared memory, V
+//                    transposed (tokens contiguous);
+//   warp 12          one thread issues tcgen05.mma (kind::f16, M 128):
+//                    S = Q K^T, then O += P V with P read from TMEM.
+// TMEM, 128 columns each: S of tile 0 | S of tile 1 | O of tile 0 | O of tile
+// 1, P in the columns of its own S; fp32 rows: S of even key tiles | P | O | S
+// of odd key tiles.  S of the next key tile overwrites P of this one only
+// after the MMAs that read it have completed (pv_done): nothing else orders
+// two MMAs of different accumulators.
+//
+// Arithmetic.  fp16 queries are taken as they are; bf16 and fp32 ones are
+// scaled by a power of two per row so that the largest is below 2^15 (a bf16
+// value then is an fp16 value, but for parts 2^-39 of the largest), and fp32
+// ones are split into two fp16 terms (22 bits), each with its own MMA.
+// Products of fp16 values are exact in the MMA and summed in fp32.
+// P = 2^(s - m) * 2^7 * vscale / vref in fp16 (fp32 rows: two terms, 22
+// bits), where vref is the largest V scale of the sequence's pages for this
+// head, so that pages of different scales add up in one accumulator; its sum
+// l is kept in fp32 from the unrounded weights.  m is a running reference: it
+// follows the row's maximum only when that has grown by more than 8 (a factor
+// of 2^8, and P stays below 2^15), which leaves O untouched for most tiles.
+// ---------------------------------------------------------------------------
+constexpr int kKvpThreads = 416, kKvpTile = 128;
+constexpr int kKvpBlock = 128 * 128 * 2;   // a 128 x 128 fp16 operand: two 128-byte-wide halves
+constexpr int kKvpSmem = 6 * kKvpBlock + 1024;
+constexpr uint32_t kKvpWaitLimit = 1u << 20;
+
+__device__ __forceinline__ uint32_t kvp_idesc(int n) {   // fp16 A and B (K-major), fp32 D, M 128
+    return (1u << 4) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
+}
+// D (TMEM) += A (TMEM: fp16 pairs, K along the columns) B (shared memory).
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n\t}"
+        ::"r"(d), "r"(a), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(0), "r"(0), "r"(0), "r"(0)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+        "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
+        "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"r"(r[0]),
+        "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
+        "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
+        "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]),
+        "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void fence_smem_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+// Four int8 values of a word as two fp16 pairs: 1024 + (value + 128) is the
+// fp16 pattern 0x6400 | (value ^ 0x80), and taking 1152 away is exact.
+__device__ __forceinline__ uint2 int8x4_to_half(uint32_t w) {
+    const uint32_t u = w ^ 0x80808080u, magic = 0x64646464u, off = 0x64806480u;
+    uint32_t a = __byte_perm(u, magic, 0x4140), b = __byte_perm(u, magic, 0x4342);
+    const __half2 o = *reinterpret_cast<const __half2*>(&off);
+    const __half2 x = __hsub2(*reinterpret_cast<__half2*>(&a), o), y = __hsub2(*reinterpret_cast<__half2*>(&b), o);
+    return make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+}
+// Byte offset of 16-byte piece ch (8 values) of a row of 128 fp16 values.
+__device__ __forceinline__ int kvp_piece(int row, int ch) {
+    return (ch >> 3) * (kKvpBlock / 2) + row * 128 + (((ch & 7) ^ (row & 7)) << 4);
+}
+
+// Wait that gives up when the block has failed or after kKvpWaitLimit polls.
+__device__ __forceinline__ bool kvp_wait(uint64_t* bar, uint32_t parity, volatile int* fail) {
+    const uint32_t b = smem_addr(bar);
+    for (uint32_t i = 0; i < kKvpWaitLimit; i++) {
+        if (mbar_try_wait(b, parity)) return true;
+        if ((i & 255u) == 255u && *fail) return false;
+    }
+    *fail = 1;
+    return false;
+}
+
+// What the softmax needs to know of a key tile: for each 16 of its keys the
+// scales, and which of them have a page.
+struct KvpMeta {
+    float ks[8], fv[8];   // fv = 2^7 vscale / vref
+    uint32_t live, nan;   // bit j: keys 16 j.. have a page; their V scale is NaN
+};
+
+template <typename T, int NQ>
+__global__ void __launch_bounds__(kKvpThreads, 1) k_kv_prompt(const KvAttnArgs a) {
+    constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;   // fp16 terms of a query and of a weight
+    static_assert(NQ * TERMS == 2, "two query tiles in shared memory");
+    constexpr int ROWS = 128 * NQ;
+    extern __shared__ __align__(1024) unsigned char psm_raw[];
+    __shared__ __align__(8) uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[NQ],
+        pv_done[NQ], done_bar;
+    __shared__ uint32_t s_tmem;
+    __shared__ float s_red[4];
+    __shared__ KvpMeta s_meta[4];
+    __shared__ volatile int s_fail;
+    unsigned char* sm = psm_raw + ((1024u - (smem_addr(psm_raw) & 1023u)) & 1023u);
+    unsigned char *qs = sm, *kst = sm + 2 * kKvpBlock, *vst = sm + 4 * kKvpBlock;
+    const KvView& c = a.c;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    // ---- the block's rows
+    const int h = blockIdx.y, place = gridDim.x - 1 - blockIdx.x;   // late rows, which see most, first
+    int blk = 0, s = 0;
+    {
+        int lo = 0, hi = a.r.n_seq - 1;   // places of a sequence: (rows before it / ROWS) + its number, on
+        auto first = [&](int i) { return (int)((long long)a.r.begin(i) * a.group / ROWS) + i; };
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (first(mid) <= place) lo = mid;
+            else hi = mid - 1;
+        }
+        s = lo;
+        blk = place - first(lo);
+    }
+    const KvSeq q = kv_seq(a, s);
+    const long long total = (long long)q.cnt * a.group;
+    if (blk < 0 || (long long)blk * ROWS >= total) return;
+    const int row0 = blk * ROWS;
+    const int rows = (int)min((long long)ROWS, total - row0);
+    const int nq = rows > 128 ? 2 : 1;
+    int nt[NQ];   // key tiles of each row tile: up to its last row's position
+#pragma unroll
+    for (int i = 0; i < NQ; i++) {
+        const int last = min(row0 + 128 * (i + 1), row0 + rows) - 1;
+        const long long seen = min((long long)q.p0 + last / a.group, (long long)q.len - 1) + 1;
+        nt[i] = i < nq ? (int)((seen + kKvpTile - 1) / kKvpTile) : 0;
+        if (q.len == 0) nt[i] = 0;
+    }
+    const int ntiles = nt[nq - 1];
+
+    if (threadIdx.x == 0) {
+        mbar_init(smem_addr(&q_full), 4 * NQ);
+        for (int i = 0; i < 2; i++) {
+            mbar_init(smem_addr(&k_full[i]), 4);
+            mbar_init(smem_addr(&k_empty[i]), 1);
+            mbar_init(smem_addr(&v_full[i]), 4);
+            mbar_init(smem_addr(&v_empty[i]), 1);
+            mbar_init(smem_addr(&s_full[i]), 1);
+        }
+        for (int i = 0; i < NQ; i++) {
+            mbar_init(smem_addr(&p_full[i]), 4);
+            mbar_init(smem_addr(&pv_done[i]), 1);
+        }
+        mbar_init(smem_addr(&done_bar), 1);
+        s_fail = 0;
+        fence_mbar_init();
+    }
+    if (warp == 12) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&s_tmem)), "r"(512)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    // ---- the largest V scale of the pages in sight
+    float vref = 0.0f;
+    const int32_t* table = c.tables + (size_t)(q.len ? q.slot : 0) * c.max_pages;
+    if (warp >= 8 && warp < 12) {
+        const int used = (int)(((long long)ntiles * kKvpTile < q.len ? (long long)ntiles * kKvpTile : q.len) + c.page - 1) >>
+                         c.page_log;
+        for (int i = threadIdx.x - 256; i < used; i += 128) {
+            const int page = table[i];
+            if (page >= 0 && page < c.n_pages)
+                vref = fmaxf(vref, c.v_scale[((long long)a.layer * c.n_pages + page) * c.nkv + h]);   // without a NaN
+        }
+        vref = warp_max(vref);
+        if (lane == 0) s_red[warp - 8] = vref;
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = s_tmem;
+    vref = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
+
+    if (warp < 4 * NQ) {
+        // ================= softmax: thread = row =================
+        const int tile = warp >> 2, r = threadIdx.x & 127, i = row0 + 128 * tile + r;
+        const int tok = i / a.group, head = h * a.group + (i - tok * a.group);
+        const bool live_row = i < total && 128 * tile + r < rows;
+        const int lim = live_row ? (int)min((long long)q.p0 + tok, (long long)q.len - 1) : -1;
+        // the query row to shared memory
+        float up = 1.0f, rs;
+        bool bad = false;
+        {
+            const T* src = (const T*)a.q + (q.t0 + tok) * a.q_stride + (long long)head * c.hd;
+            const float sign = a.scale < 0.0f ? -1.0f : 1.0f;
+            float top = 0.0f;
+            if (live_row) {
+                for (int d = 0; d < c.hd; d += 16) {
+                    float x[16];
+                    load16(src + d, a.vec_q, x);
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        const float b = fabsf(x[e]);
+                        bad = bad || !(b <= 3.402823466e38f);
+                        top = fmaxf(top, b);
+                    }
+                }
+                if (!std::is_same<T, __half>::value) {   // the largest to 2^14..2^15
+                    const int e = top > 0.0f && !bad ? max(min(14 - ilogbf(top), 126), -126) : 0;
+                    up = __int_as_float((127 + e) << 23);
+                }
+            }
+            rs = bad ? __int_as_float(0x7FC00000) : fabsf(a.scale) / up;
+            for (int d = 0; d < c.hd; d += 16) {
+                float x[16];
+                if (live_row && !bad) {
+                    load16(src + d, a.vec_q, x);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 16; e++) x[e] = 0.0f;
+                }
+                uint32_t hi[8], lo[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const float x0 = x[2 * e] * up * sign, x1 = x[2 * e + 1] * up * sign;
+                    hi[e] = half2_bits(x0, x1);
+                    if (TERMS == 2) {
+                        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi[e]));
+                        lo[e] = half2_bits(x0 - f.x, x1 - f.y);
+                    }
+                }
+#pragma unroll
+                for (int p = 0; p < 2; p++) {
+                    unsigned char* to = qs + tile * kKvpBlock + kvp_piece(r, d / 8 + p);
+                    *reinterpret_cast<uint4*>(to) = make_uint4(hi[4 * p], hi[4 * p + 1], hi[4 * p + 2], hi[4 * p + 3]);
+                    if (TERMS == 2)
+                        *reinterpret_cast<uint4*>(to + kKvpBlock) =
+                            make_uint4(lo[4 * p], lo[4 * p + 1], lo[4 * p + 2], lo[4 * p + 3]);
+                }
+            }
+        }
+        fence_smem_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_addr(&q_full));
+
+        const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
+        const uint32_t to = tmem + lanes + 256 + 128 * tile;                              // O
+        const uint32_t tp = tmem + lanes + (TERMS == 2 ? 128 : 128 * tile);               // P
+        float m = -INFINITY, l = 0.0f;
+        const int mine = nt[NQ == 2 ? tile : 0];
+        bool ok = true;
+        for (int j = 0; j < mine; j++) {
+            const int sb = TERMS == 2 ? j & 1 : tile;   // which S
+            if (!__all_sync(0xffffffffu, kvp_wait(&s_full[sb], (TERMS == 2 ? j >> 1 : j) & 1, &s_fail))) {
+                ok = false;
+                break;
+            }
+            tc_fence_after();
+            const uint32_t ts = tmem + lanes + (TERMS == 2 ? 384 * sb : 128 * tile);
+            const KvpMeta& me = s_meta[j & 3];   // written before the tile's K was announced
+            const int key0 = j * kKvpTile;
+            const bool edge = key0 + kKvpTile - 1 > lim || me.live != 0xFFu;   // some key is not seen
+            float mt = -INFINITY;
+#pragma unroll
+            for (int b = 0; b < 4; b++) {
+                uint32_t x[32];
+                tmem_ld32(ts + 32 * b, x);
+#pragma unroll
+                for (int e2 = 0; e2 < 2; e2++) {
+                    float mx = -INFINITY;
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        const float v = __uint_as_float(x[16 * e2 + e]);
+                        const bool see = !edge || (key0 + 32 * b + 16 * e2 + e <= lim && ((me.live >> (2 * b + e2)) & 1));
+                        mx = see ? fmaxf(mx, v) : mx;
+                    }
+                    mt = fmaxf(mt, mx * (me.ks[2 * b + e2] * rs));   // fmaxf leaves a NaN out: m is never one
+                }
+            }
+            // P and O of the tile before are done with (16-bit rows: as this S came after them)
+            if (TERMS == 2 && j > 0 && !__all_sync(0xffffffffu, kvp_wait(&pv_done[0], (j - 1) & 1, &s_fail))) {
+                ok = false;
+                break;
+            }
+            tc_fence_after();
+            // the reference follows the maximum in steps of more than 8
+            const bool grow = mt > m + 8.0f;
+            if (__any_sync(0xffffffffu, grow)) {
+                const float f = grow ? (m == -INFINITY ? 0.0f : kv_exp2(m - mt)) : 1.0f;
+                if (grow) m = mt;
+                l *= f;
+                if (j > 0) {
+                    for (int b = 0; b < c.hd; b += 32) {
+                        uint32_t x[32];
+                        tmem_ld32(to + b, x);
+#pragma unroll
+                        for (int e = 0; e < 32; e++) x[e] = __float_as_uint(__uint_as_float(x[e]) * f);
+                        tmem_st32(to + b, x);
+                    }
+                }
+            }
+            const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+            for (int b = 0; b < 4; b++) {
+                uint32_t x[32], p[16], pl[16];
+                tmem_ld32(ts + 32 * b, x);
+#pragma unroll
+                for (int e2 = 0; e2 < 2; e2++) {
+                    const float cs = me.ks[2 * b + e2] * rs, fv = me.fv[2 * b + e2];
+                    const bool here = (me.live >> (2 * b + e2)) & 1;
+                    if (((me.nan >> (2 * b + e2)) & 1) && here && key0 + 32 * b + 16 * e2 <= lim) l = __int_as_float(0x7FC00000);
+#pragma unroll
+                    for (int e = 0; e < 16; e += 2) {
+                        float w[2];
+#pragma unroll
+                        for (int k = 0; k < 2; k++) {
+                            const bool see = !edge || (key0 + 32 * b + 16 * e2 + e + k <= lim && here);
+                            w[k] = see ? kv_exp2(fmaf(__uint_as_float(x[16 * e2 + e + k]), cs, -ref)) : 0.0f;
+                            l += w[k];
+                            w[k] *= fv;
+                        }
+                        p[8 * e2 + e / 2] = half2_bits(w[0], w[1]);
+                        if (TERMS == 2) {
+                            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&p[8 * e2 + e / 2]));
+                            pl[8 * e2 + e / 2] = half2_bits(w[0] - f.x, w[1] - f.y);
+                        }
+                    }
+                }
+                tmem_st16(tp + 16 * b, p);
+                if (TERMS == 2) tmem_st16(tp + 64 + 16 * b, pl);
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_addr(&p_full[tile]));
+        }
+        // ---- out = O vref / (2^7 l)
+        if (ok && mine > 0) ok = __all_sync(0xffffffffu, kvp_wait(&pv_done[tile], (mine - 1) & 1, &s_fail));
+        tc_fence_after();
+        if (ok && (tile < nq)) {
+            const float f = l == 0.0f ? 0.0f : vref * 0.0078125f / l;
+            T* dst = (T*)a.out + (q.t0 + tok) * a.out_stride + (long long)head * c.hd;
+            for (int b = 0; b < c.hd; b += 16) {
+                float x[16];
+                if (mine > 0) {
+                    tmem_ld16(to + b, x);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 16; e++) x[e] = 0.0f;
+                }
+#pragma unroll
+                for (int e = 0; e < 16; e++) x[e] = l == 0.0f ? 0.0f : x[e] * f;
+                if (live_row) store16(dst + b, a.vec_out, x);
+            }
+        }
+        tc_fence_before();
+    } else if (warp >= 8 && warp < 12) {
+        // ================= K and V to fp16 =================
+        const int w4 = warp - 8, id = threadIdx.x - 256, cpr = c.hd / 16;
+        const int8_t *kp = c.k + a.layer * c.plane(), *vp = c.v + a.layer * c.plane();
+        const int tg = (lane & 7) + 8 * (w4 & 1), vc = (lane >> 3) + 4 * (w4 >> 1);   // V: 8 tokens, 16 dimensions
+        const int kr = id >> 3, kc = id & 7;                                            // K: row of 16, 16 dimensions
+        auto look = [&](int j) {   // lane e < 8: the page of keys 128 j + 16 e..
+            const int pos = j * kKvpTile + 16 * (lane & 7);
+            int page = -1;
+            if (j < ntiles && pos < q.len) {
+                page = table[pos >> c.page_log];
+                if (page < 0 || page >= c.n_pages) {
+                    kv_flag(c, KV_BAD_PAGE);
+                    page = -1;
+                }
+            }
+            return page;
+        };
+        auto load_k = [&](int j, int page, uint4 (&x)[8]) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const int pg = __shfl_sync(0xffffffffu, page, e);
+                x[e] = make_uint4(0, 0, 0, 0);
+                if (pg >= 0 && kc < cpr)
+                    x[e] = *reinterpret_cast<const uint4*>(
+                        kp + (((long long)pg * c.nkv + h) * c.page + ((j * kKvpTile + 16 * e) & (c.page - 1)) + kr) * c.hd + 16 * kc);
+            }
+        };
+        auto load_v = [&](int j, int page, uint4 (&x)[8]) {
+            const int pg = __shfl_sync(0xffffffffu, page, tg >> 1);
+            const int8_t* src = vp + (((long long)pg * c.nkv + h) * c.page + ((j * kKvpTile + 8 * tg) & (c.page - 1))) * c.hd + 16 * vc;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                x[e] = make_uint4(0, 0, 0, 0);
+                if (pg >= 0 && vc < cpr) x[e] = *reinterpret_cast<const uint4*>(src + e * c.hd);
+            }
+        };
+        uint4 kx[8], vx[8];
+        int page = look(0);
+        load_k(0, page, kx);
+        load_v(0, page, vx);
+        for (int j = 0; j < ntiles; j++) {
+            const int st = j & 1;
+            if (j >= 2 && !kvp_wait(&k_empty[st], ((j >> 1) - 1) & 1, &s_fail)) break;
+            unsigned char* kb = kst + st * kKvpBlock;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const int row = 16 * e + kr;
+                const uint2 p0 = int8x4_to_half(kx[e].x), p1 = int8x4_to_half(kx[e].y), p2 = int8x4_to_half(kx[e].z),
+                            p3 = int8x4_to_half(kx[e].w);
+                if (kc < cpr) {
+                    *reinterpret_cast<uint4*>(kb + kvp_piece(row, 2 * kc)) = make_uint4(p0.x, p0.y, p1.x, p1.y);
+                    *reinterpret_cast<uint4*>(kb + kvp_piece(row, 2 * kc + 1)) = make_uint4(p2.x, p2.y, p3.x, p3.y);
+                }
+            }
+            // Words of tile j - 4: its softmax was over before S of tile j - 2 was issued, and k_empty says that was.
+            if (w4 == 0) {
+                float ks = 0.0f, vs = 0.0f;
+                if (lane < 8 && page >= 0) {
+                    ks = c.k_scale[((long long)a.layer * c.n_pages + page) * c.nkv + h];
+                    vs = c.v_scale[((long long)a.layer * c.n_pages + page) * c.nkv + h];
+                }
+                const unsigned live = __ballot_sync(0xffffffffu, lane < 8 && page >= 0);
+                const unsigned nan = __ballot_sync(0xffffffffu, vs != vs);
+                if (lane < 8) {
+                    s_meta[j & 3].ks[lane] = ks;
+                    s_meta[j & 3].fv[lane] = vref > 0.0f && vs == vs ? vs / vref * 128.0f : 0.0f;
+                }
+                if (lane == 0) {
+                    s_meta[j & 3].live = live;
+                    s_meta[j & 3].nan = nan;
+                }
+            }
+            fence_smem_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_addr(&k_full[st]));
+            const int next = look(j + 1);
+            load_k(j + 1, next, kx);
+            if (j >= 2 && !kvp_wait(&v_empty[st], ((j >> 1) - 1) & 1, &s_fail)) break;
+            unsigned char* vb = vst + st * kKvpBlock;
+            if (vc < cpr) {
+#pragma unroll
+                for (int w = 0; w < 4; w++) {
+                    uint32_t lo[4], hi[4];   // dimension 16 vc + 4 w + d: tokens 0..3, 4..7 of the eight
+                    const uint32_t* x = reinterpret_cast<const uint32_t*>(vx) + w;
+                    transpose4(x[0], x[4], x[8], x[12], lo);
+                    transpose4(x[16], x[20], x[24], x[28], hi);
+#pragma unroll
+                    for (int d = 0; d < 4; d++) {
+                        const uint2 p0 = int8x4_to_half(lo[d]), p1 = int8x4_to_half(hi[d]);
+                        *reinterpret_cast<uint4*>(vb + kvp_piece(16 * vc + 4 * w + d, tg)) = make_uint4(p0.x, p0.y, p1.x, p1.y);
+                    }
+                }
+            }
+            fence_smem_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_addr(&v_full[st]));
+            load_v(j + 1, next, vx);
+            page = next;
+        }
+    } else if (warp == 12 && lane == 0) {
+        // ================= MMA issue =================
+        const uint32_t id_s = kvp_idesc(kKvpTile), id_o = kvp_idesc(c.hd);
+        auto scores = [&](int j, int t) {
+            const uint32_t kb = smem_addr(kst + (j & 1) * kKvpBlock);
+            const int sb = TERMS == 2 ? j & 1 : t;
+            const uint32_t d = tmem + (TERMS == 2 ? 384 * sb : 128 * t);
+#pragma unroll
+            for (int term = 0; term < TERMS; term++) {
+                const uint32_t qb = smem_addr(qs + (t + term) * kKvpBlock);
+                for (int k = 0; k < c.hd / 16; k++) {
+                    const uint32_t off = (uint32_t)(k >> 2) * (kKvpBlock / 2);
+                    umma_f16(d, umma_desc_sw128(qb + off) + 2 * (k & 3), umma_desc_sw128(kb + off) + 2 * (k & 3), id_s,
+                              (term | k) != 0);
+                }
+            }
+            umma_commit(smem_addr(&s_full[sb]));
+        };
+        auto values = [&](int j, int t) {
+            const uint32_t vb = smem_addr(vst + (j & 1) * kKvpBlock);
+            const uint32_t p = tmem + (TERMS == 2 ? 128 : 128 * t);
+#pragma unroll
+            for (int term = 0; term < TERMS; term++)
+                for (int k = 0; k < kKvpTile / 16; k++)
+                    umma_ts(tmem + 256 + 128 * t, p + 64 * term + 8 * k,
+                            umma_desc_sw128(vb + (uint32_t)(k >> 2) * (kKvpBlock / 2)) + 2 * (k & 3), id_o, (j | term | k) != 0);
+            umma_commit(smem_addr(&pv_done[t]));
+        };
+        auto wait_k = [&](int j) { return kvp_wait(&k_full[j & 1], (j >> 1) & 1, &s_fail); };
+        bool ok = ntiles == 0 || (kvp_wait(&q_full, 0, &s_fail) && wait_k(0));
+        tc_fence_after();
+        if (ok && ntiles > 0) {
+            for (int t = 0; t < nq; t++)
+                if (nt[NQ == 2 ? t : 0] > 0) scores(0, t);
+            umma_commit(smem_addr(&k_empty[0]));
+        }
+        for (int j = 0; j < ntiles && ok; j++) {
+            const bool more = j + 1 < ntiles;
+            if (more) ok = wait_k(j + 1);
+            tc_fence_after();
+            if (TERMS == 2 && more && ok) {   // S of the next tile goes to the other buffer, read two tiles ago
+                scores(j + 1, 0);
+                umma_commit(smem_addr(&k_empty[(j + 1) & 1]));
+            }
+            ok = ok && kvp_wait(&v_full[j & 1], (j >> 1) & 1, &s_fail);
+            for (int t = 0; t < nq && ok; t++) {
+                const int mine = nt[NQ == 2 ? t : 0];
+                if (j >= mine) continue;
+                ok = kvp_wait(&p_full[t], j & 1, &s_fail);
+                if (!ok) break;
+                tc_fence_after();
+                values(j, t);
+                if (TERMS == 1 && j + 1 < mine) {   // into the columns of the P just read
+                    ok = kvp_wait(&pv_done[t], j & 1, &s_fail);
+                    if (!ok) break;
+                    tc_fence_after();
+                    scores(j + 1, t);
+                }
+            }
+            if (!ok) break;
+            umma_commit(smem_addr(&v_empty[j & 1]));
+            if (TERMS == 1 && more) umma_commit(smem_addr(&k_empty[(j + 1) & 1]));
+        }
+        umma_commit(smem_addr(&done_bar));
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 12) {
+        mbar_wait(smem_addr(&done_bar), 0, kKvpWaitLimit);   // every MMA issued is complete
+        __syncwarp();
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    }
+    if (threadIdx.x == 0 && s_fail) kv_flag(c, KV_TIMEOUT);
+}
+
+}  // namespace aion
