@@ -127,6 +127,13 @@ __device__ __forceinline__ KvSeq kv_seq(const KvAttnArgs& a, int s) {
     return q;
 }
 
+// Records what is wrong with a sequence: a slot that does not exist, positions behind its table.
+__device__ __forceinline__ void kv_vet_seq(const KvAttnArgs& a, const KvSeq& q) {
+    if (q.p0 < 0 || q.cnt == 0) return;
+    if (q.slot < 0 || q.slot >= a.c.max_seqs) kv_flag(a.c, KV_BAD_ARG);
+    else if ((long long)q.p0 + q.cnt > q.len) kv_flag(a.c, KV_BAD_PAGE);
+}
+
 // A place in the line of groups.
 struct KvCursor {
     KvSeq q;
@@ -217,6 +224,7 @@ __global__ void __launch_bounds__(kKvaThreads, HDP == 64 ? 2 : 1) k_kv_attention
     long long mine = 0;
     for (int s = sa; s < sb; s++) {
         const KvSeq q = kv_seq(a, s);
+        if (blockIdx.x == 0) kv_vet_seq(a, q);
         mine += (long long)q.ng * q.nrg * c.nkv;
     }
     long long x = mine;

@@ -18,7 +18,7 @@ namespace aion {
 //   warps 8-11       bring K and V from int8 to fp16, which holds each value
 //                    exactly, into 128-byte-swizzled shared memory, V
 //                    transposed (tokens contiguous);
-//   warp 12          one thread issues tcgen05.mma (kind::f16, M 128):
+//   warp 12          issues tcgen05.mma (kind::f16, M 128):
 //                    S = Q K^T, then O += P V with P read from TMEM.
 // TMEM, 128 columns each: S of tile 0 | S of tile 1 | O of tile 0 | O of tile
 // 1, P in the columns of its own S; fp32 rows: S of even key tiles | P | O | S
@@ -46,25 +46,38 @@ constexpr uint32_t kKvpWaitLimit = 1u << 20;
 __device__ __forceinline__ uint32_t kvp_idesc(int n) {   // fp16 A and B (K-major), fp32 D, M 128
     return (1u << 4) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
 }
-// D (TMEM) += A (TMEM: fp16 pairs, K along the columns) B (shared memory).
-__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n\t}"
-        ::"r"(d), "r"(a), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(0), "r"(0), "r"(0), "r"(0)
-        : "memory");
-}
+// Loads and their wait are one instruction to the compiler: a register that a
+// load is still on its way to cannot be moved or spilled.
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
-        "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]),
+          "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]),
+          "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_ld64(uint32_t taddr, uint32_t (&x)[2][32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%64];\n\t"
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%65];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(x[0][0]), "=r"(x[0][1]), "=r"(x[0][2]), "=r"(x[0][3]), "=r"(x[0][4]), "=r"(x[0][5]), "=r"(x[0][6]),
+          "=r"(x[0][7]), "=r"(x[0][8]), "=r"(x[0][9]), "=r"(x[0][10]), "=r"(x[0][11]), "=r"(x[0][12]),
+          "=r"(x[0][13]), "=r"(x[0][14]), "=r"(x[0][15]), "=r"(x[0][16]), "=r"(x[0][17]), "=r"(x[0][18]),
+          "=r"(x[0][19]), "=r"(x[0][20]), "=r"(x[0][21]), "=r"(x[0][22]), "=r"(x[0][23]), "=r"(x[0][24]),
+          "=r"(x[0][25]), "=r"(x[0][26]), "=r"(x[0][27]), "=r"(x[0][28]), "=r"(x[0][29]), "=r"(x[0][30]),
+          "=r"(x[0][31]), "=r"(x[1][0]), "=r"(x[1][1]), "=r"(x[1][2]), "=r"(x[1][3]), "=r"(x[1][4]),
+          "=r"(x[1][5]), "=r"(x[1][6]), "=r"(x[1][7]), "=r"(x[1][8]), "=r"(x[1][9]), "=r"(x[1][10]),
+          "=r"(x[1][11]), "=r"(x[1][12]), "=r"(x[1][13]), "=r"(x[1][14]), "=r"(x[1][15]), "=r"(x[1][16]),
+          "=r"(x[1][17]), "=r"(x[1][18]), "=r"(x[1][19]), "=r"(x[1][20]), "=r"(x[1][21]), "=r"(x[1][22]),
+          "=r"(x[1][23]), "=r"(x[1][24]), "=r"(x[1][25]), "=r"(x[1][26]), "=r"(x[1][27]), "=r"(x[1][28]),
+          "=r"(x[1][29]), "=r"(x[1][30]), "=r"(x[1][31])
+        : "r"(taddr), "r"(taddr + 32)
+        : "memory");
 }
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
     asm volatile(
@@ -88,6 +101,37 @@ __device__ __forceinline__ void fence_smem_async() { asm volatile("fence.proxy.a
 __device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
+}
+// Two fp32 values in one 64-bit register, for the packed fp32 instructions.
+__device__ __forceinline__ uint64_t f2_pack(float x, float y) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ float2 f2_unpack(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
 }
 // Four int8 values of a word as two fp16 pairs: 1024 + (value + 128) is the
 // fp16 pattern 0x6400 | (value ^ 0x80), and taking 1152 away is exact.
@@ -117,8 +161,8 @@ __device__ __forceinline__ bool kvp_wait(uint64_t* bar, uint32_t parity, volatil
 // What the softmax needs to know of a key tile: for each 16 of its keys the
 // scales, and which of them have a page.
 struct KvpMeta {
-    float ks[8], fv[8];   // fv = 2^7 vscale / vref
-    uint32_t live, nan;   // bit j: keys 16 j.. have a page; their V scale is NaN
+    float ks[8], fv[8];   // fv = 2^7 vscale / vref; ks is positive (1 where the page's values are 0 or NaN)
+    uint32_t live, nan;   // bit j: keys 16 j.. have a page; one of its scales is NaN
 };
 
 template <typename T, int NQ>
@@ -169,6 +213,7 @@ __global__ void __launch_bounds__(kKvpThreads, 1) k_kv_prompt(const KvAttnArgs a
     const int ntiles = nt[nq - 1];
 
     if (threadIdx.x == 0) {
+        kv_vet_seq(a, q);
         mbar_init(smem_addr(&q_full), 4 * NQ);
         for (int i = 0; i < 2; i++) {
             mbar_init(smem_addr(&k_full[i]), 4);
@@ -239,7 +284,7 @@ __global__ void __launch_bounds__(kKvpThreads, 1) k_kv_prompt(const KvAttnArgs a
                     up = __int_as_float((127 + e) << 23);
                 }
             }
-            rs = bad ? __int_as_float(0x7FC00000) : fabsf(a.scale) / up;
+            rs = bad ? 1.0f : fabsf(a.scale) / up;
             for (int d = 0; d < c.hd; d += 16) {
                 float x[16];
                 if (live_row && !bad) {
@@ -275,7 +320,7 @@ __global__ void __launch_bounds__(kKvpThreads, 1) k_kv_prompt(const KvAttnArgs a
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
         const uint32_t to = tmem + lanes + 256 + 128 * tile;                              // O
         const uint32_t tp = tmem + lanes + (TERMS == 2 ? 128 : 128 * tile);               // P
-        float m = -INFINITY, l = 0.0f;
+        float m = -INFINITY, l = bad ? __int_as_float(0x7FC00000) : 0.0f;   // a NaN in l stays and reaches the result
         const int mine = nt[NQ == 2 ? tile : 0];
         bool ok = true;
         for (int j = 0; j < mine; j++) {
@@ -288,22 +333,36 @@ __global__ void __launch_bounds__(kKvpThreads, 1) k_kv_prompt(const KvAttnArgs a
             const uint32_t ts = tmem + lanes + (TERMS == 2 ? 384 * sb : 128 * tile);
             const KvpMeta& me = s_meta[j & 3];   // written before the tile's K was announced
             const int key0 = j * kKvpTile;
-            const bool edge = key0 + kKvpTile - 1 > lim || me.live != 0xFFu;   // some key is not seen
+            // some row of the warp does not see every key of the tile
+            const bool edge = __any_sync(0xffffffffu, key0 + kKvpTile - 1 > lim) || me.live != 0xFFu;
+            auto hide = [&](int b, uint32_t(&v)[32]) {   // -inf at the keys of 32 b.. that are not seen
+                const int n = lim - (key0 + 32 * b) + 1;
+                uint32_t see = n >= 32 ? 0xFFFFFFFFu : n <= 0 ? 0u : (1u << n) - 1u;
+                if (!((me.live >> (2 * b)) & 1)) see &= 0xFFFF0000u;
+                if (!((me.live >> (2 * b + 1)) & 1)) see &= 0xFFFFu;
+#pragma unroll
+                for (int e = 0; e < 32; e++) v[e] = (see >> e) & 1 ? v[e] : 0xFF800000u;
+            };
+            // factors of the scores: never 0, so that -inf stays -inf
+            auto factor = [&](int g) { return fmaxf(me.ks[g] * rs, 1.17549435e-38f); };
+            // ---- the tile's maximum
             float mt = -INFINITY;
+            uint32_t x[2][32];
+#pragma unroll 1
+            for (int b2 = 0; b2 < 4; b2 += 2) {
+                tmem_ld64(ts + 32 * b2, x);
+                if (edge) {
+                    hide(b2, x[0]);
+                    hide(b2 + 1, x[1]);
+                }
 #pragma unroll
-            for (int b = 0; b < 4; b++) {
-                uint32_t x[32];
-                tmem_ld32(ts + 32 * b, x);
+                for (int g = 0; g < 4; g++) {
+                    const uint32_t* v = x[g >> 1] + 16 * (g & 1);
+                    float mx = __uint_as_float(v[0]);
 #pragma unroll
-                for (int e2 = 0; e2 < 2; e2++) {
-                    float mx = -INFINITY;
-#pragma unroll
-                    for (int e = 0; e < 16; e++) {
-                        const float v = __uint_as_float(x[16 * e2 + e]);
-                        const bool see = !edge || (key0 + 32 * b + 16 * e2 + e <= lim && ((me.live >> (2 * b + e2)) & 1));
-                        mx = see ? fmaxf(mx, v) : mx;
-                    }
-                    mt = fmaxf(mt, mx * (me.ks[2 * b + e2] * rs));   // fmaxf leaves a NaN out: m is never one
+                    for (int e = 1; e < 15; e += 2) mx = max3(mx, __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
+                    mx = fmaxf(mx, __uint_as_float(v[15]));
+                    mt = fmaxf(mt, mx * factor(2 * b2 + g));
                 }
             }
             // P and O of the tile before are done with (16-bit rows: as this S came after them)
@@ -319,44 +378,57 @@ __global__ void __launch_bounds__(kKvpThreads, 1) k_kv_prompt(const KvAttnArgs a
                 if (grow) m = mt;
                 l *= f;
                 if (j > 0) {
+#pragma unroll 1
                     for (int b = 0; b < c.hd; b += 32) {
-                        uint32_t x[32];
-                        tmem_ld32(to + b, x);
+                        tmem_ld32(to + b, x[0]);
 #pragma unroll
-                        for (int e = 0; e < 32; e++) x[e] = __float_as_uint(__uint_as_float(x[e]) * f);
-                        tmem_st32(to + b, x);
+                        for (int e = 0; e < 32; e++) x[0][e] = __float_as_uint(__uint_as_float(x[0][e]) * f);
+                        tmem_st32(to + b, x[0]);
                     }
                 }
             }
+            // ---- weights
             const float ref = m == -INFINITY ? 0.0f : m;
+            const uint64_t ref2 = f2_pack(-ref, -ref);
+            uint64_t sum[2] = {0, 0};
+#pragma unroll 1
+            for (int b2 = 0; b2 < 4; b2 += 2) {
+                tmem_ld64(ts + 32 * b2, x);
+                if (edge) {
+                    hide(b2, x[0]);
+                    hide(b2 + 1, x[1]);
+                }
 #pragma unroll
-            for (int b = 0; b < 4; b++) {
-                uint32_t x[32], p[16], pl[16];
-                tmem_ld32(ts + 32 * b, x);
+                for (int b = 0; b < 2; b++) {
+                    uint32_t p[16], pl[16];
 #pragma unroll
-                for (int e2 = 0; e2 < 2; e2++) {
-                    const float cs = me.ks[2 * b + e2] * rs, fv = me.fv[2 * b + e2];
-                    const bool here = (me.live >> (2 * b + e2)) & 1;
-                    if (((me.nan >> (2 * b + e2)) & 1) && here && key0 + 32 * b + 16 * e2 <= lim) l = __int_as_float(0x7FC00000);
+                    for (int g = 0; g < 2; g++) {
+                        const float cs = factor(2 * (b2 + b) + g), fv = me.fv[2 * (b2 + b) + g];
+                        const uint64_t cs2 = f2_pack(cs, cs), fv2 = f2_pack(fv, fv);
 #pragma unroll
-                    for (int e = 0; e < 16; e += 2) {
-                        float w[2];
-#pragma unroll
-                        for (int k = 0; k < 2; k++) {
-                            const bool see = !edge || (key0 + 32 * b + 16 * e2 + e + k <= lim && here);
-                            w[k] = see ? kv_exp2(fmaf(__uint_as_float(x[16 * e2 + e + k]), cs, -ref)) : 0.0f;
-                            l += w[k];
-                            w[k] *= fv;
-                        }
-                        p[8 * e2 + e / 2] = half2_bits(w[0], w[1]);
-                        if (TERMS == 2) {
-                            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&p[8 * e2 + e / 2]));
-                            pl[8 * e2 + e / 2] = half2_bits(w[0] - f.x, w[1] - f.y);
+                        for (int e = 0; e < 16; e += 2) {
+                            float2 w = f2_unpack(f2_fma(f2_pack(__uint_as_float(x[b][16 * g + e]), __uint_as_float(x[b][16 * g + e + 1])),
+                                                        cs2, ref2));
+                            const uint64_t w2 = f2_pack(kv_exp2(w.x), kv_exp2(w.y));
+                            sum[g] = f2_add(sum[g], w2);
+                            w = f2_unpack(f2_mul(w2, fv2));
+                            p[8 * g + e / 2] = half2_bits(w.x, w.y);
+                            if (TERMS == 2) {
+                                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&p[8 * g + e / 2]));
+                                pl[8 * g + e / 2] = half2_bits(w.x - f.x, w.y - f.y);
+                            }
                         }
                     }
+                    tmem_st16(tp + 16 * (b2 + b), p);
+                    if (TERMS == 2) tmem_st16(tp + 64 + 16 * (b2 + b), pl);
                 }
-                tmem_st16(tp + 16 * b, p);
-                if (TERMS == 2) tmem_st16(tp + 64 + 16 * b, pl);
+            }
+            const float2 s0 = f2_unpack(sum[0]), s1 = f2_unpack(sum[1]);
+            l += (s0.x + s0.y) + (s1.x + s1.y);
+            if (me.nan) {   // a NaN scale reaches the rows that see a key under it
+#pragma unroll 1
+                for (int g = 0; g < 8; g++)
+                    if (((me.nan >> g) & 1) && key0 + 16 * g <= lim) l = __int_as_float(0x7FC00000);
             }
             tmem_wait_st();
             tc_fence_before();
@@ -389,81 +461,91 @@ __global__ void __launch_bounds__(kKvpThreads, 1) k_kv_prompt(const KvAttnArgs a
         const int8_t *kp = c.k + a.layer * c.plane(), *vp = c.v + a.layer * c.plane();
         const int tg = (lane & 7) + 8 * (w4 & 1), vc = (lane >> 3) + 4 * (w4 >> 1);   // V: 8 tokens, 16 dimensions
         const int kr = id >> 3, kc = id & 7;                                            // K: row of 16, 16 dimensions
-        auto look = [&](int j) {   // lane e < 8: the page of keys 128 j + 16 e..
+        // Lane e (mod 8) keeps track of keys 128 j + 16 e..+15 of a tile: where their values lie (-1: no page) and scales.
+        auto look = [&](int j) {
             const int pos = j * kKvpTile + 16 * (lane & 7);
-            int page = -1;
+            return j < ntiles && pos < q.len ? table[pos >> c.page_log] : -1;
+        };
+        struct Piece {
+            long long at;
+            float ks, vs;
+        };
+        auto find = [&](int j, int page) {
+            Piece p = {-1, 0.0f, 0.0f};
+            const int pos = j * kKvpTile + 16 * (lane & 7);
             if (j < ntiles && pos < q.len) {
-                page = table[pos >> c.page_log];
                 if (page < 0 || page >= c.n_pages) {
                     kv_flag(c, KV_BAD_PAGE);
-                    page = -1;
+                } else {
+                    const long long unit = (long long)page * c.nkv + h;
+                    p.at = (unit * c.page + (pos & (c.page - 1))) * c.hd;
+                    p.ks = c.k_scale[(long long)a.layer * c.n_pages * c.nkv + unit];
+                    p.vs = c.v_scale[(long long)a.layer * c.n_pages * c.nkv + unit];
                 }
             }
-            return page;
+            return p;
         };
-        auto load_k = [&](int j, int page, uint4 (&x)[8]) {
+        const int8_t *ksrc = kp + kr * c.hd + 16 * kc, *vsrc = vp + (8 * tg & 15) * c.hd + 16 * vc;
+        const bool kin = kc < cpr, vin = vc < cpr;
+        auto load_k = [&](const Piece& p, uint4 (&x)[8]) {
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                const int pg = __shfl_sync(0xffffffffu, page, e);
-                x[e] = make_uint4(0, 0, 0, 0);
-                if (pg >= 0 && kc < cpr)
-                    x[e] = *reinterpret_cast<const uint4*>(
-                        kp + (((long long)pg * c.nkv + h) * c.page + ((j * kKvpTile + 16 * e) & (c.page - 1)) + kr) * c.hd + 16 * kc);
+                const long long at = __shfl_sync(0xffffffffu, p.at, e);
+                x[e] = at >= 0 && kin ? *reinterpret_cast<const uint4*>(ksrc + at) : make_uint4(0, 0, 0, 0);
             }
         };
-        auto load_v = [&](int j, int page, uint4 (&x)[8]) {
-            const int pg = __shfl_sync(0xffffffffu, page, tg >> 1);
-            const int8_t* src = vp + (((long long)pg * c.nkv + h) * c.page + ((j * kKvpTile + 8 * tg) & (c.page - 1))) * c.hd + 16 * vc;
+        auto load_v = [&](const Piece& p, uint4 (&x)[8]) {
+            const long long at = __shfl_sync(0xffffffffu, p.at, tg >> 1);
+            const int8_t* src = vsrc + at;
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                x[e] = make_uint4(0, 0, 0, 0);
-                if (pg >= 0 && vc < cpr) x[e] = *reinterpret_cast<const uint4*>(src + e * c.hd);
+                x[e] = at >= 0 && vin ? *reinterpret_cast<const uint4*>(src) : make_uint4(0, 0, 0, 0);
+                src += c.hd;
             }
         };
+        const float vinv = vref > 0.0f ? 128.0f / vref : 0.0f;
+        unsigned char* kto[2] = {kst + kvp_piece(kr, 2 * kc), kst + kvp_piece(kr, 2 * kc + 1)};   // + 2 KB every 16 rows
         uint4 kx[8], vx[8];
-        int page = look(0);
-        load_k(0, page, kx);
-        load_v(0, page, vx);
+        Piece cur = find(0, look(0));
+        int page1 = look(1);
+        load_k(cur, kx);
+        load_v(cur, vx);
+#pragma unroll 1
         for (int j = 0; j < ntiles; j++) {
             const int st = j & 1;
             if (j >= 2 && !kvp_wait(&k_empty[st], ((j >> 1) - 1) & 1, &s_fail)) break;
-            unsigned char* kb = kst + st * kKvpBlock;
+            if (kin) {
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const int row = 16 * e + kr;
-                const uint2 p0 = int8x4_to_half(kx[e].x), p1 = int8x4_to_half(kx[e].y), p2 = int8x4_to_half(kx[e].z),
-                            p3 = int8x4_to_half(kx[e].w);
-                if (kc < cpr) {
-                    *reinterpret_cast<uint4*>(kb + kvp_piece(row, 2 * kc)) = make_uint4(p0.x, p0.y, p1.x, p1.y);
-                    *reinterpret_cast<uint4*>(kb + kvp_piece(row, 2 * kc + 1)) = make_uint4(p2.x, p2.y, p3.x, p3.y);
+                for (int e = 0; e < 8; e++) {
+                    const uint2 p0 = int8x4_to_half(kx[e].x), p1 = int8x4_to_half(kx[e].y), p2 = int8x4_to_half(kx[e].z),
+                                p3 = int8x4_to_half(kx[e].w);
+                    *reinterpret_cast<uint4*>(kto[0] + st * kKvpBlock + e * 2048) = make_uint4(p0.x, p0.y, p1.x, p1.y);
+                    *reinterpret_cast<uint4*>(kto[1] + st * kKvpBlock + e * 2048) = make_uint4(p2.x, p2.y, p3.x, p3.y);
                 }
             }
             // Words of tile j - 4: its softmax was over before S of tile j - 2 was issued, and k_empty says that was.
             if (w4 == 0) {
-                float ks = 0.0f, vs = 0.0f;
-                if (lane < 8 && page >= 0) {
-                    ks = c.k_scale[((long long)a.layer * c.n_pages + page) * c.nkv + h];
-                    vs = c.v_scale[((long long)a.layer * c.n_pages + page) * c.nkv + h];
-                }
-                const unsigned live = __ballot_sync(0xffffffffu, lane < 8 && page >= 0);
-                const unsigned nan = __ballot_sync(0xffffffffu, vs != vs);
+                KvpMeta& me = s_meta[j & 3];
+                const unsigned live = __ballot_sync(0xffffffffu, cur.at >= 0);
+                const unsigned nan = __ballot_sync(0xffffffffu, cur.ks != cur.ks || cur.vs != cur.vs);
                 if (lane < 8) {
-                    s_meta[j & 3].ks[lane] = ks;
-                    s_meta[j & 3].fv[lane] = vref > 0.0f && vs == vs ? vs / vref * 128.0f : 0.0f;
+                    me.ks[lane] = cur.ks > 0.0f ? cur.ks : 1.0f;
+                    me.fv[lane] = cur.vs > 0.0f ? cur.vs * vinv : 0.0f;
                 }
                 if (lane == 0) {
-                    s_meta[j & 3].live = live;
-                    s_meta[j & 3].nan = nan;
+                    me.live = live & 0xFF;
+                    me.nan = nan & 0xFF;
                 }
             }
             fence_smem_async();
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_addr(&k_full[st]));
-            const int next = look(j + 1);
-            load_k(j + 1, next, kx);
+            cur = find(j + 1, page1);
+            page1 = look(j + 2);
+            load_k(cur, kx);
             if (j >= 2 && !kvp_wait(&v_empty[st], ((j >> 1) - 1) & 1, &s_fail)) break;
-            unsigned char* vb = vst + st * kKvpBlock;
-            if (vc < cpr) {
+            if (vin) {
+                unsigned char* vb = vst + st * kKvpBlock;
 #pragma unroll
                 for (int w = 0; w < 4; w++) {
                     uint32_t lo[4], hi[4];   // dimension 16 vc + 4 w + d: tokens 0..3, 4..7 of the eight
@@ -480,73 +562,73 @@ __global__ void __launch_bounds__(kKvpThreads, 1) k_kv_prompt(const KvAttnArgs a
             fence_smem_async();
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_addr(&v_full[st]));
-            load_v(j + 1, next, vx);
-            page = next;
+            load_v(cur, vx);
         }
-    } else if (warp == 12 && lane == 0) {
+    } else if (warp == 12) {
         // ================= MMA issue =================
         const uint32_t id_s = kvp_idesc(kKvpTile), id_o = kvp_idesc(c.hd);
+        const uint32_t qd = umma_lo(smem_addr(qs)), kd = umma_lo(smem_addr(kst)), vd = umma_lo(smem_addr(vst));
+        const int nk = c.hd / 16;
+        constexpr uint32_t kTile = kKvpBlock >> 4;   // an operand in units of 16 bytes; a k-step is 2, its second half kTile / 2 on
         auto scores = [&](int j, int t) {
-            const uint32_t kb = smem_addr(kst + (j & 1) * kKvpBlock);
             const int sb = TERMS == 2 ? j & 1 : t;
-            const uint32_t d = tmem + (TERMS == 2 ? 384 * sb : 128 * t);
-#pragma unroll
-            for (int term = 0; term < TERMS; term++) {
-                const uint32_t qb = smem_addr(qs + (t + term) * kKvpBlock);
-                for (int k = 0; k < c.hd / 16; k++) {
-                    const uint32_t off = (uint32_t)(k >> 2) * (kKvpBlock / 2);
-                    umma_f16(d, umma_desc_sw128(qb + off) + 2 * (k & 3), umma_desc_sw128(kb + off) + 2 * (k & 3), id_s,
-                              (term | k) != 0);
-                }
-            }
-            umma_commit(smem_addr(&s_full[sb]));
-        };
-        auto values = [&](int j, int t) {
-            const uint32_t vb = smem_addr(vst + (j & 1) * kKvpBlock);
-            const uint32_t p = tmem + (TERMS == 2 ? 128 : 128 * t);
+            const uint32_t d = tmem + (TERMS == 2 ? 384 * sb : 128 * t), kb = kd + (j & 1) * kTile;
 #pragma unroll
             for (int term = 0; term < TERMS; term++)
-                for (int k = 0; k < kKvpTile / 16; k++)
-                    umma_ts(tmem + 256 + 128 * t, p + 64 * term + 8 * k,
-                            umma_desc_sw128(vb + (uint32_t)(k >> 2) * (kKvpBlock / 2)) + 2 * (k & 3), id_o, (j | term | k) != 0);
-            umma_commit(smem_addr(&pv_done[t]));
+#pragma unroll
+                for (int k = 0; k < 8; k++)
+                    if (k < nk) {
+                        const uint32_t off = (k >> 2) * (kTile / 2) + 2 * (k & 3);
+                        umma_f16_warp(d, umma_desc_of(qd + (t + term) * kTile + off), umma_desc_of(kb + off), id_s, (term | k) != 0);
+                    }
+            umma_commit_warp(smem_addr(&s_full[sb]));
         };
-        auto wait_k = [&](int j) { return kvp_wait(&k_full[j & 1], (j >> 1) & 1, &s_fail); };
-        bool ok = ntiles == 0 || (kvp_wait(&q_full, 0, &s_fail) && wait_k(0));
+        auto values = [&](int j, int t) {
+            const uint32_t d = tmem + 256 + 128 * t, p = tmem + (TERMS == 2 ? 128 : 128 * t), vb = vd + (j & 1) * kTile;
+#pragma unroll
+            for (int term = 0; term < TERMS; term++)
+#pragma unroll
+                for (int k = 0; k < 8; k++)
+                    umma_f16_ts_warp(d, p + 64 * term + 8 * k, umma_desc_of(vb + (k >> 2) * (kTile / 2) + 2 * (k & 3)), id_o,
+                            (term | k) != 0 || j > 0);
+            umma_commit_warp(smem_addr(&pv_done[t]));
+        };
+        auto wait_for = [&](uint64_t* bar, int parity) { return (bool)__all_sync(0xffffffffu, kvp_wait(bar, parity & 1, &s_fail)); };
+        bool ok = ntiles == 0 || (wait_for(&q_full, 0) && wait_for(&k_full[0], 0));
         tc_fence_after();
         if (ok && ntiles > 0) {
             for (int t = 0; t < nq; t++)
                 if (nt[NQ == 2 ? t : 0] > 0) scores(0, t);
-            umma_commit(smem_addr(&k_empty[0]));
+            umma_commit_warp(smem_addr(&k_empty[0]));
         }
         for (int j = 0; j < ntiles && ok; j++) {
             const bool more = j + 1 < ntiles;
-            if (more) ok = wait_k(j + 1);
+            if (more) ok = wait_for(&k_full[(j + 1) & 1], (j + 1) >> 1);
             tc_fence_after();
             if (TERMS == 2 && more && ok) {   // S of the next tile goes to the other buffer, read two tiles ago
                 scores(j + 1, 0);
-                umma_commit(smem_addr(&k_empty[(j + 1) & 1]));
+                umma_commit_warp(smem_addr(&k_empty[(j + 1) & 1]));
             }
-            ok = ok && kvp_wait(&v_full[j & 1], (j >> 1) & 1, &s_fail);
+            ok = ok && wait_for(&v_full[j & 1], j >> 1);
             for (int t = 0; t < nq && ok; t++) {
                 const int mine = nt[NQ == 2 ? t : 0];
                 if (j >= mine) continue;
-                ok = kvp_wait(&p_full[t], j & 1, &s_fail);
+                ok = wait_for(&p_full[t], j);
                 if (!ok) break;
                 tc_fence_after();
                 values(j, t);
                 if (TERMS == 1 && j + 1 < mine) {   // into the columns of the P just read
-                    ok = kvp_wait(&pv_done[t], j & 1, &s_fail);
+                    ok = wait_for(&pv_done[t], j);
                     if (!ok) break;
                     tc_fence_after();
                     scores(j + 1, t);
                 }
             }
             if (!ok) break;
-            umma_commit(smem_addr(&v_empty[j & 1]));
-            if (TERMS == 1 && more) umma_commit(smem_addr(&k_empty[(j + 1) & 1]));
+            umma_commit_warp(smem_addr(&v_empty[j & 1]));
+            if (TERMS == 1 && more) umma_commit_warp(smem_addr(&k_empty[(j + 1) & 1]));
         }
-        umma_commit(smem_addr(&done_bar));
+        umma_commit_warp(smem_addr(&done_bar));
     }
     tc_fence_before();
     __syncthreads();
