@@ -389,18 +389,18 @@ static cudaError_t launch_attention(const KvAttnArgs& a, int blocks, int dev, cu
     return e;
 }
 
-template <typename T, int NQ>
+template <typename T>
 static cudaError_t launch_prompt(const KvAttnArgs& a, int dev, cudaStream_t st) {
     static std::atomic<uint64_t> opted{0};
     const uint64_t bit = dev >= 0 && dev < 64 ? 1ull << dev : 0;
     if (!bit || !(opted.load() & bit)) {
         const cudaError_t e =
-            cudaFuncSetAttribute(k_kv_prompt<T, NQ>, cudaFuncAttributeMaxDynamicSharedMemorySize, kKvpSmem);
+            cudaFuncSetAttribute(k_kv_prompt<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kKvpSmem);
         if (e != cudaSuccess) return e;
         opted.fetch_or(bit);
     }
-    const int64_t places = (int64_t)a.r.n_tok * a.group / (128 * NQ) + a.r.n_seq;
-    k_kv_prompt<T, NQ><<<dim3((unsigned)places, a.c.nkv), kKvpThreads, kKvpSmem, st>>>(a);
+    const int64_t places = (int64_t)a.r.n_tok * a.group / 256 + a.r.n_seq;
+    k_kv_prompt<T><<<dim3((unsigned)places, a.c.nkv), kKvpThreads, kKvpSmem, st>>>(a);
     return cudaGetLastError();
 }
 
@@ -449,9 +449,9 @@ extern "C" AION_API aion_status aion_kv8_attention(const aion_kv8* kv, int32_t l
     a.parts = (KvPart*)workspace;
     const cudaStream_t st = (cudaStream_t)stream;
     if (attention_tiles(n_seq, n_tok, a.group)) {
-        if (type == AION_F32) KV_CUDA((launch_prompt<float, 1>(a, kv->device, st)));
-        else if (type == AION_F16) KV_CUDA((launch_prompt<__half, 2>(a, kv->device, st)));
-        else KV_CUDA((launch_prompt<__nv_bfloat16, 2>(a, kv->device, st)));
+        if (type == AION_F32) KV_CUDA((launch_prompt<float>(a, kv->device, st)));
+        else if (type == AION_F16) KV_CUDA((launch_prompt<__half>(a, kv->device, st)));
+        else KV_CUDA((launch_prompt<__nv_bfloat16>(a, kv->device, st)));
         return AION_OK;
     }
     const int blocks = attention_blocks(kv);

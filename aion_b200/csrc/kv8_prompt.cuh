@@ -10,21 +10,25 @@
 namespace aion {
 
 // ---------------------------------------------------------------------------
-// A block takes one K/V head and 256 rows (two tiles of 128; one of 128 for
-// fp32 rows) of a sequence: the rows of a K/V head are its tokens times the
-// query heads that read it, so grouped heads share every key.  Keys come in
-// tiles of 128:
+// A block takes one K/V head and 256 rows (two tiles of 128) of a sequence: the
+// rows of a K/V head are its tokens times the query heads that read it, so
+// grouped heads share every key.  Keys come in tiles of 64:
 //   warps 0-3, 4-7   softmax of row tile 0, 1: one thread a row;
-//   warps 8-11       bring K and V from int8 to fp16, which holds each value
-//                    exactly, into 128-byte-swizzled shared memory, V
-//                    transposed (tokens contiguous);
-//   warp 12          issues tcgen05.mma (kind::f16, M 128):
+//   warps 8-15       fetch K (warps 8, 9, 12, 13) and V (the others) with
+//                    cp.async and bring them from int8 to fp16, which holds
+//                    each value exactly, in 128-byte-swizzled shared memory,
+//                    V transposed (tokens contiguous);
+//   warps 16, 17     issue tcgen05.mma (kind::f16, M 128) for row tile 0, 1:
 //                    S = Q K^T, then O += P V with P read from TMEM.
-// TMEM, 128 columns each: S of tile 0 | S of tile 1 | O of tile 0 | O of tile
-// 1, P in the columns of its own S; fp32 rows: S of even key tiles | P | O | S
-// of odd key tiles.  S of the next key tile overwrites P of this one only
-// after the MMAs that read it have completed (pv_done): nothing else orders
-// two MMAs of different accumulators.
+// Each role is a chain of waits, so none is given two tiles' or two operands'
+// work; the softmax, the longest, takes registers from the others (setmaxnreg).
+// Loops are kept short, and K and V warps on sub-partitions of their own: the
+// roles of a sub-partition share its instruction cache.
+// TMEM, for each row tile: two S buffers of 64 columns, O of 128.  P takes the
+// place of its own S (which the softmax holds in registers by then), so S of
+// key tile i + 2 waits for the MMAs that read P of tile i (pv_done: nothing
+// else orders two MMAs of different accumulators), while the softmax works on
+// tile i + 1.
 //
 // Arithmetic.  fp16 queries are taken as they are; bf16 and fp32 ones are
 // scaled by a power of two per row so that the largest is below 2^15 (a bf16
@@ -38,10 +42,18 @@ namespace aion {
 // follows the row's maximum only when that has grown by more than 8 (a factor
 // of 2^8, and P stays below 2^15), which leaves O untouched for most tiles.
 // ---------------------------------------------------------------------------
-constexpr int kKvpThreads = 416, kKvpTile = 128;
-constexpr int kKvpBlock = 128 * 128 * 2;   // a 128 x 128 fp16 operand: two 128-byte-wide halves
-constexpr int kKvpSmem = 6 * kKvpBlock + 1024;
+constexpr int kKvpThreads = 640, kKvpTile = 64;
+constexpr int kKvpQ = 128 * 128 * 2;        // a query operand: 128 rows of two 128-byte-wide halves
+constexpr int kKvpStage = 64 * 128 * 2;     // a key tile's K (64 rows, two halves) or V (up to 128 dimensions x 64 tokens)
+constexpr int kKvpRaw = 64 * 128;           // a key tile's K or V as the cache holds it
+constexpr int kKvpSmem = 2 * kKvpQ + 8 * kKvpStage + 4 * kKvpRaw + 1024;
 constexpr uint32_t kKvpWaitLimit = 1u << 20;
+
+// Registers a thread, by warpgroup; at launch all have 96 (640 threads).
+constexpr int kKvpRegsSoft = 144, kKvpRegsConv = 72, kKvpRegsMma = 40;
+static_assert(2 * kKvpRegsSoft + 2 * kKvpRegsConv + kKvpRegsMma <= 5 * 96, "the registers of the launch");
+template <int N> __device__ __forceinline__ void regs_more() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void regs_less() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
 __device__ __forceinline__ uint32_t kvp_idesc(int n) {   // fp16 A and B (K-major), fp32 D, M 128
     return (1u << 4) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
@@ -142,9 +154,10 @@ __device__ __forceinline__ uint2 int8x4_to_half(uint32_t w) {
     const __half2 x = __hsub2(*reinterpret_cast<__half2*>(&a), o), y = __hsub2(*reinterpret_cast<__half2*>(&b), o);
     return make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
 }
-// Byte offset of 16-byte piece ch (8 values) of a row of 128 fp16 values.
-__device__ __forceinline__ int kvp_piece(int row, int ch) {
-    return (ch >> 3) * (kKvpBlock / 2) + row * 128 + (((ch & 7) ^ (row & 7)) << 4);
+// Byte offset of 16-byte piece ch (8 values) of a row of an operand of `rows`
+// rows, in halves of 64 values with the 128-byte swizzle.
+__device__ __forceinline__ int kvp_piece(int rows, int row, int ch) {
+    return (ch >> 3) * rows * 128 + row * 128 + (((ch & 7) ^ (row & 7)) << 4);
 }
 
 // Wait that gives up when the block has failed or after kKvpWaitLimit polls.
@@ -161,24 +174,26 @@ __device__ __forceinline__ bool kvp_wait(uint64_t* bar, uint32_t parity, volatil
 // What the softmax needs to know of a key tile: for each 16 of its keys the
 // scales, and which of them have a page.
 struct KvpMeta {
-    float ks[8], fv[8];   // fv = 2^7 vscale / vref; ks is positive (1 where the page's values are 0 or NaN)
+    float ks[4], fv[4];   // fv = 2^7 vscale / vref; ks is positive (1 where the page's values are 0 or NaN)
     uint32_t live, nan;   // bit j: keys 16 j.. have a page; one of its scales is NaN
 };
 
-template <typename T, int NQ>
+template <typename T>
 __global__ void __launch_bounds__(kKvpThreads, 1) k_kv_prompt(const KvAttnArgs a) {
     constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;   // fp16 terms of a query and of a weight
-    static_assert(NQ * TERMS == 2, "two query tiles in shared memory");
-    constexpr int ROWS = 128 * NQ;
+    constexpr int NQ = 2, ROWS = 128 * NQ;
+    constexpr int ST = TERMS == 2 ? 2 : 4;          // stages of K and of V
+    static_assert(NQ * TERMS * kKvpQ + 2 * ST * kKvpStage + 4 * kKvpRaw + 1024 == kKvpSmem, "shared memory");
     extern __shared__ __align__(1024) unsigned char psm_raw[];
-    __shared__ __align__(8) uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[NQ],
-        pv_done[NQ], done_bar;
+    __shared__ __align__(8) uint64_t q_full, k_full[ST], k_empty[ST], v_full[ST], v_empty[ST], s_full[NQ][2], p_full[NQ][2],
+        pv_done[NQ], o_full[NQ], done_bar;
     __shared__ uint32_t s_tmem;
     __shared__ float s_red[4];
-    __shared__ KvpMeta s_meta[4];
+    __shared__ KvpMeta s_meta[8];
+    __shared__ float s_scale[2][8];   // K and V scales of a tile's four pieces on their way; K scale -1: no page
     __shared__ volatile int s_fail;
     unsigned char* sm = psm_raw + ((1024u - (smem_addr(psm_raw) & 1023u)) & 1023u);
-    unsigned char *qs = sm, *kst = sm + 2 * kKvpBlock, *vst = sm + 4 * kKvpBlock;
+    unsigned char *qs = sm, *kst = sm + NQ * TERMS * kKvpQ, *vst = kst + ST * kKvpStage, *raw = vst + ST * kKvpStage;
     const KvView& c = a.c;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -207,30 +222,32 @@ __global__ void __launch_bounds__(kKvpThreads, 1) k_kv_prompt(const KvAttnArgs a
     for (int i = 0; i < NQ; i++) {
         const int last = min(row0 + 128 * (i + 1), row0 + rows) - 1;
         const long long seen = min((long long)q.p0 + last / a.group, (long long)q.len - 1) + 1;
-        nt[i] = i < nq ? (int)((seen + kKvpTile - 1) / kKvpTile) : 0;
-        if (q.len == 0) nt[i] = 0;
+        nt[i] = i < nq && q.len ? (int)((seen + kKvpTile - 1) / kKvpTile) : 0;
     }
     const int ntiles = nt[nq - 1];
 
     if (threadIdx.x == 0) {
         kv_vet_seq(a, q);
         mbar_init(smem_addr(&q_full), 4 * NQ);
-        for (int i = 0; i < 2; i++) {
+        for (int i = 0; i < ST; i++) {
             mbar_init(smem_addr(&k_full[i]), 4);
-            mbar_init(smem_addr(&k_empty[i]), 1);
+            mbar_init(smem_addr(&k_empty[i]), NQ);
             mbar_init(smem_addr(&v_full[i]), 4);
-            mbar_init(smem_addr(&v_empty[i]), 1);
-            mbar_init(smem_addr(&s_full[i]), 1);
+            mbar_init(smem_addr(&v_empty[i]), NQ);
         }
         for (int i = 0; i < NQ; i++) {
-            mbar_init(smem_addr(&p_full[i]), 4);
+            for (int b = 0; b < 2; b++) {
+                mbar_init(smem_addr(&s_full[i][b]), 1);
+                mbar_init(smem_addr(&p_full[i][b]), 4);
+            }
             mbar_init(smem_addr(&pv_done[i]), 1);
+            mbar_init(smem_addr(&o_full[i]), 1);
         }
-        mbar_init(smem_addr(&done_bar), 1);
+        mbar_init(smem_addr(&done_bar), NQ);
         s_fail = 0;
         fence_mbar_init();
     }
-    if (warp == 12) {
+    if (warp == 16) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&s_tmem)), "r"(512)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -255,8 +272,9 @@ __global__ void __launch_bounds__(kKvpThreads, 1) k_kv_prompt(const KvAttnArgs a
     const uint32_t tmem = s_tmem;
     vref = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
 
-    if (warp < 4 * NQ) {
+    if (warp < 8) {
         // ================= softmax: thread = row =================
+        regs_more<kKvpRegsSoft>();
         const int tile = warp >> 2, r = threadIdx.x & 127, i = row0 + 128 * tile + r;
         const int tok = i / a.group, head = h * a.group + (i - tok * a.group);
         const bool live_row = i < total && 128 * tile + r < rows;
@@ -305,10 +323,10 @@ __global__ void __launch_bounds__(kKvpThreads, 1) k_kv_prompt(const KvAttnArgs a
                 }
 #pragma unroll
                 for (int p = 0; p < 2; p++) {
-                    unsigned char* to = qs + tile * kKvpBlock + kvp_piece(r, d / 8 + p);
+                    unsigned char* to = qs + tile * TERMS * kKvpQ + kvp_piece(128, r, d / 8 + p);
                     *reinterpret_cast<uint4*>(to) = make_uint4(hi[4 * p], hi[4 * p + 1], hi[4 * p + 2], hi[4 * p + 3]);
                     if (TERMS == 2)
-                        *reinterpret_cast<uint4*>(to + kKvpBlock) =
+                        *reinterpret_cast<uint4*>(to + kKvpQ) =
                             make_uint4(lo[4 * p], lo[4 * p + 1], lo[4 * p + 2], lo[4 * p + 3]);
                 }
             }
@@ -318,59 +336,48 @@ __global__ void __launch_bounds__(kKvpThreads, 1) k_kv_prompt(const KvAttnArgs a
         if (lane == 0) mbar_arrive(smem_addr(&q_full));
 
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
-        const uint32_t to = tmem + lanes + 256 + 128 * tile;                              // O
-        const uint32_t tp = tmem + lanes + (TERMS == 2 ? 128 : 128 * tile);               // P
+        const uint32_t to = tmem + lanes + 256 + 128 * tile;   // O
         float m = -INFINITY, l = bad ? __int_as_float(0x7FC00000) : 0.0f;   // a NaN in l stays and reaches the result
-        const int mine = nt[NQ == 2 ? tile : 0];
+        const int mine = nt[tile];
         bool ok = true;
+        auto wait_for = [&](uint64_t* bar, int parity) { return (bool)__all_sync(0xffffffffu, kvp_wait(bar, parity & 1, &s_fail)); };
+#pragma unroll 1
         for (int j = 0; j < mine; j++) {
-            const int sb = TERMS == 2 ? j & 1 : tile;   // which S
-            if (!__all_sync(0xffffffffu, kvp_wait(&s_full[sb], (TERMS == 2 ? j >> 1 : j) & 1, &s_fail))) {
-                ok = false;
-                break;
-            }
+            ok = wait_for(&s_full[tile][j & 1], j >> 1);
+            if (!ok) break;
             tc_fence_after();
-            const uint32_t ts = tmem + lanes + (TERMS == 2 ? 384 * sb : 128 * tile);
-            const KvpMeta& me = s_meta[j & 3];   // written before the tile's K was announced
+            const uint32_t ts = tmem + lanes + 128 * tile + 64 * (j & 1);   // S, then P
+            const KvpMeta& me = s_meta[j & 7];   // written before the tile's K was announced
             const int key0 = j * kKvpTile;
+            uint32_t x[2][32];
+            tmem_ld64(ts, x);
             // some row of the warp does not see every key of the tile
-            const bool edge = __any_sync(0xffffffffu, key0 + kKvpTile - 1 > lim) || me.live != 0xFFu;
-            auto hide = [&](int b, uint32_t(&v)[32]) {   // -inf at the keys of 32 b.. that are not seen
-                const int n = lim - (key0 + 32 * b) + 1;
-                uint32_t see = n >= 32 ? 0xFFFFFFFFu : n <= 0 ? 0u : (1u << n) - 1u;
-                if (!((me.live >> (2 * b)) & 1)) see &= 0xFFFF0000u;
-                if (!((me.live >> (2 * b + 1)) & 1)) see &= 0xFFFFu;
+            if (__any_sync(0xffffffffu, key0 + kKvpTile - 1 > lim) || me.live != 0xFu) {
 #pragma unroll
-                for (int e = 0; e < 32; e++) v[e] = (see >> e) & 1 ? v[e] : 0xFF800000u;
-            };
+                for (int b = 0; b < 2; b++) {   // -inf at the keys that are not seen
+                    const int n = lim - (key0 + 32 * b) + 1;
+                    uint32_t see = n >= 32 ? 0xFFFFFFFFu : n <= 0 ? 0u : (1u << n) - 1u;
+                    if (!((me.live >> (2 * b)) & 1)) see &= 0xFFFF0000u;
+                    if (!((me.live >> (2 * b + 1)) & 1)) see &= 0xFFFFu;
+#pragma unroll
+                    for (int e = 0; e < 32; e++) x[b][e] = (see >> e) & 1 ? x[b][e] : 0xFF800000u;
+                }
+            }
             // factors of the scores: never 0, so that -inf stays -inf
-            auto factor = [&](int g) { return fmaxf(me.ks[g] * rs, 1.17549435e-38f); };
+            float cs[4];
+#pragma unroll
+            for (int g = 0; g < 4; g++) cs[g] = fmaxf(me.ks[g] * rs, 1.17549435e-38f);
             // ---- the tile's maximum
             float mt = -INFINITY;
-            uint32_t x[2][32];
-#pragma unroll 1
-            for (int b2 = 0; b2 < 4; b2 += 2) {
-                tmem_ld64(ts + 32 * b2, x);
-                if (edge) {
-                    hide(b2, x[0]);
-                    hide(b2 + 1, x[1]);
-                }
 #pragma unroll
-                for (int g = 0; g < 4; g++) {
-                    const uint32_t* v = x[g >> 1] + 16 * (g & 1);
-                    float mx = __uint_as_float(v[0]);
+            for (int g = 0; g < 4; g++) {
+                const uint32_t* v = x[g >> 1] + 16 * (g & 1);
+                float mx = __uint_as_float(v[0]);
 #pragma unroll
-                    for (int e = 1; e < 15; e += 2) mx = max3(mx, __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
-                    mx = fmaxf(mx, __uint_as_float(v[15]));
-                    mt = fmaxf(mt, mx * factor(2 * b2 + g));
-                }
+                for (int e = 1; e < 15; e += 2) mx = max3(mx, __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
+                mx = fmaxf(mx, __uint_as_float(v[15]));
+                mt = fmaxf(mt, mx * cs[g]);   // fmaxf leaves a NaN out: m is never one
             }
-            // P and O of the tile before are done with (16-bit rows: as this S came after them)
-            if (TERMS == 2 && j > 0 && !__all_sync(0xffffffffu, kvp_wait(&pv_done[0], (j - 1) & 1, &s_fail))) {
-                ok = false;
-                break;
-            }
-            tc_fence_after();
             // the reference follows the maximum in steps of more than 8
             const bool grow = mt > m + 8.0f;
             if (__any_sync(0xffffffffu, grow)) {
@@ -378,12 +385,17 @@ __global__ void __launch_bounds__(kKvpThreads, 1) k_kv_prompt(const KvAttnArgs a
                 if (grow) m = mt;
                 l *= f;
                 if (j > 0) {
+                    ok = wait_for(&pv_done[tile], j - 1);   // O is whole up to the tile before
+                    if (!ok) break;
+                    tc_fence_after();
 #pragma unroll 1
-                    for (int b = 0; b < c.hd; b += 32) {
-                        tmem_ld32(to + b, x[0]);
+                    for (int b = 0; b < c.hd; b += 16) {
+                        float o[16];
+                        uint32_t u[16];
+                        tmem_ld16(to + b, o);
 #pragma unroll
-                        for (int e = 0; e < 32; e++) x[0][e] = __float_as_uint(__uint_as_float(x[0][e]) * f);
-                        tmem_st32(to + b, x[0]);
+                        for (int e = 0; e < 16; e++) u[e] = __float_as_uint(o[e] * f);
+                        tmem_st16(to + b, u);
                     }
                 }
             }
@@ -391,52 +403,44 @@ __global__ void __launch_bounds__(kKvpThreads, 1) k_kv_prompt(const KvAttnArgs a
             const float ref = m == -INFINITY ? 0.0f : m;
             const uint64_t ref2 = f2_pack(-ref, -ref);
             uint64_t sum[2] = {0, 0};
-#pragma unroll 1
-            for (int b2 = 0; b2 < 4; b2 += 2) {
-                tmem_ld64(ts + 32 * b2, x);
-                if (edge) {
-                    hide(b2, x[0]);
-                    hide(b2 + 1, x[1]);
-                }
 #pragma unroll
-                for (int b = 0; b < 2; b++) {
-                    uint32_t p[16], pl[16];
+            for (int b = 0; b < 2; b++) {
+                uint32_t p[16], pl[16];
 #pragma unroll
-                    for (int g = 0; g < 2; g++) {
-                        const float cs = factor(2 * (b2 + b) + g), fv = me.fv[2 * (b2 + b) + g];
-                        const uint64_t cs2 = f2_pack(cs, cs), fv2 = f2_pack(fv, fv);
+                for (int g = 0; g < 2; g++) {
+                    const float fv = me.fv[2 * b + g];
+                    const uint64_t cs2 = f2_pack(cs[2 * b + g], cs[2 * b + g]), fv2 = f2_pack(fv, fv);
 #pragma unroll
-                        for (int e = 0; e < 16; e += 2) {
-                            float2 w = f2_unpack(f2_fma(f2_pack(__uint_as_float(x[b][16 * g + e]), __uint_as_float(x[b][16 * g + e + 1])),
-                                                        cs2, ref2));
-                            const uint64_t w2 = f2_pack(kv_exp2(w.x), kv_exp2(w.y));
-                            sum[g] = f2_add(sum[g], w2);
-                            w = f2_unpack(f2_mul(w2, fv2));
-                            p[8 * g + e / 2] = half2_bits(w.x, w.y);
-                            if (TERMS == 2) {
-                                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&p[8 * g + e / 2]));
-                                pl[8 * g + e / 2] = half2_bits(w.x - f.x, w.y - f.y);
-                            }
+                    for (int e = 0; e < 16; e += 2) {
+                        float2 w = f2_unpack(f2_fma(
+                            f2_pack(__uint_as_float(x[b][16 * g + e]), __uint_as_float(x[b][16 * g + e + 1])), cs2, ref2));
+                        const uint64_t w2 = f2_pack(kv_exp2(w.x), kv_exp2(w.y));
+                        sum[g] = f2_add(sum[g], w2);
+                        w = f2_unpack(f2_mul(w2, fv2));
+                        p[8 * g + e / 2] = half2_bits(w.x, w.y);
+                        if (TERMS == 2) {
+                            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&p[8 * g + e / 2]));
+                            pl[8 * g + e / 2] = half2_bits(w.x - f.x, w.y - f.y);
                         }
                     }
-                    tmem_st16(tp + 16 * (b2 + b), p);
-                    if (TERMS == 2) tmem_st16(tp + 64 + 16 * (b2 + b), pl);
                 }
+                tmem_st16(ts + 16 * b, p);
+                if (TERMS == 2) tmem_st16(ts + 32 + 16 * b, pl);
             }
             const float2 s0 = f2_unpack(sum[0]), s1 = f2_unpack(sum[1]);
             l += (s0.x + s0.y) + (s1.x + s1.y);
             if (me.nan) {   // a NaN scale reaches the rows that see a key under it
 #pragma unroll 1
-                for (int g = 0; g < 8; g++)
+                for (int g = 0; g < 4; g++)
                     if (((me.nan >> g) & 1) && key0 + 16 * g <= lim) l = __int_as_float(0x7FC00000);
             }
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(smem_addr(&p_full[tile]));
+            if (lane == 0) mbar_arrive(smem_addr(&p_full[tile][j & 1]));
         }
         // ---- out = O vref / (2^7 l)
-        if (ok && mine > 0) ok = __all_sync(0xffffffffu, kvp_wait(&pv_done[tile], (mine - 1) & 1, &s_fail));
+        if (ok && mine > 0) ok = wait_for(&o_full[tile], 0);
         tc_fence_after();
         if (ok && (tile < nq)) {
             const float f = l == 0.0f ? 0.0f : vref * 0.0078125f / l;
@@ -455,184 +459,203 @@ __global__ void __launch_bounds__(kKvpThreads, 1) k_kv_prompt(const KvAttnArgs a
             }
         }
         tc_fence_before();
-    } else if (warp >= 8 && warp < 12) {
-        // ================= K and V to fp16 =================
-        const int w4 = warp - 8, id = threadIdx.x - 256, cpr = c.hd / 16;
-        const int8_t *kp = c.k + a.layer * c.plane(), *vp = c.v + a.layer * c.plane();
-        const int tg = (lane & 7) + 8 * (w4 & 1), vc = (lane >> 3) + 4 * (w4 >> 1);   // V: 8 tokens, 16 dimensions
-        const int kr = id >> 3, kc = id & 7;                                            // K: row of 16, 16 dimensions
-        // Lane e (mod 8) keeps track of keys 128 j + 16 e..+15 of a tile: where their values lie (-1: no page) and scales.
+    } else if (warp < 16) {
+        // ================= K or V to fp16 =================
+        regs_less<kKvpRegsConv>();
+        const bool is_k = (warp & 2) == 0;
+        const int w4 = (warp & 1) | ((warp >> 1) & 2), id = 32 * w4 + lane;   // of the four warps of K, or of V
+        // Lane e (mod 4) keeps track of keys 64 j + 16 e..+15 of a tile.  Values are fetched two tiles ahead, pages three.
         auto look = [&](int j) {
-            const int pos = j * kKvpTile + 16 * (lane & 7);
+            const int pos = j * kKvpTile + 16 * (lane & 3);
             return j < ntiles && pos < q.len ? table[pos >> c.page_log] : -1;
         };
-        struct Piece {
-            long long at;
-            float ks, vs;
+        // (page, head) of the lane's 16 keys, or -1
+        auto unit_of = [&](int j, int page) {
+            const int pos = j * kKvpTile + 16 * (lane & 3);
+            if (j >= ntiles || pos >= q.len) return -1LL;
+            if (page < 0 || page >= c.n_pages) {
+                kv_flag(c, KV_BAD_PAGE);
+                return -1LL;
+            }
+            return (long long)page * c.nkv + h;
         };
-        auto find = [&](int j, int page) {
-            Piece p = {-1, 0.0f, 0.0f};
-            const int pos = j * kKvpTile + 16 * (lane & 7);
-            if (j < ntiles && pos < q.len) {
-                if (page < 0 || page >= c.n_pages) {
-                    kv_flag(c, KV_BAD_PAGE);
-                } else {
-                    const long long unit = (long long)page * c.nkv + h;
-                    p.at = (unit * c.page + (pos & (c.page - 1))) * c.hd;
-                    p.ks = c.k_scale[(long long)a.layer * c.n_pages * c.nkv + unit];
-                    p.vs = c.v_scale[(long long)a.layer * c.n_pages * c.nkv + unit];
+        // where the values of its 16 keys lie, or -1
+        auto at_of = [&](int j, long long unit) {
+            return unit < 0 ? -1LL : (unit * c.page + ((j * kKvpTile + 16 * (lane & 3)) & (c.page - 1))) * c.hd;
+        };
+        if (is_k) {
+            const int kr = id >> 3, kc = id & 7;   // row of each 16, 16 dimensions
+            const bool in = 16 * kc < c.hd;
+            const int8_t* src = c.k + a.layer * c.plane() + kr * c.hd + 16 * kc;
+            const float* scales = ((lane & 4) ? c.v_scale : c.k_scale) + (long long)a.layer * c.n_pages * c.nkv;
+            const float vinv = vref > 0.0f ? 128.0f / vref : 0.0f;
+            unsigned char *mine = raw + 16 * id;   // the thread's pieces, 2 KB apart
+            unsigned char *to0 = kst + kvp_piece(64, kr, 2 * kc), *to1 = kst + kvp_piece(64, kr, 2 * kc + 1);   // + 2 KB every 16 rows
+            auto fetch = [&](int j, int page) {
+                const long long unit = unit_of(j, page), at0 = at_of(j, unit);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const long long at = __shfl_sync(0xffffffffu, at0, e);
+                    if (at >= 0 && in) cp_async16(mine + (j & 1) * kKvpRaw + 2048 * e, src + at);
                 }
-            }
-            return p;
-        };
-        const int8_t *ksrc = kp + kr * c.hd + 16 * kc, *vsrc = vp + (8 * tg & 15) * c.hd + 16 * vc;
-        const bool kin = kc < cpr, vin = vc < cpr;
-        auto load_k = [&](const Piece& p, uint4 (&x)[8]) {
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const long long at = __shfl_sync(0xffffffffu, p.at, e);
-                x[e] = at >= 0 && kin ? *reinterpret_cast<const uint4*>(ksrc + at) : make_uint4(0, 0, 0, 0);
-            }
-        };
-        auto load_v = [&](const Piece& p, uint4 (&x)[8]) {
-            const long long at = __shfl_sync(0xffffffffu, p.at, tg >> 1);
-            const int8_t* src = vsrc + at;
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                x[e] = at >= 0 && vin ? *reinterpret_cast<const uint4*>(src) : make_uint4(0, 0, 0, 0);
-                src += c.hd;
-            }
-        };
-        const float vinv = vref > 0.0f ? 128.0f / vref : 0.0f;
-        unsigned char* kto[2] = {kst + kvp_piece(kr, 2 * kc), kst + kvp_piece(kr, 2 * kc + 1)};   // + 2 KB every 16 rows
-        uint4 kx[8], vx[8];
-        Piece cur = find(0, look(0));
-        int page1 = look(1);
-        load_k(cur, kx);
-        load_v(cur, vx);
+                if (w4 == 0 && lane < 8) {
+                    float* to = &s_scale[j & 1][lane];
+                    if (unit >= 0)
+                        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_addr(to)), "l"(scales + unit) : "memory");
+                    else
+                        *to = -1.0f;
+                }
+                cp_async_commit();
+            };
+            fetch(0, look(0));
+            fetch(1, look(1));
+            int page = look(2);
 #pragma unroll 1
-        for (int j = 0; j < ntiles; j++) {
-            const int st = j & 1;
-            if (j >= 2 && !kvp_wait(&k_empty[st], ((j >> 1) - 1) & 1, &s_fail)) break;
-            if (kin) {
+            for (int j = 0; j < ntiles; j++) {
+                const int st = j % ST;
+                cp_async_wait<1>();
+                if (j >= ST && !kvp_wait(&k_empty[st], (j / ST - 1) & 1, &s_fail)) break;
+                if (in) {
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const uint2 p0 = int8x4_to_half(kx[e].x), p1 = int8x4_to_half(kx[e].y), p2 = int8x4_to_half(kx[e].z),
-                                p3 = int8x4_to_half(kx[e].w);
-                    *reinterpret_cast<uint4*>(kto[0] + st * kKvpBlock + e * 2048) = make_uint4(p0.x, p0.y, p1.x, p1.y);
-                    *reinterpret_cast<uint4*>(kto[1] + st * kKvpBlock + e * 2048) = make_uint4(p2.x, p2.y, p3.x, p3.y);
-                }
-            }
-            // Words of tile j - 4: its softmax was over before S of tile j - 2 was issued, and k_empty says that was.
-            if (w4 == 0) {
-                KvpMeta& me = s_meta[j & 3];
-                const unsigned live = __ballot_sync(0xffffffffu, cur.at >= 0);
-                const unsigned nan = __ballot_sync(0xffffffffu, cur.ks != cur.ks || cur.vs != cur.vs);
-                if (lane < 8) {
-                    me.ks[lane] = cur.ks > 0.0f ? cur.ks : 1.0f;
-                    me.fv[lane] = cur.vs > 0.0f ? cur.vs * vinv : 0.0f;
-                }
-                if (lane == 0) {
-                    me.live = live & 0xFF;
-                    me.nan = nan & 0xFF;
-                }
-            }
-            fence_smem_async();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_addr(&k_full[st]));
-            cur = find(j + 1, page1);
-            page1 = look(j + 2);
-            load_k(cur, kx);
-            if (j >= 2 && !kvp_wait(&v_empty[st], ((j >> 1) - 1) & 1, &s_fail)) break;
-            if (vin) {
-                unsigned char* vb = vst + st * kKvpBlock;
-#pragma unroll
-                for (int w = 0; w < 4; w++) {
-                    uint32_t lo[4], hi[4];   // dimension 16 vc + 4 w + d: tokens 0..3, 4..7 of the eight
-                    const uint32_t* x = reinterpret_cast<const uint32_t*>(vx) + w;
-                    transpose4(x[0], x[4], x[8], x[12], lo);
-                    transpose4(x[16], x[20], x[24], x[28], hi);
-#pragma unroll
-                    for (int d = 0; d < 4; d++) {
-                        const uint2 p0 = int8x4_to_half(lo[d]), p1 = int8x4_to_half(hi[d]);
-                        *reinterpret_cast<uint4*>(vb + kvp_piece(16 * vc + 4 * w + d, tg)) = make_uint4(p0.x, p0.y, p1.x, p1.y);
+                    for (int e = 0; e < 4; e++) {
+                        const uint4 x = *reinterpret_cast<const uint4*>(mine + (j & 1) * kKvpRaw + 2048 * e);
+                        const uint2 p0 = int8x4_to_half(x.x), p1 = int8x4_to_half(x.y), p2 = int8x4_to_half(x.z),
+                                    p3 = int8x4_to_half(x.w);
+                        *reinterpret_cast<uint4*>(to0 + st * kKvpStage + e * 2048) = make_uint4(p0.x, p0.y, p1.x, p1.y);
+                        *reinterpret_cast<uint4*>(to1 + st * kKvpStage + e * 2048) = make_uint4(p2.x, p2.y, p3.x, p3.y);
                     }
                 }
-            }
-            fence_smem_async();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_addr(&v_full[st]));
-            load_v(cur, vx);
-        }
-    } else if (warp == 12) {
-        // ================= MMA issue =================
-        const uint32_t id_s = kvp_idesc(kKvpTile), id_o = kvp_idesc(c.hd);
-        const uint32_t qd = umma_lo(smem_addr(qs)), kd = umma_lo(smem_addr(kst)), vd = umma_lo(smem_addr(vst));
-        const int nk = c.hd / 16;
-        constexpr uint32_t kTile = kKvpBlock >> 4;   // an operand in units of 16 bytes; a k-step is 2, its second half kTile / 2 on
-        auto scores = [&](int j, int t) {
-            const int sb = TERMS == 2 ? j & 1 : t;
-            const uint32_t d = tmem + (TERMS == 2 ? 384 * sb : 128 * t), kb = kd + (j & 1) * kTile;
-#pragma unroll
-            for (int term = 0; term < TERMS; term++)
-#pragma unroll
-                for (int k = 0; k < 8; k++)
-                    if (k < nk) {
-                        const uint32_t off = (k >> 2) * (kTile / 2) + 2 * (k & 3);
-                        umma_f16_warp(d, umma_desc_of(qd + (t + term) * kTile + off), umma_desc_of(kb + off), id_s, (term | k) != 0);
+                // Words of tile j - 8: k_empty says that S of tile j - ST (4 at most) was issued, which P of the tile
+                // two before that preceded, so the softmax of both row tiles is past it.
+                if (w4 == 0) {
+                    __syncwarp();   // the scales that lanes 0..7 copied
+                    const float ks = s_scale[j & 1][lane & 3], vs = s_scale[j & 1][4 + (lane & 3)];
+                    KvpMeta& me = s_meta[j & 7];
+                    const unsigned live = __ballot_sync(0xffffffffu, ks != -1.0f);
+                    const unsigned nan = __ballot_sync(0xffffffffu, ks != ks || vs != vs);
+                    if (lane < 4) {
+                        me.ks[lane] = ks > 0.0f ? ks : 1.0f;
+                        me.fv[lane] = vs > 0.0f ? vs * vinv : 0.0f;
                     }
-            umma_commit_warp(smem_addr(&s_full[sb]));
-        };
-        auto values = [&](int j, int t) {
-            const uint32_t d = tmem + 256 + 128 * t, p = tmem + (TERMS == 2 ? 128 : 128 * t), vb = vd + (j & 1) * kTile;
-#pragma unroll
-            for (int term = 0; term < TERMS; term++)
-#pragma unroll
-                for (int k = 0; k < 8; k++)
-                    umma_f16_ts_warp(d, p + 64 * term + 8 * k, umma_desc_of(vb + (k >> 2) * (kTile / 2) + 2 * (k & 3)), id_o,
-                            (term | k) != 0 || j > 0);
-            umma_commit_warp(smem_addr(&pv_done[t]));
-        };
-        auto wait_for = [&](uint64_t* bar, int parity) { return (bool)__all_sync(0xffffffffu, kvp_wait(bar, parity & 1, &s_fail)); };
-        bool ok = ntiles == 0 || (wait_for(&q_full, 0) && wait_for(&k_full[0], 0));
-        tc_fence_after();
-        if (ok && ntiles > 0) {
-            for (int t = 0; t < nq; t++)
-                if (nt[NQ == 2 ? t : 0] > 0) scores(0, t);
-            umma_commit_warp(smem_addr(&k_empty[0]));
-        }
-        for (int j = 0; j < ntiles && ok; j++) {
-            const bool more = j + 1 < ntiles;
-            if (more) ok = wait_for(&k_full[(j + 1) & 1], (j + 1) >> 1);
-            tc_fence_after();
-            if (TERMS == 2 && more && ok) {   // S of the next tile goes to the other buffer, read two tiles ago
-                scores(j + 1, 0);
-                umma_commit_warp(smem_addr(&k_empty[(j + 1) & 1]));
+                    if (lane == 0) {
+                        me.live = live & 0xF;
+                        me.nan = nan & 0xF;
+                    }
+                }
+                fence_smem_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_addr(&k_full[st]));
+                fetch(j + 2, page);
+                page = look(j + 3);
             }
-            ok = ok && wait_for(&v_full[j & 1], j >> 1);
-            for (int t = 0; t < nq && ok; t++) {
-                const int mine = nt[NQ == 2 ? t : 0];
-                if (j >= mine) continue;
-                ok = wait_for(&p_full[t], j);
-                if (!ok) break;
+        } else {
+            const int tg = lane & 7, vd = 8 * ((lane >> 3) + 4 * w4);   // 8 tokens, 8 dimensions
+            const bool in = vd < c.hd;
+            const int8_t* src = c.v + a.layer * c.plane() + (8 * tg & 15) * c.hd + vd;
+            unsigned char *mine = raw + 2 * kKvpRaw + 8 * id;   // the thread's pieces, 1 KB apart
+            unsigned char* to = vst + vd * 128;
+            auto fetch = [&](int j, int page) {
+                const long long at = __shfl_sync(0xffffffffu, at_of(j, unit_of(j, page)), tg >> 1);
+                if (at >= 0 && in) {
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+                        asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(
+                                         smem_addr(mine + (j & 1) * kKvpRaw + 1024 * e)),
+                                     "l"(src + at + e * c.hd)
+                                     : "memory");
+                }
+                cp_async_commit();
+            };
+            fetch(0, look(0));
+            fetch(1, look(1));
+            int page = look(2);
+#pragma unroll 1
+            for (int j = 0; j < ntiles; j++) {
+                const int st = j % ST;
+                cp_async_wait<1>();
+                if (j >= ST && !kvp_wait(&v_empty[st], (j / ST - 1) & 1, &s_fail)) break;
+                if (in) {
+                    uint2 x[8];
+#pragma unroll
+                    for (int e = 0; e < 8; e++) x[e] = *reinterpret_cast<const uint2*>(mine + (j & 1) * kKvpRaw + 1024 * e);
+#pragma unroll
+                    for (int w = 0; w < 2; w++) {
+                        uint32_t lo[4], hi[4];   // dimension vd + 4 w + d: tokens 0..3, 4..7 of the eight
+                        auto word = [&](int e) { return w ? x[e].y : x[e].x; };
+                        transpose4(word(0), word(1), word(2), word(3), lo);
+                        transpose4(word(4), word(5), word(6), word(7), hi);
+#pragma unroll
+                        for (int d = 0; d < 4; d++) {   // vd is a multiple of 8: row & 7 is 4 w + d
+                            const uint2 p0 = int8x4_to_half(lo[d]), p1 = int8x4_to_half(hi[d]);
+                            *reinterpret_cast<uint4*>(to + st * kKvpStage + (4 * w + d) * 128 + ((tg ^ (4 * w + d)) << 4)) =
+                                make_uint4(p0.x, p0.y, p1.x, p1.y);
+                        }
+                    }
+                }
+                fence_smem_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_addr(&v_full[st]));
+                fetch(j + 2, page);
+                page = look(j + 3);
+            }
+        }
+        cp_async_wait<0>();
+    } else {
+        // ================= MMA issue, row tile t =================
+        regs_less<kKvpRegsMma>();
+        const int t = warp - 16, mine = t < NQ ? nt[t & 1] : 0;
+        if (t < NQ) {
+            // Descriptors count in 16 bytes; a k-step of 16 values is 2.
+            const uint32_t id_s = kvp_idesc(kKvpTile), id_o = kvp_idesc(c.hd);
+            const uint32_t qd = umma_lo(smem_addr(qs)), kd = umma_lo(smem_addr(kst)), vd = umma_lo(smem_addr(vst));
+            const int nk = c.hd / 16;
+            auto scores = [&](int j) {
+                const uint32_t d = tmem + 128 * t + 64 * (j & 1), kb = kd + (j % ST) * (kKvpStage >> 4);
+#pragma unroll
+                for (int term = 0; term < TERMS; term++)
+                    umma_run_ss(d, qd + (t * TERMS + term) * (kKvpQ >> 4), kb, kKvpQ >> 5, kKvpStage >> 5, id_s, nk, term);
+                umma_commit_warp(smem_addr(&s_full[t][j & 1]));
+            };
+            auto values = [&](int j) {
+                const uint32_t d = tmem + 256 + 128 * t, p = tmem + 128 * t + 64 * (j & 1), vb = vd + (j % ST) * (kKvpStage >> 4);
+#pragma unroll
+                for (int term = 0; term < TERMS; term++) umma_run4_ts(d, p + 32 * term, vb, id_o, term != 0 || j > 0);
+                umma_commit_warp(smem_addr(&pv_done[t]));
+            };
+            auto wait_for = [&](uint64_t* bar, int parity) { return kvp_wait(bar, parity & 1, &s_fail); };
+            // A wait that gives up is looked at once a turn: what is issued until then has no reader.
+            bool ok = ntiles == 0 || wait_for(&q_full, 0);
+            for (int j = 0; j < 2 && j < ntiles; j++) {
+                ok = wait_for(&k_full[j], 0) && ok;
                 tc_fence_after();
-                values(j, t);
-                if (TERMS == 1 && j + 1 < mine) {   // into the columns of the P just read
-                    ok = wait_for(&pv_done[t], j);
-                    if (!ok) break;
-                    tc_fence_after();
-                    scores(j + 1, t);
-                }
+                __syncwarp();
+                if (j < mine) scores(j);
+                umma_commit_warp(smem_addr(&k_empty[j]));
             }
-            if (!ok) break;
-            umma_commit_warp(smem_addr(&v_empty[j & 1]));
-            if (TERMS == 1 && more) umma_commit_warp(smem_addr(&k_empty[(j + 1) & 1]));
+#pragma unroll 1
+            for (int j = 0; j < ntiles && __all_sync(0xffffffffu, ok); j++) {
+                // a warp past its own tiles goes on at the others' pace, so that its commits count for the right tile
+                ok = wait_for(&v_full[j % ST], j / ST) && ok;
+                if (j < mine) ok = wait_for(&p_full[t][j & 1], j >> 1) && ok;
+                tc_fence_after();
+                __syncwarp();
+                if (j < mine) values(j);
+                if (j == mine - 1) umma_commit_warp(smem_addr(&o_full[t]));
+                umma_commit_warp(smem_addr(&v_empty[j % ST]));
+                if (j + 2 >= ntiles) continue;
+                ok = wait_for(&k_full[(j + 2) % ST], (j + 2) / ST) && ok;
+                if (j + 2 < mine) ok = wait_for(&pv_done[t], j) && ok;   // P of tile j lies where this S goes
+                tc_fence_after();
+                __syncwarp();
+                if (j + 2 < mine) scores(j + 2);
+                umma_commit_warp(smem_addr(&k_empty[(j + 2) % ST]));
+            }
+            umma_commit_warp(smem_addr(&done_bar));
         }
-        umma_commit_warp(smem_addr(&done_bar));
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 12) {
+    if (warp == 16) {
         mbar_wait(smem_addr(&done_bar), 0, kKvpWaitLimit);   // every MMA issued is complete
         __syncwarp();
         tc_fence_after();

@@ -11,10 +11,10 @@ namespace aion {
 // rows of 128 bytes, 8-row groups 1024 bytes apart (SBO), version 1.  Only
 // the low word depends on the address (umma_lo), in units of 16 bytes.
 __device__ __forceinline__ uint32_t umma_lo(uint32_t saddr) { return ((saddr >> 4) & 0x3FFFu) | (1u << 16); }
-__device__ __forceinline__ uint64_t umma_desc_of(uint32_t lo) {
-    return (uint64_t)lo | ((uint64_t)((1024u >> 4) | (1u << 14) | (2u << 29)) << 32);
+constexpr uint32_t kUmmaDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint64_t umma_desc_sw128(uint32_t saddr) {
+    return (uint64_t)umma_lo(saddr) | ((uint64_t)kUmmaDescHi << 32);
 }
-__device__ __forceinline__ uint64_t umma_desc_sw128(uint32_t saddr) { return umma_desc_of(umma_lo(saddr)); }
 
 // One tcgen05.mma of kind::f16 with both operands in shared memory: D (TMEM)
 // += A B^T, M and N and the operands' type (bf16 or fp16, the same for both)
@@ -34,27 +34,53 @@ __device__ __forceinline__ void umma_commit(uint32_t bar) {
                  : "memory");
 }
 
-// The same, called by a whole converged warp, of which one elected lane
-// issues: the operands stay in uniform registers.
-__device__ __forceinline__ void umma_f16_warp(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
-                                              uint32_t accumulate) {
+// A run of tcgen05.mma issued by one elected lane of a converged warp, in one
+// piece: D (TMEM) (+)= A B^T over `steps` (1..8) k-steps of 16 fp16 or bf16
+// values (the type by `idesc`), both operands in shared memory, in the
+// 128-byte-swizzled halves of 64 values that umma_lo points to; `half_a` and
+// `half_b` (in 16 bytes) lead to the second halves.
+// One piece, because the operands of each MMA pass through uniform registers,
+// and an election for each took longer than the MMA itself.
+#define UMMA_STEP(K, A, B)                                                     \
+    "setp.gt.and.s32 on, %6, " K ", lead;\n\t"                                 \
+    "add.u32 al, " A ";\n\tadd.u32 bl, " B ";\n\t"                             \
+    "mov.b64 ad, {al, %7};\n\tmov.b64 bd, {bl, %7};\n\t"                       \
+    "@on tcgen05.mma.cta_group::1.kind::f16 [%0], ad, bd, %3, one;\n\t"
+__device__ __forceinline__ void umma_run_ss(uint32_t tmem_d, uint32_t a, uint32_t b, uint32_t half_a, uint32_t half_b,
+                                            uint32_t idesc, int steps, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p, q;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "elect.sync _|q, 0xffffffff;\n\t"
-        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}"
-        ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(0), "r"(0), "r"(0), "r"(0)
+        "{\n\t.reg .pred lead, acc, one, on;\n\t.reg .b32 al, bl;\n\t.reg .b64 ad, bd;\n\t"
+        "elect.sync _|lead, 0xffffffff;\n\t"
+        "setp.ne.b32 acc, %5, 0;\n\t"
+        "setp.eq.b32 one, 0, 0;\n\t"
+        "mov.b64 ad, {%1, %7};\n\tmov.b64 bd, {%2, %7};\n\t"
+        "@lead tcgen05.mma.cta_group::1.kind::f16 [%0], ad, bd, %3, acc;\n\t"
+        UMMA_STEP("1", "%1, 2", "%2, 2") UMMA_STEP("2", "%1, 4", "%2, 4") UMMA_STEP("3", "%1, 6", "%2, 6")
+        UMMA_STEP("4", "%4, 0", "%8, 0") UMMA_STEP("5", "%4, 2", "%8, 2") UMMA_STEP("6", "%4, 4", "%8, 4")
+        UMMA_STEP("7", "%4, 6", "%8, 6") "}"
+        ::"r"(tmem_d), "r"(a), "r"(b), "r"(idesc), "r"(a + half_a), "r"(accumulate), "r"(steps), "r"(kUmmaDescHi),
+        "r"(b + half_b)
         : "memory");
 }
-// A from TMEM: lanes are rows, a column holds two 16-bit values along K.
-__device__ __forceinline__ void umma_f16_ts_warp(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc,
-                                                 uint32_t accumulate) {
+#undef UMMA_STEP
+// The same with A in TMEM (lanes are rows, a column holds two values along K)
+// and four k-steps, in one half of B.
+__device__ __forceinline__ void umma_run4_ts(uint32_t tmem_d, uint32_t tmem_a, uint32_t b, uint32_t idesc,
+                                             uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p, q;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "elect.sync _|q, 0xffffffff;\n\t"
-        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n\t}"
-        ::"r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(0), "r"(0), "r"(0), "r"(0)
+        "{\n\t.reg .pred lead, acc, one;\n\t.reg .b32 al, bl;\n\t.reg .b64 bd;\n\t"
+        "elect.sync _|lead, 0xffffffff;\n\t"
+        "setp.ne.b32 acc, %4, 0;\n\t"
+        "setp.eq.b32 one, 0, 0;\n\t"
+        "mov.b64 bd, {%2, %5};\n\t"
+        "@lead tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], bd, %3, acc;\n\t"
+        "add.u32 al, %1, 8;\n\tadd.u32 bl, %2, 2;\n\tmov.b64 bd, {bl, %5};\n\t"
+        "@lead tcgen05.mma.cta_group::1.kind::f16 [%0], [al], bd, %3, one;\n\t"
+        "add.u32 al, %1, 16;\n\tadd.u32 bl, %2, 4;\n\tmov.b64 bd, {bl, %5};\n\t"
+        "@lead tcgen05.mma.cta_group::1.kind::f16 [%0], [al], bd, %3, one;\n\t"
+        "add.u32 al, %1, 24;\n\tadd.u32 bl, %2, 6;\n\tmov.b64 bd, {bl, %5};\n\t"
+        "@lead tcgen05.mma.cta_group::1.kind::f16 [%0], [al], bd, %3, one;\n\t}"
+        ::"r"(tmem_d), "r"(tmem_a), "r"(b), "r"(idesc), "r"(accumulate), "r"(kUmmaDescHi)
         : "memory");
 }
 __device__ __forceinline__ void umma_commit_warp(uint32_t bar) {
