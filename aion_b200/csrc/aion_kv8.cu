@@ -355,8 +355,6 @@ extern "C" AION_API aion_status aion_kv8_read(const aion_kv8* kv, int32_t layer,
 constexpr int kTileRows = 32;
 static bool attention_tiles(int n_seq, int n_tok, int group) { return (int64_t)n_tok * group >= (int64_t)kTileRows * n_seq; }
 
-// Blocks of k_kv_attention: one an SM with 128-dimension slots, two with 64.
-static int attention_blocks(const aion_kv8* kv) { return sm_count(kv->device) * (kv->head_size <= 64 ? 2 : 1); }
 // Units of at most this many groups of 64 keys go to one block whole: no join
 // launch.
 constexpr int kWholeGroups = 8;
@@ -369,24 +367,33 @@ extern "C" AION_API int64_t aion_kv8_attention_workspace(const aion_kv8* kv, int
     if (check_shape(kv, "aion_kv8_attention_workspace") != AION_OK) return -1;
     if (n_heads < 1 || n_heads % kv->n_kv_heads || n_seq < 0 || n_tok < 0) return -1;
     if (attention_tiles(n_seq, n_tok, n_heads / kv->n_kv_heads)) return 0;
-    return attention_whole(kv) ? 0 : (int64_t)attention_blocks(kv) * 2 * sizeof(KvPart);
+    return attention_whole(kv) ? 0 : (int64_t)sm_count(kv->device) * 2 * 2 * sizeof(KvPart);   // two blocks an SM at most
 }
 
-template <typename T, int HDP, int D>
-static cudaError_t launch_attention(const KvAttnArgs& a, int blocks, int dev, cudaStream_t st) {
+template <typename T, int HDP, int D, bool WIDE>
+static cudaError_t launch_attention(KvAttnArgs a, int dev, cudaStream_t st) {
+    using SH = KvaShape<HDP, D, WIDE>;
     static std::atomic<uint64_t> opted{0};   // devices whose shared-memory limit is raised
     const uint64_t bit = dev >= 0 && dev < 64 ? 1ull << dev : 0;
     if (!bit || !(opted.load() & bit)) {
-        const cudaError_t e = cudaFuncSetAttribute(k_kv_attention<T, HDP, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                   KvaSmem<HDP>::kTotal);
+        const cudaError_t e = cudaFuncSetAttribute(k_kv_attention<T, HDP, D, WIDE>,
+                                                   cudaFuncAttributeMaxDynamicSharedMemorySize, SH::kTotal);
         if (e != cudaSuccess) return e;
         opted.fetch_or(bit);
     }
-    k_kv_attention<T, HDP, D><<<blocks, kKvaThreads, KvaSmem<HDP>::kTotal, st>>>(a);
+    a.unit_log = SH::kUnitLog;
+    const int blocks = sm_count(dev) * SH::kBlocks;
+    k_kv_attention<T, HDP, D, WIDE><<<blocks, kKvaThreads, SH::kTotal, st>>>(a);
     cudaError_t e = cudaGetLastError();
     if (e == cudaSuccess && !a.whole && blocks > 1)
         e = launch_pdl(k_kv_attention_join<T>, dim3(blocks - 1), dim3(kKvJoinThreads), 0, st, a, blocks);
     return e;
+}
+template <typename T, int D>
+static cudaError_t launch_attention_of(const KvAttnArgs& a, int rows, int dev, cudaStream_t st) {
+    const bool wide = rows > (D == 2 ? 4 : 2);
+    if (a.c.hd > 64) return wide ? launch_attention<T, 128, D, true>(a, dev, st) : launch_attention<T, 128, D, false>(a, dev, st);
+    return wide ? launch_attention<T, 64, D, true>(a, dev, st) : launch_attention<T, 64, D, false>(a, dev, st);
 }
 
 template <typename T>
@@ -447,6 +454,7 @@ extern "C" AION_API aion_status aion_kv8_attention(const aion_kv8* kv, int32_t l
     a.vec_out = vectors(out, out_stride, type);
     a.whole = attention_whole(kv);
     a.parts = (KvPart*)workspace;
+    a.unit_log = 0;
     const cudaStream_t st = (cudaStream_t)stream;
     if (attention_tiles(n_seq, n_tok, a.group)) {
         if (type == AION_F32) KV_CUDA((launch_prompt<float>(a, kv->device, st)));
@@ -454,18 +462,11 @@ extern "C" AION_API aion_status aion_kv8_attention(const aion_kv8* kv, int32_t l
         else KV_CUDA((launch_prompt<__nv_bfloat16>(a, kv->device, st)));
         return AION_OK;
     }
-    const int blocks = attention_blocks(kv);
-    const bool wide = kv->head_size > 64;
+    const int rows = (int)(((int64_t)n_tok + n_seq - 1) / n_seq * a.group);   // of a K/V head, on average
     cudaError_t e;
-    if (type == AION_F32)
-        e = wide ? launch_attention<float, 128, 3>(a, blocks, kv->device, st)
-                 : launch_attention<float, 64, 3>(a, blocks, kv->device, st);
-    else if (type == AION_F16)
-        e = wide ? launch_attention<__half, 128, 2>(a, blocks, kv->device, st)
-                 : launch_attention<__half, 64, 2>(a, blocks, kv->device, st);
-    else
-        e = wide ? launch_attention<__nv_bfloat16, 128, 2>(a, blocks, kv->device, st)
-                 : launch_attention<__nv_bfloat16, 64, 2>(a, blocks, kv->device, st);
+    if (type == AION_F32) e = launch_attention_of<float, 3>(a, rows, kv->device, st);
+    else if (type == AION_F16) e = launch_attention_of<__half, 2>(a, rows, kv->device, st);
+    else e = launch_attention_of<__nv_bfloat16, 2>(a, rows, kv->device, st);
     KV_CUDA(e);
     return AION_OK;
 }

@@ -17,6 +17,7 @@ struct KvAttnArgs {
     long long q_stride, out_stride;
     float scale;                 // of the scores, times log2(e): the softmax is in base 2
     int vec_q, vec_out;          // rows are 16-byte aligned
+    int unit_log;                // rows of a unit of k_kv_attention: 1 << unit_log
     int whole;                   // blocks take whole units: nothing is left to join
     struct KvPart* parts;        // [blocks][2], else
 };
@@ -32,12 +33,16 @@ struct KvAttnArgs {
 //   out += V scale * 2^(group max - running max) / (256^D - 1) * sum_d ....
 // D is 3 for fp32 rows (a step of 2^-23 of the largest value: fp32's own) and
 // 2 for 16-bit rows (2^-15, against the 2^-8 or 2^-11 of a rounded result).
-// Digits of one row are columns of different MMAs, so a lane joins them
-// without an exchange.  Weights are relative to the largest of their 64
-// positions, so a position far below its row's maximum keeps its share.  Sums
-// run in fp32.
+// Weights are relative to the largest of their 64 positions, so a position far
+// below its row's maximum keeps its share.  Sums run in fp32.
 //
-// Work.  A unit is (sequence, K/V head, up to 8 rows: tokens x query heads of
+// Rows and digits are the columns of the MMAs (8 of them).  WIDE: 8 rows, an
+// MMA for each digit, which a lane joins by itself.  Else one MMA holds 4 rows
+// x 2 digits (lane t of a quad has both of row t) or 2 rows x 3 digits in fours
+// (two lanes have a row and swap halves), and half or less of the work around
+// the MMAs is left: one query head per K/V head, or few, as most models decode.
+//
+// Work.  A unit is (sequence, K/V head, so many rows: tokens x query heads of
 // that K/V head); its keys come in groups of 64.  All groups of all units form
 // one line that is cut evenly over the blocks and, in a block, over its warps,
 // so uneven lengths and one long sequence load the card alike.  A warp streams
@@ -49,11 +54,11 @@ struct KvAttnArgs {
 // Memory.  Each warp has a ring of three slots of 64 rows; K and V slots
 // alternate, so two slots (16 KB a warp, 128 KB an SM) are in flight while one
 // is used.  16 rows of a page and head are contiguous: a lane copies 16-byte
-// pieces (cp.async).  K fragments are 16-byte shared-memory reads (the order
-// of the dimensions inside a dot is free, as q's digits take the same order);
-// V fragments need four tokens of one dimension in a word: four words of four
-// tokens, transposed with byte permutes.  The pieces are XOR-swizzled so that
-// both reads touch every bank once.
+// pieces (cp.async), XOR-swizzled so that the eight rows that one phase of an
+// ldmatrix reads lie in different banks.  K fragments (tokens x dimensions) are
+// plain ldmatrix, V fragments (dimensions x tokens) its transposing 8-bit form.
+// Page numbers and scales pass through shared memory, too: a register that
+// waits for memory would hold up the warp when the pipeline moves on.
 // ---------------------------------------------------------------------------
 constexpr int kKvaWarps = 8, kKvaThreads = 32 * kKvaWarps, kKvaT = 64, kKvaRows = 8;
 
@@ -83,6 +88,21 @@ __device__ __forceinline__ void mma_su(int (&d)[4], const uint32_t (&a)[4], uint
         : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// 16 rows x 32 bytes as an A fragment: lanes 0..15 give the rows' first 16
+// bytes, lanes 16..31 their second.
+__device__ __forceinline__ void ldsm_rows(uint32_t (&a)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3])
+                 : "r"(addr)
+                 : "memory");
+}
+// 32 rows x 16 bytes, transposed, as an A fragment of 16 x 32: lane i gives row i.
+__device__ __forceinline__ void ldsm_cols(uint32_t (&a)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m16n16.x2.trans.shared.b8 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3])
+                 : "r"(addr)
+                 : "memory");
+}
 // Four words of four bytes, transposed.
 __device__ __forceinline__ void transpose4(uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t (&r)[4]) {
     const uint32_t ab0 = __byte_perm(a, b, 0x5140), ab1 = __byte_perm(a, b, 0x7362);
@@ -96,16 +116,9 @@ template <int N> __device__ __forceinline__ void cp_async_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-
-template <int D> struct KvDigits {
-    static constexpr float kQ = D == 3 ? 127.0f * 65536.0f : 127.0f * 256.0f;
-    static constexpr float kP = D == 3 ? 16777215.0f : 65535.0f;
-    // sum over the digits of 256^(D-1-d) c[d]; each c[d] is below 2^24
-    static __device__ __forceinline__ float join(const int (&c)[D][4], int e) {
-        if constexpr (D == 3) return fmaf((float)c[0][e], 65536.0f, fmaf((float)c[1][e], 256.0f, (float)c[2][e]));
-        else return fmaf((float)c[0][e], 256.0f, (float)c[1][e]);
-    }
-};
+__device__ __forceinline__ void cp_async4(void* dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_addr(dst)), "l"(src) : "memory");
+}
 
 // What a call says about sequence s.
 struct KvSeq {
@@ -123,7 +136,7 @@ __device__ __forceinline__ KvSeq kv_seq(const KvAttnArgs& a, int s) {
     q.len = (int)min(len, (long long)a.c.max_pages << a.c.page_log);
     // a sequence that sees nothing has one group without keys: its rows become zero
     q.ng = q.cnt ? max((q.len + kKvaT - 1) / kKvaT, 1) : 0;
-    q.nrg = (q.cnt * a.group + kKvaRows - 1) / kKvaRows;
+    q.nrg = (q.cnt * a.group + (1 << a.unit_log) - 1) >> a.unit_log;
     return q;
 }
 
@@ -160,62 +173,83 @@ struct KvCursor {
     }
 };
 
-template <int HDP> struct KvaSmem {
-    static constexpr int kSlot = kKvaT * HDP;
-    static constexpr int kRing = 3 * kSlot;
-    static constexpr int kPiece = (kKvaRows * HDP + 2 * kKvaRows) * 4;   // o, m, l
-    struct Info {   // of a piece; the unit's groups from the block's first one on
-        int begin, end, s, h, rg, valid;
-    };
-    static_assert(kPiece % 16 == 0 && kRing % 16 == 0 && kKvaRows * 68 * 4 <= kSlot, "float4 pieces, the weights' place");
-    static constexpr int kInfo = kKvaWarps * kRing + kKvaWarps * kPiece;
-    static constexpr int kTotal = kInfo + 2 * kKvaWarps * (int)sizeof(Info);
-};
-
 // Rows of a unit as the lanes see them.
 struct KvRow {
-    long long q, out;   // element offsets
-    int lim;            // last position seen; -1: no row
+    long long q, out;   // element offsets; out -1: no row
+    int lim;            // last position seen; -1: none
 };
 __device__ __forceinline__ KvRow kv_row(const KvAttnArgs& a, const KvSeq& q, int h, int rg, int r) {
     KvRow w;
-    const int i = rg * kKvaRows + r, tok = i / a.group, head = h * a.group + (i - tok * a.group);
-    w.lim = i < q.cnt * a.group ? (int)min((long long)q.p0 + tok, (long long)q.len - 1) : -1;
+    const int i = (rg << a.unit_log) + r, tok = i / a.group, head = h * a.group + (i - tok * a.group);
+    const bool row = i < q.cnt * a.group;
+    w.lim = row ? (int)min((long long)q.p0 + tok, (long long)q.len - 1) : -1;
     w.q = (q.t0 + tok) * a.q_stride + (long long)head * a.c.hd;
-    w.out = i < q.cnt * a.group ? (q.t0 + tok) * a.out_stride + (long long)head * a.c.hd : -1;
+    w.out = row ? (q.t0 + tok) * a.out_stride + (long long)head * a.c.hd : -1;
     return w;
 }
 
+// Four consecutive values; `vec`: rows start on 16 bytes.
+template <typename T>
+__device__ __forceinline__ float4 load4(const T* p, bool vec) {
+    T t[4];
+    if (vec) {
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(t) = *reinterpret_cast<const uint4*>(p);
+        else *reinterpret_cast<uint2*>(t) = *reinterpret_cast<const uint2*>(p);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) t[i] = p[i];
+    }
+    return make_float4(to_f32(t[0]), to_f32(t[1]), to_f32(t[2]), to_f32(t[3]));
+}
 template <typename T>
 __device__ __forceinline__ void store4(T* p, bool vec, float4 x) {
+    T t[4] = {from_f32<T>(x.x), from_f32<T>(x.y), from_f32<T>(x.z), from_f32<T>(x.w)};
     if (vec) {
-        if constexpr (sizeof(T) == 4) {
-            *reinterpret_cast<float4*>(p) = x;
-        } else {
-            T t[4] = {from_f32<T>(x.x), from_f32<T>(x.y), from_f32<T>(x.z), from_f32<T>(x.w)};
-            *reinterpret_cast<uint2*>(p) = *reinterpret_cast<uint2*>(t);
-        }
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(p) = *reinterpret_cast<uint4*>(t);
+        else *reinterpret_cast<uint2*>(p) = *reinterpret_cast<uint2*>(t);
     } else {
-        p[0] = from_f32<T>(x.x);
-        p[1] = from_f32<T>(x.y);
-        p[2] = from_f32<T>(x.z);
-        p[3] = from_f32<T>(x.w);
+#pragma unroll
+        for (int i = 0; i < 4; i++) p[i] = t[i];
     }
 }
 
-template <typename T, int HDP, int D>
-__global__ void __launch_bounds__(kKvaThreads, HDP == 64 ? 2 : 1) k_kv_attention(const KvAttnArgs a) {
-    using SM = KvaSmem<HDP>;
-    using DG = KvDigits<D>;
-    constexpr int NW = HDP / 32;    // 32-dimension segments
-    constexpr int NP = HDP / 64;    // pairs of k-steps of the score dot
+template <int HDP, int D, bool WIDE> struct KvaShape {
+    static constexpr int kUnitLog = WIDE ? 3 : D == 2 ? 2 : 1, kUnit = 1 << kUnitLog;   // rows
+    static constexpr int kSlot = kKvaT * HDP;
+    static constexpr int kRing = 3 * kSlot;
+    static constexpr int kPiece = (kUnit * HDP + 2 * kUnit) * 4;   // o, m, l
+    static constexpr int kWords = D == 2 && !WIDE ? 36 : 68;   // of a row of weights: 64 of them (16-bit for 4 rows x 2 digits), padded
+    static_assert(kRing % 16 == 0 && kUnit * kWords * 4 <= kSlot && kPiece <= kRing && kPiece % 16 == 0, "the places of the weights and pieces");
+    struct Info {   // of a piece; the unit's groups from the block's first one on
+        int begin, end, s, h, rg, valid;
+    };
+    static constexpr int kQueue = (4 * 4 + 4 * 8) * 4;   // pages and scales of four groups
+    static constexpr int kPieces = kKvaWarps * kRing, kQueues = kPieces + kKvaWarps * kPiece;
+    static constexpr int kInfo = kQueues + kKvaWarps * kQueue;
+    static constexpr int kSums = kInfo + 2 * kKvaWarps * (int)sizeof(Info);   // warps' sums, the block's stretch
+    static constexpr int kTotal = kSums + (kKvaWarps + 2) * 8;
+    static_assert(kSums % 8 == 0 && kTotal <= 227 * 1024, "shared memory");
+    static constexpr int kBlocks = 2 * (kTotal + 1024 + 128) <= 228 * 1024 ? 2 : 1;   // blocks an SM has room for
+};
+
+template <typename T, int HDP, int D, bool WIDE>
+__global__ void __launch_bounds__(kKvaThreads, KvaShape<HDP, D, WIDE>::kBlocks) k_kv_attention(const KvAttnArgs a) {
+    using SH = KvaShape<HDP, D, WIDE>;
+    constexpr float kQ = D == 3 ? 127.0f * 65536.0f : 127.0f * 256.0f, kP = D == 3 ? 16777215.0f : 65535.0f;
+    constexpr int KS = HDP / 32, MT = HDP / 16;   // k-steps of a score, 16-dimension tiles of a result
+    constexpr int RL = WIDE ? 2 : 1;              // rows a lane has scores of
+    constexpr int NV = WIDE ? 4 : D == 2 ? 2 : 1; // its scores of 16 positions
+    constexpr int ND = WIDE ? D : 1;              // MMAs for the digits
     extern __shared__ __align__(16) unsigned char smem[];
-    __shared__ long long s_range[2], s_red[kKvaWarps];
+    if (!a.whole) pdl_launch_dependents();   // the join's launch overlaps; it waits for this grid before it reads
     const KvView& c = a.c;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    unsigned char* ring = smem + warp * SM::kRing;
-    float* piece0 = reinterpret_cast<float*>(smem + kKvaWarps * SM::kRing + warp * SM::kPiece);
-    typename SM::Info* info = reinterpret_cast<typename SM::Info*>(smem + SM::kInfo);
+    unsigned char* ring = smem + warp * SH::kRing;
+    float* piece0 = reinterpret_cast<float*>(smem + SH::kPieces + warp * SH::kPiece);
+    int* q_page = reinterpret_cast<int*>(smem + SH::kQueues + warp * SH::kQueue);   // [4][4]: of the 16-key tiles of a group
+    float* q_scale = reinterpret_cast<float*>(q_page + 16);                         // [4][8]: K scales, V scales
+    typename SH::Info* info = reinterpret_cast<typename SH::Info*>(smem + SH::kInfo);
+    long long *s_red = reinterpret_cast<long long*>(smem + SH::kSums), *s_range = s_red + kKvaWarps;
 
     // ---- the line: prefix sums of the sequences' groups (in the ring's memory), the block's and the warp's stretch
     long long* pre = reinterpret_cast<long long*>(smem);
@@ -225,6 +259,7 @@ __global__ void __launch_bounds__(kKvaThreads, HDP == 64 ? 2 : 1) k_kv_attention
     for (int s = sa; s < sb; s++) {
         const KvSeq q = kv_seq(a, s);
         if (blockIdx.x == 0) kv_vet_seq(a, q);
+        pre[s] = mine;
         mine += (long long)q.ng * q.nrg * c.nkv;
     }
     long long x = mine;
@@ -235,18 +270,13 @@ __global__ void __launch_bounds__(kKvaThreads, HDP == 64 ? 2 : 1) k_kv_attention
     }
     if (lane == 31) s_red[warp] = x;
     __syncthreads();
-    long long W = 0, base = 0;
+    long long W = 0, base = x - mine;
+#pragma unroll
     for (int w = 0; w < kKvaWarps; w++) {
-        if (w == warp) base = W;
+        if (w < warp) base += s_red[w];
         W += s_red[w];
     }
-    long long run = base + x - mine;
-    for (int s = sa; s < sb; s++) {
-        pre[s] = run;
-        const KvSeq q = kv_seq(a, s);
-        run += (long long)q.ng * q.nrg * c.nkv;
-    }
-    if (threadIdx.x == 0) pre[a.r.n_seq] = W;
+    for (int s = sa; s < sb; s++) pre[s] += base;
     __syncthreads();
     auto find = [&](long long v) {   // the sequence that group v < W lies in
         int lo = 0, hi = a.r.n_seq - 1;
@@ -259,367 +289,367 @@ __global__ void __launch_bounds__(kKvaThreads, HDP == 64 ? 2 : 1) k_kv_attention
     };
     // a group for each warp at least: few blocks where there is little to do
     const long long nb = min((long long)gridDim.x, (W + kKvaWarps - 1) / kKvaWarps);
-    if (threadIdx.x < 2) {
-        const long long b = blockIdx.x + threadIdx.x;
-        long long v = b >= nb ? W : W * b / nb;
-        if (a.whole && v < W) {   // up to the next unit's start
-            const int s = find(v);
-            const long long ng = kv_seq(a, s).ng, rest = v - pre[s];
-            v = pre[s] + (rest + ng - 1) / ng * ng;
+    long long b0 = blockIdx.x >= nb ? W : W * blockIdx.x / nb, b1 = blockIdx.x + 1 >= nb ? W : W * (blockIdx.x + 1) / nb;
+    if (a.whole) {   // up to the next unit's start
+        if (threadIdx.x < 2) {
+            long long v = threadIdx.x ? b1 : b0;
+            if (v < W) {
+                const int s = find(v);
+                const long long ng = kv_seq(a, s).ng, rest = v - pre[s];
+                v = pre[s] + (rest + ng - 1) / ng * ng;
+            }
+            s_range[threadIdx.x] = v;
         }
-        s_range[threadIdx.x] = v;
+        __syncthreads();
+        b0 = s_range[0];
+        b1 = s_range[1];
     }
-    __syncthreads();
-    const long long b0 = s_range[0], b1 = s_range[1];
     const long long w0 = b0 + (b1 - b0) * warp / kKvaWarps, w1 = b0 + (b1 - b0) * (warp + 1) / kKvaWarps;
     const int n = (int)(w1 - w0);
-    KvCursor cur, ahead;   // the group in use; the group whose pages are looked up
+    KvCursor ahead;   // the group whose pages are looked up next
     if (n > 0) {
         const int s = find(w0);
-        cur.seek(a, s, w0 - pre[s]);
-        ahead = cur;
+        ahead.seek(a, s, w0 - pre[s]);
     }
     if (lane < 2) info[2 * warp + lane].valid = 0;
     __syncthreads();   // the ring is free
 
     // ---- copies
-    // A lane's pieces of 16 rows: source 16 (lane + 32 e), destinations swizzled.
-    constexpr int NE = HDP / 32;
-    int kdst[NE], vdst[NE];
+    constexpr int NE = HDP / 32;   // a lane's pieces of 16 rows: source 16 (lane + 32 e)
+    int dst[NE];
     const int cpr = c.hd / 16;
-#pragma unroll
-    for (int e = 0; e < NE; e++) {
-        const int i = lane + 32 * e, row = i / cpr, ch = i - row * cpr;
-        if constexpr (HDP == 128) {
-            kdst[e] = row * 128 + (ch ^ (4 * (row & 1))) * 16;
-            vdst[e] = row * 128 + ((ch >> 1) ^ ((row >> 2) & 3)) * 32 + (ch & 1) * 16;
-        } else {
-            kdst[e] = row * 64 + ch * 16;
-            vdst[e] = row * 64 + ((ch >> 1) ^ ((row >> 2) & 1)) * 32 + (ch & 1) * 16;
-        }
-    }
-    struct Item {   // pages (lanes 4 i + j: tile j of 16 positions; -1: none), place
-        int page, h, g, want;
+    auto place = [](int row, int ch) {
+        return HDP == 128 ? row * 128 + ((ch ^ (row & 7)) << 4) : row * 64 + ((ch ^ ((row >> 1) & 3)) << 4);
     };
-    auto look = [&](const KvCursor& k) {
-        Item it;
-        it.h = k.h;
-        it.g = k.g;
-        it.page = -1;
-        const int pos = k.g * kKvaT + 16 * t;
-        it.want = pos < k.q.len;
-        if (it.want) it.page = c.tables[(size_t)k.q.slot * c.max_pages + (pos >> c.page_log)];
+#pragma unroll
+    for (int e = 0; e < NE; e++) dst[e] = place((lane + 32 * e) / cpr, (lane + 32 * e) % cpr);
+    struct Item {   // a group of the line; g: its number in the unit, the sign bit says that it is the unit's last
+        int s, h, rg, g;
+    };
+    // The next group's place; its pages (lane j < 4: of 16 keys; -2: past the keys) go to queue entry k.
+    auto take = [&](int k) {
+        Item it = {ahead.s, ahead.h, ahead.rg, ahead.g | (ahead.g + 1 == ahead.q.ng ? (int)0x80000000 : 0)};
+        if (lane < 4) {
+            const int pos = ahead.g * kKvaT + 16 * lane;
+            int* to = q_page + 4 * k + lane;
+            if (pos < ahead.q.len) cp_async4(to, c.tables + (size_t)ahead.q.slot * c.max_pages + (pos >> c.page_log));
+            else *to = -2;
+        }
+        ahead.next(a);
         return it;
     };
-    auto vet = [&](Item& it) {   // pages that are missing are left out
-        if (it.page < 0 || it.page >= c.n_pages) {
-            if (it.want) kv_flag(c, KV_BAD_PAGE);
-            it.page = -1;
+    // Rows of a group to a slot; `with_scales`: K, with which the scales of both come.
+    auto copy = [&](const Item& it, int k, const int8_t* pool, int slot, bool with_scales) {
+        int page = q_page[4 * k + t];
+        if (page < 0 || page >= c.n_pages) {   // pages that are missing are left out
+            if (page != -2 && with_scales) kv_flag(c, KV_BAD_PAGE);
+            page = -1;
         }
-    };
-    auto copy = [&](const Item& it, const int8_t* pool, const int (&dst)[NE], int slot) {
-        const uint32_t to = smem_addr(ring + slot * SM::kSlot);
+        const long long unit = (long long)page * c.nkv + it.h;
+        if (with_scales && lane < 8) {
+            float* to = q_scale + 8 * k + lane;
+            if (page >= 0) cp_async4(to, (lane < 4 ? c.k_scale : c.v_scale) + (long long)a.layer * c.n_pages * c.nkv + unit);
+            else *to = -1.0f;
+        }
+        const int row0 = (it.g & 0x7FFFFFFF) * kKvaT + 16 * t;
+        const long long at = page < 0 ? -1 : (unit * c.page + (row0 & (c.page - 1))) * c.hd;
+        const uint32_t to = smem_addr(ring + slot * SH::kSlot);
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            const int page = __shfl_sync(0xffffffffu, it.page, j);
-            if (page < 0) continue;
-            const int8_t* from =
-                pool + (((long long)page * c.nkv + it.h) * c.page + ((it.g * kKvaT + 16 * j) & (c.page - 1))) * c.hd;
+            const long long from = __shfl_sync(0xffffffffu, at, j);
+            if (from < 0) continue;
+            const int8_t* src = pool + from + 16 * lane;
 #pragma unroll
             for (int e = 0; e < NE; e++)
                 if (lane + 32 * e < c.hd)
                     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + j * 16 * HDP + dst[e]),
-                                 "l"(from + 16 * (lane + 32 * e))
+                                 "l"(src + 512 * e)
                                  : "memory");
         }
     };
     const int8_t *kp = c.k + a.layer * c.plane(), *vp = c.v + a.layer * c.plane();
-    const float* scales = (lane < 4 ? c.k_scale : c.v_scale) + (long long)a.layer * c.n_pages * c.nkv;
-    auto scale_of = [&](const Item& it) {   // lanes 0..3: K scales of the tiles, 4..7: V scales
-        return it.page >= 0 ? scales[(long long)it.page * c.nkv + it.h] : 0.0f;
-    };
 
     // ---- state of the unit in use
-    float o[NW][2][4], m[2], l[2], rs[2];
-    int lim[2];
-    uint32_t qd[D][NP][4];
-    bool fresh = true;   // the unit began in this warp's stretch
-    auto begin_unit = [&]() {
+    auto my_row = [&](int e) { return WIDE ? 2 * t + e : D == 2 ? t : t >> 1; };   // rows a lane has scores of
+    float o[MT][NV], m[RL], l[RL], rs[RL];
+    int lim[RL];
+    uint32_t qd[ND][KS][2];
+    // Lane (g, t) brings column g of the score MMAs: a row, or a digit of one; dimensions 32 k + 4 t..+3 and + 16.
+    auto begin_unit = [&](const Item& it) {
 #pragma unroll
-        for (int w = 0; w < NW; w++)
+        for (int i = 0; i < MT; i++)
 #pragma unroll
-            for (int i = 0; i < 8; i++) o[w][i >> 2][i & 3] = 0.0f;
-        m[0] = m[1] = -INFINITY;
-        l[0] = l[1] = 0.0f;
-        // lane (g, t): row g, dimensions 16 (4 p + t)..+15
-        const KvRow row = kv_row(a, cur.q, cur.h, cur.rg, g);
-        float v[NP][16], top = 0.0f;
+            for (int e = 0; e < NV; e++) o[i][e] = 0.0f;
+        const KvSeq q = kv_seq(a, it.s);
+        const KvRow row = kv_row(a, q, it.h, it.rg, WIDE ? g : D == 2 ? g >> 1 : g >> 2);
+        float4 v[KS][2];
+        float top = 0.0f;
         bool bad = false;
 #pragma unroll
-        for (int p = 0; p < NP; p++) {
-            const int d0 = 16 * (4 * p + t);
-            if (row.lim >= 0 && d0 < c.hd) {
-                load16((const T*)a.q + row.q + d0, a.vec_q, v[p]);
-            } else {
+        for (int k = 0; k < KS; k++)
 #pragma unroll
-                for (int i = 0; i < 16; i++) v[p][i] = 0.0f;
-            }
-#pragma unroll
-            for (int i = 0; i < 16; i++) {
-                const float b = fabsf(v[p][i]);
-                bad = bad || !(b <= 3.402823466e38f);
+            for (int i = 0; i < 2; i++) {
+                const int d0 = 32 * k + 16 * i + 4 * t;
+                v[k][i] = row.lim >= 0 && d0 < c.hd ? load4((const T*)a.q + row.q + d0, a.vec_q) : make_float4(0, 0, 0, 0);
+                const float b = fmaxf(fmaxf(fabsf(v[k][i].x), fabsf(v[k][i].y)), fmaxf(fabsf(v[k][i].z), fabsf(v[k][i].w)));
+                const float sum = (v[k][i].x + v[k][i].y) + (v[k][i].z + v[k][i].w);
+                bad = bad || !(b <= 3.402823466e38f) || sum != sum;   // max leaves a NaN out, a sum does not
                 top = fmaxf(top, b);
             }
-        }
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const unsigned bads = __ballot_sync(0xffffffffu, bad);
-        bad = (bads >> (4 * g)) & 15;
+        bad = (__ballot_sync(0xffffffffu, bad) >> (4 * g)) & 15;
         // rows of tiny values are scaled up first, so that the factor stays finite
         const float up = top < 8.6736174e-19f ? 1.8446744e19f : 1.0f;   // 2^-60, 2^64
-        const float f = top > 0.0f && !bad ? DG::kQ / (top * up) : 0.0f;
+        const float f = top > 0.0f && !bad ? kQ / (top * up) : 0.0f;
 #pragma unroll
-        for (int p = 0; p < NP; p++)
+        for (int k = 0; k < KS; k++)
 #pragma unroll
-            for (int w = 0; w < 4; w++) {
-                int d[D][4];
+            for (int i = 0; i < 2; i++) {
+                const float* w = reinterpret_cast<const float*>(&v[k][i]);
+                int dg[D][4];
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    int z = bad ? 0 : __float2int_rn(v[p][4 * w + i] * up * f);
+                for (int e = 0; e < 4; e++) {
+                    int z = bad ? 0 : __float2int_rn(w[e] * up * f);
 #pragma unroll
-                    for (int k = D - 1; k >= 0; k--) {
-                        d[k][i] = (int8_t)z;
-                        z = (z - d[k][i]) >> 8;
+                    for (int d = D - 1; d >= 0; d--) {
+                        dg[d][e] = (int8_t)z;
+                        z = (z - dg[d][e]) >> 8;
                     }
                 }
+                uint32_t pk[D];
 #pragma unroll
-                for (int k = 0; k < D; k++) qd[k][p][w] = pack4(d[k][0], d[k][1], d[k][2], d[k][3]);
+                for (int d = 0; d < D; d++) pk[d] = pack4(dg[d][0], dg[d][1], dg[d][2], dg[d][3]);
+                if constexpr (WIDE) {
+#pragma unroll
+                    for (int d = 0; d < D; d++) qd[d][k][i] = pk[d];
+                } else if constexpr (D == 2) {
+                    qd[0][k][i] = g & 1 ? pk[1] : pk[0];
+                } else {
+                    qd[0][k][i] = (g & 3) == 0 ? pk[0] : (g & 3) == 1 ? pk[1] : (g & 3) == 2 ? pk[D - 1] : 0u;
+                }
             }
-        float r = bad ? __int_as_float(0x7FC00000) : top / DG::kQ * a.scale;
-        rs[0] = __shfl_sync(0xffffffffu, r, 8 * t);        // rows 2 t, 2 t + 1
-        rs[1] = __shfl_sync(0xffffffffu, r, 8 * t + 4);
-        lim[0] = __shfl_sync(0xffffffffu, row.lim, 8 * t);
-        lim[1] = __shfl_sync(0xffffffffu, row.lim, 8 * t + 4);
-    };
-    auto sum_l = [&]() {   // the lanes of a row have summed their own positions
+        const float r = bad ? __int_as_float(0x7FC00000) : top / kQ * a.scale;
 #pragma unroll
-        for (int e = 0; e < 2; e++) {
+        for (int e = 0; e < RL; e++) {
+            const int from = 4 * (WIDE ? 2 * t + e : D == 2 ? 2 * t : 4 * (t >> 1));   // a lane of that row
+            rs[e] = __shfl_sync(0xffffffffu, r, from);
+            lim[e] = __shfl_sync(0xffffffffu, row.lim, from);
+            m[e] = -INFINITY;
+            l[e] = 0.0f;
+        }
+    };
+    // The digits' dots of an accumulator, joined: values e < NV.
+    auto join = [&](const int (&acc)[ND][4], float (&v)[NV]) {
+        if constexpr (WIDE) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                if constexpr (D == 3) v[e] = fmaf((float)acc[0][e], 65536.0f, fmaf((float)acc[1][e], 256.0f, (float)acc[ND - 1][e]));
+                else v[e] = fmaf((float)acc[0][e], 256.0f, (float)acc[ND - 1][e]);
+            }
+        } else if constexpr (D == 2) {
+            v[0] = fmaf((float)acc[0][0], 256.0f, (float)acc[0][1]);
+            v[NV - 1] = fmaf((float)acc[0][2], 256.0f, (float)acc[0][3]);
+        } else {   // even lanes have digits 0 and 1, odd ones digit 2; even ones keep the first 8 of 16, odd ones the others
+            const bool odd = t & 1;
+            const float lo = odd ? (float)acc[0][0] : fmaf((float)acc[0][0], 65536.0f, (float)acc[0][1] * 256.0f);
+            const float hi = odd ? (float)acc[0][2] : fmaf((float)acc[0][2], 65536.0f, (float)acc[0][3] * 256.0f);
+            v[0] = (odd ? hi : lo) + __shfl_xor_sync(0xffffffffu, odd ? lo : hi, 1);
+        }
+    };
+    auto sub = [&](int e) { return g + 8 * (WIDE ? e >> 1 : D == 2 ? e : t & 1); };   // of 16 positions, or dimensions
+    constexpr int kLow = !WIDE && D == 3 ? 1 : 4;   // lanes that share a row differ in these bits: 4, 8, 16 and, here, 1
+    // What the warp has of a unit that ends, or goes on elsewhere, with group `at` (from the block's first on).
+    auto end_unit = [&](const Item& it, bool whole_unit, float* piece, int which, int at) {
+#pragma unroll
+        for (int e = 0; e < RL; e++) {
+            if (kLow == 1) l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
             l[e] += __shfl_xor_sync(0xffffffffu, l[e], 4);
             l[e] += __shfl_xor_sync(0xffffffffu, l[e], 8);
             l[e] += __shfl_xor_sync(0xffffffffu, l[e], 16);
         }
-    };
-    // The unit's sums so far into a piece; `at`: the group in use, from the block's first on.
-    auto put_piece = [&](float* p, int which, int at) {
-        sum_l();
+        const KvSeq q = kv_seq(a, it.s);
+        if (whole_unit) {
 #pragma unroll
-        for (int e = 0; e < 2; e++) {
-            float* row = p + (2 * t + e) * HDP;
+            for (int e = 0; e < RL; e++) {
+                const KvRow row = kv_row(a, q, it.h, it.rg, my_row(e));
+                if (row.out < 0) continue;
+                const float inv = l[e] == 0.0f ? 0.0f : 1.0f / l[e];
+                T* to = (T*)a.out + row.out;
 #pragma unroll
-            for (int w = 0; w < NW; w++)
-                *reinterpret_cast<float4*>(row + 32 * w + 4 * g) =
-                    make_float4(o[w][0][e], o[w][0][2 + e], o[w][1][e], o[w][1][2 + e]);
+                for (int i = 0; i < MT; i++)
+                    if (16 * i < c.hd)
+#pragma unroll
+                        for (int k = e; k < NV; k += RL) to[16 * i + sub(k)] = from_f32<T>(o[i][k] * inv);
+            }
+            return;
+        }
+#pragma unroll
+        for (int e = 0; e < RL; e++) {
+            float* row = piece + my_row(e) * HDP;
+#pragma unroll
+            for (int i = 0; i < MT; i++)
+#pragma unroll
+                for (int k = e; k < NV; k += RL) row[16 * i + sub(k)] = o[i][k];
             if (g == 0) {
-                p[kKvaRows * HDP + 2 * t + e] = m[e];
-                p[kKvaRows * HDP + kKvaRows + 2 * t + e] = l[e];
+                piece[SH::kUnit * HDP + my_row(e)] = m[e];
+                piece[SH::kUnit * HDP + SH::kUnit + my_row(e)] = l[e];
             }
         }
-        if (lane == 0) info[2 * warp + which] = {at - cur.g, at - cur.g + cur.q.ng, cur.s, cur.h, cur.rg, 1};
-    };
-    auto put_rows = [&]() {
-        sum_l();
-#pragma unroll
-        for (int e = 0; e < 2; e++) {
-            const KvRow row = kv_row(a, cur.q, cur.h, cur.rg, 2 * t + e);
-            if (row.out < 0) continue;
-            const float inv = l[e] == 0.0f ? 0.0f : 1.0f / l[e];
-#pragma unroll
-            for (int w = 0; w < NW; w++)
-                if (32 * w + 4 * g < c.hd)
-                    store4((T*)a.out + row.out + 32 * w + 4 * g, a.vec_out,
-                           make_float4(o[w][0][e] * inv, o[w][0][2 + e] * inv, o[w][1][e] * inv, o[w][1][2 + e] * inv));
-        }
+        const int gg = it.g & 0x7FFFFFFF;
+        if (lane == 0) info[2 * warp + which] = {at - gg, at - gg + q.ng, it.s, it.h, it.rg, 1};
     };
 
+    // ---- the stretch.  Turn i uses group i; it also fetches V of i + 1, K of i + 2 and the pages of i + 3, and the
+    // turns before 0 do only that.
     if (n > 0) {
-        Item i1, i2, i3;      // one, two, three groups ahead of the one in use
-        float sc0, sc1, sc2;  // scales of the group in use and the two behind it
-        Item i0 = look(ahead);
-        vet(i0);
-        i1 = i2 = i3 = i0;
-        i1.page = i2.page = i3.page = -1;
-        if (n > 1) {
-            ahead.next(a);
-            i1 = look(ahead);
-            vet(i1);
-        }
-        copy(i0, kp, kdst, 0);
-        cp_async_commit();
-        copy(i0, vp, vdst, 1);
-        cp_async_commit();
-        copy(i1, kp, kdst, 2);
-        cp_async_commit();
-        sc0 = scale_of(i0);
-        sc1 = scale_of(i1);
-        sc2 = 0.0f;
-        if (n > 2) {
-            ahead.next(a);
-            i2 = look(ahead);   // vetted when it is used: the load is on its way
-        }
-        fresh = cur.g == 0;
-        begin_unit();
-        int slot = 0;   // of the next K or V rows to be used
-        for (int i = 0; i < n; i++) {
-            if (i > 0) {
-                const bool last = cur.g + 1 == cur.q.ng;
-                if (last) {   // the unit ended with the group before
-                    if (fresh) put_rows();
-                    else put_piece(piece0, 0, (int)(w0 - b0) + i - 1);
+        Item i0, i1, i2, i3;
+        i0 = i1 = i2 = i3 = Item{0, 0, 0, 0};
+        bool begins = true, fresh = false;
+        int kslot = 0;   // of K of group i (2 i mod 3); V of i lies in the next one
+#pragma unroll 1
+        for (int i = -3; i < n; i++) {
+            const int vslot = kslot == 2 ? 0 : kslot + 1;
+            float alpha[RL], wt[RL];
+            uint32_t pd[ND][4];   // weights as B fragments: 16 h + 4 t..+3 for h = 0..3
+            if (i >= 0) {
+                if (begins) {
+                    begin_unit(i0);
+                    fresh = (i0.g & 0x7FFFFFFF) == 0;
+                    begins = false;
                 }
-                cur.next(a);
-                if (last) {
-                    fresh = true;
-                    begin_unit();
-                }
-            }
-            // ---- scores
-            cp_async_wait<2>();
-            __syncwarp();
-            unsigned char* ks = ring + slot * SM::kSlot;
-            const float vs[4] = {__shfl_sync(0xffffffffu, sc0, 4), __shfl_sync(0xffffffffu, sc0, 5),
-                                 __shfl_sync(0xffffffffu, sc0, 6), __shfl_sync(0xffffffffu, sc0, 7)};
-            const unsigned live = __ballot_sync(0xffffffffu, i0.page >= 0);
-            float p[4][4], mg[2] = {-INFINITY, -INFINITY};   // p[tile][e]: positions g, g + 8 (e >> 1), rows 2 t + (e & 1)
+                // ---- scores
+                cp_async_wait<2>();
+                __syncwarp();
+                const int key0 = (i0.g & 0x7FFFFFFF) * kKvaT;
+                const float4 kscale = *reinterpret_cast<const float4*>(q_scale + 8 * (i & 3));
+                const float4 vscale = *reinterpret_cast<const float4*>(q_scale + 8 * (i & 3) + 4);
+                const float ksc[4] = {kscale.x, kscale.y, kscale.z, kscale.w}, vs[4] = {vscale.x, vscale.y, vscale.z, vscale.w};
+                const uint32_t ks = smem_addr(ring + kslot * SH::kSlot);
+                float p[4][NV], mg[RL];
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                int acc[D][4];
+                for (int e = 0; e < RL; e++) mg[e] = -INFINITY;
 #pragma unroll
-                for (int d = 0; d < D; d++) acc[d][0] = acc[d][1] = acc[d][2] = acc[d][3] = 0;
+                for (int j = 0; j < 4; j++) {
+                    int acc[ND][4];
 #pragma unroll
-                for (int pp = 0; pp < NP; pp++) {
-                    const int r0 = 16 * j + g;
-                    const int at = HDP == 128 ? r0 * 128 + ((4 * pp + t) ^ (4 * (g & 1))) * 16 : r0 * 64 + t * 16;
-                    const uint4 lo = *reinterpret_cast<const uint4*>(ks + at);
-                    const uint4 hi = *reinterpret_cast<const uint4*>(ks + at + 8 * HDP);
-                    const uint32_t f0[4] = {lo.x, hi.x, lo.y, hi.y}, f1[4] = {lo.z, hi.z, lo.w, hi.w};
+                    for (int d = 0; d < ND; d++) acc[d][0] = acc[d][1] = acc[d][2] = acc[d][3] = 0;
 #pragma unroll
-                    for (int d = 0; d < D; d++) {
-                        mma_ss(acc[d], f0, qd[d][pp][0], qd[d][pp][1]);
-                        mma_ss(acc[d], f1, qd[d][pp][2], qd[d][pp][3]);
+                    for (int k = 0; k < KS; k++) {
+                        if (32 * k >= c.hd) break;
+                        uint32_t f[4];
+                        ldsm_rows(f, ks + 16 * j * HDP + place(lane & 15, 2 * k + (lane >> 4)));
+#pragma unroll
+                        for (int d = 0; d < ND; d++) mma_ss(acc[d], f, qd[d][k][0], qd[d][k][1]);
+                    }
+                    join(acc, p[j]);
+#pragma unroll
+                    for (int e = 0; e < NV; e++) {
+                        const int pos = ksc[j] == -1.0f ? 0x7FFFFFFF : key0 + 16 * j + sub(e);   // -1: no page
+                        p[j][e] = pos <= lim[e % RL] ? p[j][e] * (rs[e % RL] * ksc[j]) : -INFINITY;
+                        mg[e % RL] = fmaxf(mg[e % RL], p[j][e]);
                     }
                 }
-                const float kscale = __shfl_sync(0xffffffffu, sc0, j);
+                // ---- weights relative to the group's largest
+                const float vmax = fmaxf(0.0f, fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3])));   // without a NaN or a missing page
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const int pos = cur.g * kKvaT + 16 * j + g + 8 * (e >> 1);
-                    const bool see = pos <= lim[e & 1] && ((live >> j) & 1);
-                    p[j][e] = see ? DG::join(acc, e) * (rs[e & 1] * kscale) : -INFINITY;
-                    mg[e & 1] = fmaxf(mg[e & 1], p[j][e]);
+                for (int e = 0; e < RL; e++) {
+                    if (kLow == 1) mg[e] = fmaxf(mg[e], __shfl_xor_sync(0xffffffffu, mg[e], 1));
+                    mg[e] = fmaxf(mg[e], __shfl_xor_sync(0xffffffffu, mg[e], 4));
+                    mg[e] = fmaxf(mg[e], __shfl_xor_sync(0xffffffffu, mg[e], 8));
+                    mg[e] = fmaxf(mg[e], __shfl_xor_sync(0xffffffffu, mg[e], 16));
+                    const float mn = fmaxf(m[e], mg[e]);
+                    alpha[e] = m[e] == -INFINITY ? 0.0f : kv_exp2(m[e] - mn);
+                    wt[e] = mg[e] == -INFINITY ? 0.0f : kv_exp2(mg[e] - mn);
+                    m[e] = mn;
+                    if (mg[e] == -INFINITY) mg[e] = 0.0f;   // nothing seen: weights of 2^-inf
                 }
-            }
-            // ---- weights relative to the group's largest
-            float alpha[2], wt[2], vmax = 0.0f;
+                uint32_t* fx = reinterpret_cast<uint32_t*>(ring + kslot * SH::kSlot);   // K is read: [row][kWords]
+                __syncwarp();
+                float sum[RL] = {};
 #pragma unroll
-            for (int j = 0; j < 4; j++)
-                if ((live >> j) & 1) vmax = fmaxf(vmax, vs[j]);   // without a NaN
+                for (int j = 0; j < 4; j++) {
+                    const float ratio = kP * (c.page >= kKvaT ? 1.0f : vmax > 0.0f ? vs[j] / vmax : 0.0f);
 #pragma unroll
-            for (int e = 0; e < 2; e++) {
-                mg[e] = fmaxf(mg[e], __shfl_xor_sync(0xffffffffu, mg[e], 4));
-                mg[e] = fmaxf(mg[e], __shfl_xor_sync(0xffffffffu, mg[e], 8));
-                mg[e] = fmaxf(mg[e], __shfl_xor_sync(0xffffffffu, mg[e], 16));
-                const float mn = fmaxf(m[e], mg[e]);
-                alpha[e] = m[e] == -INFINITY ? 0.0f : kv_exp2(m[e] - mn);
-                wt[e] = mg[e] == -INFINITY ? 0.0f : kv_exp2(mg[e] - mn);
-                m[e] = mn;
-            }
-            uint32_t* fx = reinterpret_cast<uint32_t*>(ks);   // [row][68]: the K slot is read
-            __syncwarp();
-            float sum[2] = {0.0f, 0.0f};
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const float ratio = DG::kP * (c.page >= kKvaT ? 1.0f : vmax > 0.0f ? vs[j] / vmax : 0.0f);
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const bool none = p[j][e] == -INFINITY;
-                    const float w = none ? 0.0f : kv_exp2(p[j][e] - mg[e & 1]);
-                    sum[e & 1] += !none && vs[j] != vs[j] ? vs[j] : w;   // a NaN scale reaches the rows that see it
-                    fx[(2 * t + (e & 1)) * 68 + 16 * j + g + 8 * (e >> 1)] = __float2uint_rn(w * ratio);
+                    for (int e = 0; e < NV; e++) {
+                        const float w = kv_exp2(p[j][e] - mg[e % RL]);
+                        sum[e % RL] += w;
+                        if (vs[j] != vs[j] && p[j][e] != -INFINITY) sum[e % RL] = vs[j];   // a NaN scale reaches the rows that see it
+                        const uint32_t z = __float2uint_rn(w * ratio);
+                        const int at = 16 * j + sub(e);
+                        if constexpr (D == 2 && !WIDE) reinterpret_cast<uint16_t*>(fx + my_row(0) * SH::kWords)[at] = (uint16_t)z;
+                        else fx[my_row(e % RL) * SH::kWords + at] = z;
+                    }
                 }
-            }
 #pragma unroll
-            for (int e = 0; e < 2; e++) {
-                l[e] = l[e] * alpha[e] + wt[e] * sum[e];
-                wt[e] *= vmax * (1.0f / DG::kP);
-            }
-            __syncwarp();
-            uint32_t pd[D][4];   // row g, tokens 16 h + 4 t..+3 for h = 0..3
-#pragma unroll
-            for (int h = 0; h < 4; h++) {
-                const uint4 f = *reinterpret_cast<const uint4*>(fx + g * 68 + 16 * h + 4 * t);
-#pragma unroll
-                for (int d = 0; d < D; d++) {
-                    const int b = D - 1 - d, sel = b | (b + 4) << 4;
-                    pd[d][h] = __byte_perm(__byte_perm(f.x, f.y, sel), __byte_perm(f.z, f.w, sel), 0x5410);
+                for (int e = 0; e < RL; e++) {
+                    l[e] = l[e] * alpha[e] + wt[e] * sum[e];
+                    wt[e] *= vmax * (1.0f / kP);
                 }
-            }
-            __syncwarp();
-            if (i + 1 < n) copy(i1, vp, vdst, slot);   // the next group's V into the slot of this group's K
-            cp_async_commit();
-            slot = slot == 2 ? 0 : slot + 1;
-            // ---- out += V^T w
-            cp_async_wait<2>();
-            __syncwarp();
-            const unsigned char* v8 = ring + slot * SM::kSlot;
-#pragma unroll
-            for (int w = 0; w < NW; w++) {
-                const int seg = HDP == 128 ? (w ^ t) * 32 : (w ^ (t & 1)) * 32;
-                uint32_t f[4][4];   // [16 tokens][dimension 32 w + 4 g + b]: tokens 16 h + 4 t..+3
+                __syncwarp();
 #pragma unroll
                 for (int h = 0; h < 4; h++) {
-                    const unsigned char* at = v8 + (16 * h + 4 * t) * HDP + seg + 4 * g;
-                    transpose4(*reinterpret_cast<const uint32_t*>(at), *reinterpret_cast<const uint32_t*>(at + HDP),
-                               *reinterpret_cast<const uint32_t*>(at + 2 * HDP),
-                               *reinterpret_cast<const uint32_t*>(at + 3 * HDP), f[h]);
-                }
+                    if constexpr (D == 2 && !WIDE) {   // column g: row g >> 1, digit g & 1
+                        const uint2 f = *reinterpret_cast<const uint2*>(fx + (g >> 1) * SH::kWords + 8 * h + 2 * t);
+                        pd[0][h] = __byte_perm(f.x, f.y, g & 1 ? 0x6420 : 0x7531);
+                    } else {
+                        const uint4 f = *reinterpret_cast<const uint4*>(fx + (WIDE ? g : g >> 2) * SH::kWords + 16 * h + 4 * t);
 #pragma unroll
-                for (int mt = 0; mt < 2; mt++) {
-                    int acc[D][4];
-                    const uint32_t f0[4] = {f[0][2 * mt], f[0][2 * mt + 1], f[1][2 * mt], f[1][2 * mt + 1]};
-                    const uint32_t f1[4] = {f[2][2 * mt], f[2][2 * mt + 1], f[3][2 * mt], f[3][2 * mt + 1]};
-#pragma unroll
-                    for (int d = 0; d < D; d++) {
-                        acc[d][0] = acc[d][1] = acc[d][2] = acc[d][3] = 0;
-                        mma_su(acc[d], f0, pd[d][0], pd[d][1]);
-                        mma_su(acc[d], f1, pd[d][2], pd[d][3]);
+                        for (int d = 0; d < ND; d++) {
+                            const int b = WIDE ? D - 1 - d : 2 - min(g & 3, 2), sel = b | (b + 4) << 4;
+                            pd[d][h] = __byte_perm(__byte_perm(f.x, f.y, sel), __byte_perm(f.z, f.w, sel), 0x5410);
+                        }
+                        if (!WIDE && (g & 3) == 3) pd[0][h] = 0;
                     }
+                }
+                __syncwarp();
+            }
+            if (i + 3 < n) i3 = take((i + 3) & 3);
+            if (i >= -1 && i + 1 < n) copy(i1, (i + 1) & 3, vp, kslot, false);   // over K of group i
+            cp_async_commit();
+            if (i >= 0) {
+                // ---- out += V^T w
+                cp_async_wait<2>();
+                __syncwarp();
+                const uint32_t v8 = smem_addr(ring + vslot * SH::kSlot);
 #pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        o[w][mt][e] = fmaf(DG::join(acc, e), wt[e & 1], o[w][mt][e] * alpha[e & 1]);
+                for (int mt = 0; mt < MT; mt++) {
+                    if (16 * mt >= c.hd) break;
+                    int acc[ND][4];
+#pragma unroll
+                    for (int d = 0; d < ND; d++) acc[d][0] = acc[d][1] = acc[d][2] = acc[d][3] = 0;
+#pragma unroll
+                    for (int k = 0; k < 2; k++) {
+                        uint32_t f[4];
+                        ldsm_cols(f, v8 + 32 * k * HDP + place(lane, mt));
+#pragma unroll
+                        for (int d = 0; d < ND; d++) mma_su(acc[d], f, pd[d][2 * k], pd[d][2 * k + 1]);
+                    }
+                    float v[NV];
+                    join(acc, v);
+#pragma unroll
+                    for (int e = 0; e < NV; e++) o[mt][e] = fmaf(v[e], wt[e % RL], o[mt][e] * alpha[e % RL]);
+                }
+                __syncwarp();
+                if (i0.g < 0 || i + 1 == n) {   // the unit's last group, or the stretch's
+                    const bool all = i0.g < 0 && fresh;
+                    end_unit(i0, all, fresh ? reinterpret_cast<float*>(ring) : piece0, fresh, (int)(w0 - b0) + i);
+                    begins = true;
                 }
             }
-            __syncwarp();
-            // ---- two groups on: its K into the slot of this group's V; three on: its pages
-            if (i + 2 < n) {
-                vet(i2);
-                copy(i2, kp, kdst, slot);
-                sc2 = scale_of(i2);
+            if (i >= -2 && i + 2 < n) {   // over V of group i; its pages are there, as the last wait says
+                if (i == -2) {   // pages of groups 0 and 1: those of 2 on are there by the waits of the turns
+                    cp_async_wait<0>();
+                    __syncwarp();
+                }
+                copy(i2, (i + 2) & 3, kp, vslot, true);
             }
             cp_async_commit();
-            slot = slot == 2 ? 0 : slot + 1;
-            if (i + 3 < n) {
-                ahead.next(a);
-                i3 = look(ahead);
-            }
+            kslot = vslot == 2 ? 0 : vslot + 1;
             i0 = i1;
             i1 = i2;
             i2 = i3;
-            sc0 = sc1;
-            sc1 = sc2;
         }
-        cp_async_wait<0>();
-        // what the warp holds of its last unit
-        if (fresh && cur.g + 1 == cur.q.ng) put_rows();
-        else put_piece(fresh ? reinterpret_cast<float*>(ring) : piece0, fresh, (int)(w1 - 1 - b0));
     }
 
     // ---- units that warps share, and what is left of them for other blocks
@@ -630,8 +660,9 @@ __global__ void __launch_bounds__(kKvaThreads, HDP == 64 ? 2 : 1) k_kv_attention
     }
     __syncthreads();
     const int nblk = (int)(b1 - b0);
+#pragma unroll 1
     for (int first = warp; first < 2 * kKvaWarps; first += kKvaWarps) {
-        const typename SM::Info f = info[first];
+        const typename SH::Info f = info[first];
         if (!f.valid) continue;
         int prev = first - 1;
         while (prev >= 0 && !info[prev].valid) prev--;
@@ -648,34 +679,35 @@ __global__ void __launch_bounds__(kKvaThreads, HDP == 64 ? 2 : 1) k_kv_attention
         }
         const KvSeq q = kv_seq(a, f.s);
         auto piece = [&](int i) {
-            return reinterpret_cast<const float*>(
-                i & 1 ? smem + (i >> 1) * SM::kRing : smem + kKvaWarps * SM::kRing + (i >> 1) * SM::kPiece);
+            return reinterpret_cast<const float*>(i & 1 ? smem + (i >> 1) * SH::kRing : smem + SH::kPieces + (i >> 1) * SH::kPiece);
         };
-        for (int r = 0; r < kKvaRows; r++) {
+#pragma unroll 1
+        for (int r = 0; r < SH::kUnit; r++) {
             const KvRow row = kv_row(a, q, f.h, f.rg, r);
             if (row.out < 0) break;
             float mx = -INFINITY, ls = 0.0f, os[HDP / 32];
+#pragma unroll 1
             for (int i = first; i < 2 * kKvaWarps; i++)
-                if (info[i].valid && info[i].begin == f.begin) mx = fmaxf(mx, piece(i)[kKvaRows * HDP + r]);
+                if (info[i].valid && info[i].begin == f.begin) mx = fmaxf(mx, piece(i)[SH::kUnit * HDP + r]);
 #pragma unroll
             for (int e = 0; e < HDP / 32; e++) os[e] = 0.0f;
+#pragma unroll 1
             for (int i = first; i < 2 * kKvaWarps; i++) {
                 if (!info[i].valid || info[i].begin != f.begin) continue;
                 const float* p = piece(i);
-                const float pm = p[kKvaRows * HDP + r], wgt = pm == -INFINITY ? 0.0f : kv_exp2(pm - mx);
-                ls += wgt * p[kKvaRows * HDP + kKvaRows + r];
+                const float pm = p[SH::kUnit * HDP + r], wgt = pm == -INFINITY ? 0.0f : kv_exp2(pm - mx);
+                ls += wgt * p[SH::kUnit * HDP + SH::kUnit + r];
 #pragma unroll
-                for (int e = 0; e < HDP / 32; e++) os[e] += wgt * p[r * HDP + (HDP / 32) * lane + e];
+                for (int e = 0; e < HDP / 32; e++) os[e] += wgt * p[r * HDP + lane + 32 * e];
             }
-            const int d0 = (HDP / 32) * lane;
             if (all) {
                 const float inv = ls == 0.0f ? 0.0f : 1.0f / ls;
 #pragma unroll
                 for (int e = 0; e < HDP / 32; e++)
-                    if (d0 + e < c.hd) ((T*)a.out)[row.out + d0 + e] = from_f32<T>(os[e] * inv);
+                    if (lane + 32 * e < c.hd) ((T*)a.out)[row.out + lane + 32 * e] = from_f32<T>(os[e] * inv);
             } else {
 #pragma unroll
-                for (int e = 0; e < HDP / 32; e++) part->o[r][d0 + e] = os[e];
+                for (int e = 0; e < HDP / 32; e++) part->o[r][lane + 32 * e] = os[e];
                 if (lane == 0) {
                     part->m[r] = mx;
                     part->l[r] = ls;
@@ -686,27 +718,37 @@ __global__ void __launch_bounds__(kKvaThreads, HDP == 64 ? 2 : 1) k_kv_attention
 }
 
 // Units that blocks share.  Block b - 1 takes the border before block b: the
-// unit that lies across it, if this is the first border inside the unit.
+// unit that lies across it, if this is the first border inside the unit.  The
+// records of the blocks from b - 1 on are read at once, lane i that of b - 1 + i.
 constexpr int kKvJoinThreads = 128;
 template <typename T>
 __global__ void __launch_bounds__(kKvJoinThreads) k_kv_attention_join(const KvAttnArgs a, int blocks) {
     pdl_wait();
     const int b = blockIdx.x + 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const KvPart* lead = a.parts + 2 * (size_t)b;
-    if (!lead->valid || lead->begin >= lead->at) return;
-    const long long begin = lead->begin, before = a.parts[2 * (size_t)(b - 1)].at;
-    if (begin < before) return;
-    const KvPart* head = a.parts + 2 * (size_t)(b - 1) + (begin == before ? 0 : 1);
-    int end = b + 1;
-    while (end < blocks && a.parts[2 * (size_t)end].valid && a.parts[2 * (size_t)end].begin == begin) end++;
-    const KvSeq q = kv_seq(a, lead->s);
-    for (int r = warp; r < kKvaRows; r += kKvJoinThreads / 32) {
-        const KvRow row = kv_row(a, q, lead->h, lead->rg, r);
+    const KvPart* p0 = a.parts + 2 * (size_t)(b - 1);
+    const KvPart* mine = p0 + 2 * (size_t)lane;
+    const bool there = b - 1 + lane < blocks;
+    const long long begin = there && mine->valid ? mine->begin : -1, at = there ? mine->at : -1;
+    const KvPart* lead = p0 + 2;
+    const int s = lead->s, h = lead->h, rg = lead->rg;
+    const long long ubegin = __shfl_sync(0xffffffffu, begin, 1), uat = __shfl_sync(0xffffffffu, at, 1);
+    const long long before = __shfl_sync(0xffffffffu, at, 0);
+    if (ubegin < 0 || ubegin >= uat || ubegin < before) return;
+    const KvPart* head = p0 + (ubegin == before ? 0 : 1);
+    // blocks b..end-1 hold a part in their first record; a unit over more than 31 blocks is followed one by one
+    const unsigned other = ~__ballot_sync(0xffffffffu, lane == 0 || begin == ubegin);
+    int end = b - 1 + (other ? __ffs(other) - 1 : 32);
+    if (!other)
+        while (end < blocks && a.parts[2 * (size_t)end].valid && a.parts[2 * (size_t)end].begin == ubegin) end++;
+    const KvSeq q = kv_seq(a, s);
+    for (int r = warp; r < 1 << a.unit_log; r += kKvJoinThreads / 32) {
+        const KvRow row = kv_row(a, q, h, rg, r);
         if (row.out < 0) break;
         float mx = head->m[r];
         for (int i = b; i < end; i++) mx = fmaxf(mx, a.parts[2 * (size_t)i].m[r]);
         float ls = 0.0f;
         float4 os = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
         for (int i = b - 1; i < end; i++) {
             const KvPart* p = i < b ? head : a.parts + 2 * (size_t)i;
             const float pm = p->m[r], wgt = pm == -INFINITY ? 0.0f : kv_exp2(pm - mx);
