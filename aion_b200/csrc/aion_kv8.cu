@@ -268,6 +268,8 @@ static aion_status check_rows(const aion_kv8* kv, int layer, int type, const int
     KV_ARG(type == AION_F32 || type == AION_F16 || type == AION_BF16, "%s: unknown element type %d", what, type);
     KV_ARG(n_seq >= 0 && n_seq <= kKvMaxSeqs && n_tok >= 0 && n_tok <= (1 << 24),
            "%s: %d sequences (at most %d), %d rows (at most %d)", what, n_seq, kKvMaxSeqs, n_tok, 1 << 24);
+    KV_ARG(((int64_t)(n_tok >> 4) + 2 * n_seq) * kv->n_kv_heads * 2 < ((int64_t)1 << 31), "%s: %d rows of %d heads are too many",
+           what, n_tok, kv->n_kv_heads);
     KV_ARG(cu || n_seq == n_tok, "%s: without cu every sequence has one row (%d sequences, %d rows)", what, n_seq, n_tok);
     KV_ARG(n_seq == 0 || (seqs && pos0), "%s: null seqs or pos0", what);
     return AION_OK;
@@ -285,6 +287,33 @@ static aion_status check_matrix(const void* p, int64_t stride, int64_t width, in
 }
 static bool vectors(const void* p, int64_t stride, int type) {
     return ((uintptr_t)p & 15) == 0 && (stride * type_bytes(type)) % 16 == 0;
+}
+
+template <typename T>
+static cudaError_t launch_append(const KvAppendArgs& a, cudaStream_t st) {
+    if (!a.r.cu) {
+        const int64_t warps = (int64_t)a.r.n_seq * a.c.nkv * 2;
+        k_kv_append_one<T><<<(unsigned)((warps + kKvAppendThreads / 32 - 1) / (kKvAppendThreads / 32)), kKvAppendThreads, 0, st>>>(a);
+        return cudaGetLastError();
+    }
+    const unsigned grid = (unsigned)((int64_t)kv_places(true, a.r.n_seq, a.r.n_tok, a.c.page_log, 2) * a.c.nkv * 2);
+    if (a.c.page == 16) k_kv_append<T, 2><<<grid, kKvAppendThreads, 0, st>>>(a);
+    else if (a.c.page == 32) k_kv_append<T, 4><<<grid, kKvAppendThreads, 0, st>>>(a);
+    else if (a.c.page == 64) k_kv_append<T, 8><<<grid, kKvAppendThreads, 0, st>>>(a);
+    else k_kv_append<T, 16><<<grid, kKvAppendThreads, 0, st>>>(a);
+    return cudaGetLastError();
+}
+
+template <typename T>
+static cudaError_t launch_read(const KvReadArgs& a, cudaStream_t st) {
+    if (!a.r.cu) {
+        const int64_t warps = (int64_t)a.r.n_seq * a.c.nkv * 2;
+        k_kv_read_one<T><<<(unsigned)((warps + kKvAppendThreads / 32 - 1) / (kKvAppendThreads / 32)), kKvAppendThreads, 0, st>>>(a);
+    } else {
+        const int64_t grid = (int64_t)kv_places(true, a.r.n_seq, a.r.n_tok, kKvReadLog, 1) * a.c.nkv * 2;
+        k_kv_read<T><<<(unsigned)grid, kKvReadThreads, 0, st>>>(a);
+    }
+    return cudaGetLastError();
 }
 
 extern "C" AION_API aion_status aion_kv8_append(const aion_kv8* kv, int32_t layer, const void* k, const void* v,
@@ -308,12 +337,9 @@ extern "C" AION_API aion_status aion_kv8_append(const aion_kv8* kv, int32_t laye
     a.k_stride = k_stride;
     a.v_stride = v_stride;
     a.vec = vectors(k, k_stride, type) && vectors(v, v_stride, type);
-    const dim3 grid(kv_places(cu != nullptr, n_seq, n_tok, a.c.page_log, 2), kv->n_kv_heads, 2);
-    const cudaStream_t st = (cudaStream_t)stream;
-    if (type == AION_F32) k_kv_append<float><<<grid, kKvAppendThreads, 0, st>>>(a);
-    else if (type == AION_F16) k_kv_append<__half><<<grid, kKvAppendThreads, 0, st>>>(a);
-    else k_kv_append<__nv_bfloat16><<<grid, kKvAppendThreads, 0, st>>>(a);
-    KV_CUDA(cudaGetLastError());
+    KV_CUDA(type == AION_F32 ? launch_append<float>(a, (cudaStream_t)stream)
+            : type == AION_F16 ? launch_append<__half>(a, (cudaStream_t)stream)
+                               : launch_append<__nv_bfloat16>(a, (cudaStream_t)stream));
     return AION_OK;
 }
 
@@ -338,12 +364,9 @@ extern "C" AION_API aion_status aion_kv8_read(const aion_kv8* kv, int32_t layer,
     a.k_stride = k_stride;
     a.v_stride = v_stride;
     a.vec = (!k || vectors(k, k_stride, type)) && (!v || vectors(v, v_stride, type));
-    const dim3 grid(kv_places(cu != nullptr, n_seq, n_tok, kKvReadLog, 1), kv->n_kv_heads);
-    const cudaStream_t st = (cudaStream_t)stream;
-    if (type == AION_F32) k_kv_read<float><<<grid, kKvReadThreads, 0, st>>>(a);
-    else if (type == AION_F16) k_kv_read<__half><<<grid, kKvReadThreads, 0, st>>>(a);
-    else k_kv_read<__nv_bfloat16><<<grid, kKvReadThreads, 0, st>>>(a);
-    KV_CUDA(cudaGetLastError());
+    KV_CUDA(type == AION_F32 ? launch_read<float>(a, (cudaStream_t)stream)
+            : type == AION_F16 ? launch_read<__half>(a, (cudaStream_t)stream)
+                               : launch_read<__nv_bfloat16>(a, (cudaStream_t)stream));
     return AION_OK;
 }
 

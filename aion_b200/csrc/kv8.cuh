@@ -318,6 +318,21 @@ struct KvRows {
     __device__ __forceinline__ int end(int i) const { return cu ? cu[i + 1] : i + 1; }
 };
 
+// The last i < n with first(i) <= u, where first does not fall and first(0) <=
+// u: by a converged warp, 32 places at a time, since one after the other each
+// would be a trip to memory.
+template <typename First>
+__device__ __forceinline__ int kv_warp_find(int n, long long u, First first) {
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int step = (hi - lo + 31) / 32, i = lo + (threadIdx.x & 31) * step;
+        const unsigned in = __ballot_sync(0xffffffffu, i < hi && first(i) <= u) | 1u;
+        lo += (31 - __clz(in)) * step;
+        hi = min(lo + step, hi);
+    }
+    return lo;
+}
+
 // Blocks of `1 << log` rows or positions are dealt out without a pass over the
 // lengths: sequence i has the virtual places (cu[i] >> log) + extra * i and
 // on, up to the next one's.  Its cnt = cu[i+1] - cu[i] rows need at most
@@ -329,12 +344,7 @@ __device__ __forceinline__ int kv_seq_of(const KvRows& r, int u, int log, int ex
         *index = 0;
         return u;
     }
-    int lo = 0, hi = r.n_seq - 1;   // the last sequence whose first place is <= u
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if ((r.cu[mid] >> log) + extra * mid <= u) lo = mid;
-        else hi = mid - 1;
-    }
+    const int lo = kv_warp_find(r.n_seq, u, [&](int i) { return (r.cu[i] >> log) + extra * i; });
     *index = u - ((r.cu[lo] >> log) + extra * lo);
     return lo;
 }
@@ -380,6 +390,31 @@ __device__ __forceinline__ void store16(T* p, bool vec, const float (&x)[16]) {
     }
 }
 
+// Four consecutive values; `vec`: rows start on 16 bytes.
+template <typename T>
+__device__ __forceinline__ float4 load4(const T* p, bool vec) {
+    T t[4];
+    if (vec) {
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(t) = *reinterpret_cast<const uint4*>(p);
+        else *reinterpret_cast<uint2*>(t) = *reinterpret_cast<const uint2*>(p);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) t[i] = p[i];
+    }
+    return make_float4(to_f32(t[0]), to_f32(t[1]), to_f32(t[2]), to_f32(t[3]));
+}
+template <typename T>
+__device__ __forceinline__ void store4(T* p, bool vec, float4 x) {
+    T t[4] = {from_f32<T>(x.x), from_f32<T>(x.y), from_f32<T>(x.z), from_f32<T>(x.w)};
+    if (vec) {
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(p) = *reinterpret_cast<uint4*>(t);
+        else *reinterpret_cast<uint2*>(p) = *reinterpret_cast<uint2*>(t);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) p[i] = t[i];
+    }
+}
+
 // The integer nearest to the exact x / s (ties to even), within +-127; s > 0.
 // The rounded quotient can only be off next to a border between two integers;
 // x - q s is exact there (a multiple of the smaller ulp, below 2^24 of them),
@@ -397,6 +432,45 @@ __device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d) {
     return (a & 0xFF) | (b & 0xFF) << 8 | (c & 0xFF) << 16 | (uint32_t)d << 24;
 }
 
+// Four values under a page's scale s > 0, packed.  q = rint(x (1 / s)) can only
+// be off where x - q s, which the fma gives exactly, reaches half a scale:
+// those and tiny scales take the exact way.
+__device__ __forceinline__ uint32_t kv_quant4(float4 x, float s, float inv) {
+    constexpr float kMagic = 12582912.0f;   // 1.5 2^23: the sum's low byte is the integer's
+    const float m0 = fmaf(x.x, inv, kMagic), m1 = fmaf(x.y, inv, kMagic), m2 = fmaf(x.z, inv, kMagic),
+                m3 = fmaf(x.w, inv, kMagic);
+    const float h = 0.5f * s;
+    const bool close = fabsf(fmaf(m0 - kMagic, -s, x.x)) >= h || fabsf(fmaf(m1 - kMagic, -s, x.y)) >= h ||
+                       fabsf(fmaf(m2 - kMagic, -s, x.z)) >= h || fabsf(fmaf(m3 - kMagic, -s, x.w)) >= h;
+    if (close || s < 1e-30f) return pack4(kv_quant(x.x, s), kv_quant(x.y, s), kv_quant(x.z, s), kv_quant(x.w, s));
+    return __byte_perm(__byte_perm(__float_as_uint(m0), __float_as_uint(m1), 0x0040),
+                       __byte_perm(__float_as_uint(m2), __float_as_uint(m3), 0x0040), 0x5410);
+}
+// Largest magnitude so far, as bits: a NaN or an infinity stays the largest.
+__device__ __forceinline__ uint32_t kv_top4(uint32_t top, float4 x) {
+    const uint32_t a = max(__float_as_uint(x.x) & 0x7FFFFFFFu, __float_as_uint(x.y) & 0x7FFFFFFFu);
+    const uint32_t b = max(__float_as_uint(x.z) & 0x7FFFFFFFu, __float_as_uint(x.w) & 0x7FFFFFFFu);
+    return max(top, max(a, b));
+}
+// The scale of a page whose new rows reach `top`; `old`: that of its earlier rows, if it has any.
+__device__ __forceinline__ float kv_scale_of(uint32_t top, bool held, float old) {
+    const float nan = __int_as_float(0x7FC00000);
+    const float need = top < 0x7F800000u ? __fdiv_rn(__uint_as_float(top), 127.0f) : nan;
+    if (!held) return need;
+    if (need <= old) return old;
+    return need == need && old == old ? fmaxf(need, 1.25f * old) : nan;
+}
+// Earlier values of a page under its grown scale: words i0, i0 + step, ... of n.
+__device__ __forceinline__ void kv_rescale(int8_t* pool, int n, int i0, int step, float old, float s) {
+    const float ratio = s > 0.0f ? __fdiv_rn(old, s) : 0.0f;   // also a NaN scale: the values become 0
+    for (int i = i0; i < n; i += step) {
+        uint32_t* w = reinterpret_cast<uint32_t*>(pool) + i;
+        const uint32_t u = *w;
+        *w = pack4(kv_requant((int8_t)u, ratio), kv_requant((int8_t)(u >> 8), ratio), kv_requant((int8_t)(u >> 16), ratio),
+                   kv_requant((int8_t)(u >> 24), ratio));
+    }
+}
+
 struct KvAppendArgs {
     KvView c;
     KvRows r;
@@ -405,85 +479,119 @@ struct KvAppendArgs {
     long long k_stride, v_stride;
     int vec;
 };
-// Block (place, head, K or V): the rows of one page and head.
-constexpr int kKvAppendThreads = 128;
-template <typename T>
+// Block (place, K or V, head, heads fastest: neighbours read neighbouring
+// rows): the rows of one page and head, four values a thread and step, all of
+// them loaded before the scale is known and kept in registers (PIECES = page /
+// 8 steps at most).  Bound by memory: a row is read once and leaves as a
+// quarter (or half) of its bytes.
+constexpr int kKvAppendThreads = 256;
+template <typename T, int PIECES>
 __global__ void __launch_bounds__(kKvAppendThreads) k_kv_append(KvAppendArgs a) {
-    __shared__ float red[kKvAppendThreads / 32];
+    __shared__ uint32_t red[kKvAppendThreads / 32];
     const KvView& c = a.c;
+    const int h = blockIdx.x % c.nkv, isv = (blockIdx.x / c.nkv) & 1;
     int idx;
-    const int s = kv_seq_of(a.r, blockIdx.x, c.page_log, 2, &idx), h = blockIdx.y, isv = blockIdx.z;
+    const int s = kv_seq_of(a.r, blockIdx.x / (2 * c.nkv), c.page_log, 2, &idx);
     const int t0 = a.r.begin(s), t1 = min(a.r.end(s), a.r.n_tok), p0 = a.r.pos0[s], slot = a.r.seqs[s];
     if (p0 < 0 || t1 <= t0) return;
     const int pg = (p0 >> c.page_log) + idx;                        // page of the slot
     const long long lo = max((long long)p0, (long long)pg << c.page_log);
     const long long hi = min((long long)p0 + (t1 - t0), (long long)(pg + 1) << c.page_log);
     if (lo >= hi) return;
-    bool bad = t0 < 0 || slot < 0 || slot >= c.max_seqs;
+    if (t0 < 0) {
+        if (threadIdx.x == 0) kv_flag(c, KV_BAD_ARG);
+        return;
+    }
+    // the rows are on their way while the page is looked up and checked
+    const long long stride = isv ? a.v_stride : a.k_stride;
+    const T* x = (isv ? (const T*)a.v : (const T*)a.k) + (t0 + (lo - p0)) * stride + (long long)h * c.hd;
+    const int rows = (int)(hi - lo), row0 = (int)(lo & (c.page - 1)), ppr = c.hd / 4, n = rows * ppr;   // pieces of a row
+    float4 v[PIECES];
+    uint32_t top = 0;
+    const int dr = kKvAppendThreads / ppr, dc = kKvAppendThreads - dr * ppr;
+    int row = threadIdx.x / ppr, col = threadIdx.x - row * ppr;
+#pragma unroll
+    for (int e = 0; e < PIECES; e++) {
+        v[e] = (int)threadIdx.x + e * kKvAppendThreads < n ? load4(x + row * stride + 4 * col, a.vec) : make_float4(0, 0, 0, 0);
+        row += dr;
+        col += dc;
+        if (col >= ppr) {
+            col -= ppr;
+            row++;
+        }
+    }
+    bool bad = slot < 0 || slot >= c.max_seqs;
     for (int j = threadIdx.x; j < s; j += kKvAppendThreads) bad = bad || a.r.seqs[j] == slot;
+    const int page = slot >= 0 && slot < c.max_seqs && pg < c.max_pages ? c.tables[(size_t)slot * c.max_pages + pg] : -1;
     if (__syncthreads_or(bad)) {
         if (threadIdx.x == 0) kv_flag(c, KV_BAD_ARG);
         return;
     }
-    const int page = pg < c.max_pages ? c.tables[(size_t)slot * c.max_pages + pg] : -1;
     if (page < 0 || page >= c.n_pages || c.refs[page] != 1) {
         if (threadIdx.x == 0) kv_flag(c, KV_BAD_PAGE);
         return;
     }
-    const T* x = (isv ? (const T*)a.v + (t0 + (lo - p0)) * a.v_stride : (const T*)a.k + (t0 + (lo - p0)) * a.k_stride) +
-                 (long long)h * c.hd;
-    const long long stride = isv ? a.v_stride : a.k_stride;
-    const int rows = (int)(hi - lo), row0 = (int)(lo & (c.page - 1)), cpr = c.hd / 16;   // 16-value chunks a row
     int8_t* pool = (isv ? c.v : c.k) + a.layer * c.plane() + ((long long)page * c.nkv + h) * c.page * c.hd;
     float* scale = (isv ? c.v_scale : c.k_scale) + ((long long)a.layer * c.n_pages + page) * c.nkv + h;
-    float m = 0.0f;   // NaN once a value is not finite: max() below keeps it
-    for (int i = threadIdx.x; i < rows * cpr; i += kKvAppendThreads) {
-        float v[16];
-        load16(x + (i / cpr) * stride + (i % cpr) * 16, a.vec, v);
+    const float old = row0 ? *scale : 0.0f;
 #pragma unroll
-        for (int e = 0; e < 16; e++) {
-            const float b = fabsf(v[e]);
-            m = b <= 3.402823466e38f ? fmaxf(m, b) : INFINITY;
-        }
-    }
-    m = warp_max(m);
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
-    __syncthreads();
-    m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    const float need = m <= 3.402823466e38f ? __fdiv_rn(m, 127.0f) : __int_as_float(0x7FC00000);
-    const float s0 = row0 ? *scale : 0.0f;
-    float sc = need;
-    if (row0 && need <= s0) sc = s0;
-    else if (row0 && need == need && s0 == s0) sc = fmaxf(need, 1.25f * s0);
-    else if (row0) sc = __int_as_float(0x7FC00000);
-    __syncthreads();   // every thread has the old scale
+    for (int e = 0; e < PIECES; e++) top = kv_top4(top, v[e]);
+    top = __reduce_max_sync(0xffffffffu, top);
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = top;
+    __syncthreads();   // every thread has the old scale, too
+#pragma unroll
+    for (int w = 0; w < kKvAppendThreads / 32; w++) top = max(top, red[w]);
+    const float sc = kv_scale_of(top, row0 != 0, old);
     if (threadIdx.x == 0) *scale = sc;
-    if (row0 && sc != s0) {   // also a NaN scale: the earlier values become 0
-        const float ratio = sc > 0.0f ? __fdiv_rn(s0, sc) : 0.0f;
-        for (int i = threadIdx.x; i < row0 * cpr; i += kKvAppendThreads) {
-            uint4* at = reinterpret_cast<uint4*>(pool) + i;
-            uint4 w = *at;
-            uint32_t* u = reinterpret_cast<uint32_t*>(&w);
+    if (row0 && sc != old) kv_rescale(pool, row0 * ppr, threadIdx.x, kKvAppendThreads, old, sc);
+    const float inv = __fdiv_rn(1.0f, sc);
+    uint32_t* to = reinterpret_cast<uint32_t*>(pool) + row0 * ppr;
 #pragma unroll
-            for (int e = 0; e < 4; e++)
-                u[e] = pack4(kv_requant((int8_t)u[e], ratio), kv_requant((int8_t)(u[e] >> 8), ratio),
-                             kv_requant((int8_t)(u[e] >> 16), ratio), kv_requant((int8_t)(u[e] >> 24), ratio));
-            *at = w;
-        }
+    for (int e = 0; e < PIECES; e++) {
+        const int i = threadIdx.x + e * kKvAppendThreads;
+        if (i < n) to[i] = sc > 0.0f ? kv_quant4(v[e], sc, inv) : 0u;
     }
-    for (int i = threadIdx.x; i < rows * cpr; i += kKvAppendThreads) {
-        float v[16];
-        load16(x + (i / cpr) * stride + (i % cpr) * 16, a.vec, v);
-        int q[16];
-#pragma unroll
-        for (int e = 0; e < 16; e++) q[e] = sc > 0.0f ? kv_quant(v[e], sc) : 0;
-        uint4 w;
-        w.x = pack4(q[0], q[1], q[2], q[3]);
-        w.y = pack4(q[4], q[5], q[6], q[7]);
-        w.z = pack4(q[8], q[9], q[10], q[11]);
-        w.w = pack4(q[12], q[13], q[14], q[15]);
-        *(reinterpret_cast<uint4*>(pool) + row0 * cpr + i) = w;
+}
+
+// One row a sequence: a warp takes a sequence, head, and K or V; lane l has
+// dimensions 4 l..+3.  Bound by the trips to memory that depend on one another
+// (slot and position, page, its scale); the row is loaded alongside the first.
+template <typename T>
+__global__ void __launch_bounds__(kKvAppendThreads) k_kv_append_one(KvAppendArgs a) {
+    const KvView& c = a.c;
+    const int lane = threadIdx.x & 31;
+    const long long u = (long long)blockIdx.x * (kKvAppendThreads / 32) + (threadIdx.x >> 5);
+    const int h = (int)(u % c.nkv), isv = (int)(u / c.nkv) & 1, s = (int)(u / (2 * c.nkv));
+    if (s >= a.r.n_seq) return;
+    const int p0 = a.r.pos0[s], slot = a.r.seqs[s];
+    const T* x = isv ? (const T*)a.v + s * a.v_stride : (const T*)a.k + s * a.k_stride;
+    const float4 v = 4 * lane < c.hd ? load4(x + (long long)h * c.hd + 4 * lane, a.vec) : make_float4(0, 0, 0, 0);
+    bool twice = false;
+    for (int j = lane; j < s; j += 32) twice = twice || a.r.seqs[j] == slot;
+    if (p0 < 0) return;
+    if (__any_sync(0xffffffffu, twice) || slot < 0 || slot >= c.max_seqs) {
+        if (lane == 0) kv_flag(c, KV_BAD_ARG);
+        return;
     }
+    const int pg = p0 >> c.page_log, page = pg < c.max_pages ? c.tables[(size_t)slot * c.max_pages + pg] : -1;
+    if (page < 0 || page >= c.n_pages) {
+        if (lane == 0) kv_flag(c, KV_BAD_PAGE);
+        return;
+    }
+    const int row0 = p0 & (c.page - 1), ppr = c.hd / 4;
+    int8_t* pool = (isv ? c.v : c.k) + a.layer * c.plane() + ((long long)page * c.nkv + h) * c.page * c.hd;
+    float* scale = (isv ? c.v_scale : c.k_scale) + ((long long)a.layer * c.n_pages + page) * c.nkv + h;
+    const float old = *scale;
+    if (c.refs[page] != 1) {
+        if (lane == 0) kv_flag(c, KV_BAD_PAGE);
+        return;
+    }
+    const float sc = kv_scale_of(__reduce_max_sync(0xffffffffu, kv_top4(0, v)), row0 != 0, old);
+    __syncwarp();   // every lane has the old scale
+    if (lane == 0) *scale = sc;
+    if (row0 && sc != old) kv_rescale(pool, row0 * ppr, lane, 32, old, sc);
+    if (4 * lane < c.hd)
+        reinterpret_cast<uint32_t*>(pool)[row0 * ppr + lane] = sc > 0.0f ? kv_quant4(v, sc, __fdiv_rn(1.0f, sc)) : 0u;
 }
 
 struct KvReadArgs {
@@ -494,42 +602,99 @@ struct KvReadArgs {
     long long k_stride, v_stride;
     int vec;
 };
-// Block (place of 32 rows, head): 16 values a thread and step, K then V.
-constexpr int kKvReadThreads = 128, kKvReadLog = 5;
+// One row a sequence: a warp takes a sequence, head, and K or V; lane l has
+// dimensions 4 l..+3.
+template <typename T>
+__global__ void __launch_bounds__(kKvAppendThreads) k_kv_read_one(KvReadArgs a) {
+    const KvView& c = a.c;
+    const int lane = threadIdx.x & 31;
+    const long long u = (long long)blockIdx.x * (kKvAppendThreads / 32) + (threadIdx.x >> 5);
+    const int h = (int)(u % c.nkv), isv = (int)(u / c.nkv) & 1, s = (int)(u / (2 * c.nkv));
+    T* out = isv ? (T*)a.v : (T*)a.k;
+    if (s >= a.r.n_seq || !out) return;
+    const int p0 = a.r.pos0[s], slot = a.r.seqs[s];
+    const bool held = slot >= 0 && slot < c.max_seqs;
+    uint32_t w = 0;
+    float sc = 0.0f;
+    if (p0 >= 0 && held) {
+        const int pg = p0 >> c.page_log, page = pg < c.max_pages ? c.tables[(size_t)slot * c.max_pages + pg] : -1;
+        if (page >= 0 && page < c.n_pages) {
+            const long long unit = (long long)page * c.nkv + h;
+            sc = (isv ? c.v_scale : c.k_scale)[(long long)a.layer * c.n_pages * c.nkv + unit];
+            if (4 * lane < c.hd)
+                w = *reinterpret_cast<const uint32_t*>((isv ? c.v : c.k) + a.layer * c.plane() +
+                                                       (unit * c.page + (p0 & (c.page - 1))) * c.hd + 4 * lane);
+        } else if (lane == 0) {
+            kv_flag(c, KV_BAD_PAGE);
+        }
+    } else if (p0 >= 0 && lane == 0) {
+        kv_flag(c, KV_BAD_ARG);
+    }
+    if (4 * lane < c.hd)
+        store4(out + s * (isv ? a.v_stride : a.k_stride) + (long long)h * c.hd + 4 * lane, a.vec,
+               make_float4((float)(int8_t)w * sc, (float)(int8_t)(w >> 8) * sc, (float)(int8_t)(w >> 16) * sc,
+                           (float)(int8_t)(w >> 24) * sc));
+}
+
+// Block (place of 64 rows, K or V, head, heads fastest): four values a thread
+// and step, eight steps in flight.  Bound by memory, the writes above all.
+constexpr int kKvReadThreads = 256, kKvReadLog = 6, kKvReadSteps = 8;
 template <typename T>
 __global__ void __launch_bounds__(kKvReadThreads) k_kv_read(KvReadArgs a) {
+    __shared__ long long s_at[8];
+    __shared__ float s_scale[8];
     const KvView& c = a.c;
+    const int h = blockIdx.x % c.nkv, isv = (blockIdx.x / c.nkv) & 1;
+    T* out = isv ? (T*)a.v : (T*)a.k;
+    if (!out) return;
     int idx;
-    const int s = kv_seq_of(a.r, blockIdx.x, kKvReadLog, 1, &idx), h = blockIdx.y;
+    const int s = kv_seq_of(a.r, blockIdx.x / (2 * c.nkv), kKvReadLog, 1, &idx);
     const int t0 = a.r.begin(s), t1 = min(a.r.end(s), a.r.n_tok), p0 = a.r.pos0[s], slot = a.r.seqs[s];
-    const int i0 = idx << kKvReadLog, rows = min(t1 - t0 - i0, 1 << kKvReadLog), cpr = c.hd / 16;
+    const int i0 = idx << kKvReadLog, rows = min(t1 - t0 - i0, 1 << kKvReadLog), ppr = c.hd / 4, n = rows * ppr;
     if (rows <= 0 || t0 < 0) return;
     const bool held = slot >= 0 && slot < c.max_seqs;
     if (!held && p0 >= 0 && threadIdx.x == 0) kv_flag(c, KV_BAD_ARG);
-    for (int i = threadIdx.x; i < 2 * rows * cpr; i += kKvReadThreads) {
-        const int isv = i >= rows * cpr, j = i - isv * rows * cpr, row = i0 + j / cpr, ch = j % cpr;
-        T* out = isv ? (T*)a.v : (T*)a.k;
-        if (!out) continue;
-        float x[16];
-#pragma unroll
-        for (int e = 0; e < 16; e++) x[e] = 0.0f;
-        if (held && p0 >= 0) {
-            const long long pos = (long long)p0 + row;
-            const long long pg = pos >> c.page_log;
+    // the pages that the rows lie in: five at most
+    const long long first = (long long)p0 + i0, pg0 = first >> c.page_log;
+    if (threadIdx.x < 8) {
+        const long long pg = pg0 + threadIdx.x;
+        long long at = -1;
+        float sc = 0.0f;
+        if (held && p0 >= 0 && pg <= (first + rows - 1) >> c.page_log) {
             const int page = pg < c.max_pages ? c.tables[(size_t)slot * c.max_pages + pg] : -1;
-            if (page >= 0 && page < c.n_pages) {
-                const float sc = (isv ? c.v_scale : c.k_scale)[((long long)a.layer * c.n_pages + page) * c.nkv + h];
-                const int8_t* pool = (isv ? c.v : c.k) + a.layer * c.plane() +
-                                     ((long long)page * c.nkv + h) * c.page * c.hd + (pos & (c.page - 1)) * c.hd + 16 * ch;
-                const uint4 w = *reinterpret_cast<const uint4*>(pool);
-                const int8_t* b = reinterpret_cast<const int8_t*>(&w);
-#pragma unroll
-                for (int e = 0; e < 16; e++) x[e] = (float)b[e] * sc;
-            } else {
+            if (page < 0 || page >= c.n_pages) {
                 kv_flag(c, KV_BAD_PAGE);
+            } else {
+                const long long unit = (long long)page * c.nkv + h;
+                at = a.layer * c.plane() + unit * c.page * c.hd;
+                sc = (isv ? c.v_scale : c.k_scale)[(long long)a.layer * c.n_pages * c.nkv + unit];
             }
         }
-        store16(out + (t0 + row) * (isv ? a.v_stride : a.k_stride) + (long long)h * c.hd + 16 * ch, a.vec, x);
+        s_at[threadIdx.x] = at;
+        s_scale[threadIdx.x] = sc;
+    }
+    __syncthreads();
+    const long long stride = isv ? a.v_stride : a.k_stride;
+    const int8_t* pool = isv ? c.v : c.k;
+    const int in = (int)(first & (c.page - 1));   // the first row's place in its page
+    out += (long long)(t0 + i0) * stride + (long long)h * c.hd;
+    for (int base = 0; base < n; base += kKvReadSteps * kKvReadThreads) {
+        uint32_t w[kKvReadSteps];
+#pragma unroll
+        for (int e = 0; e < kKvReadSteps; e++) {
+            const int i = base + e * kKvReadThreads + threadIdx.x, row = i / ppr, r = in + row;
+            const long long at = i < n ? s_at[r >> c.page_log] : -1;
+            w[e] = at >= 0 ? *reinterpret_cast<const uint32_t*>(pool + at + (r & (c.page - 1)) * c.hd + 4 * (i - row * ppr)) : 0u;
+        }
+#pragma unroll
+        for (int e = 0; e < kKvReadSteps; e++) {
+            const int i = base + e * kKvReadThreads + threadIdx.x, row = i / ppr;
+            if (i >= n) break;
+            const float sc = s_scale[(in + row) >> c.page_log];
+            store4(out + row * stride + 4 * (i - row * ppr), a.vec,
+                   make_float4((float)(int8_t)w[e] * sc, (float)(int8_t)(w[e] >> 8) * sc, (float)(int8_t)(w[e] >> 16) * sc,
+                               (float)(int8_t)(w[e] >> 24) * sc));
+        }
     }
 }
 

@@ -188,31 +188,6 @@ __device__ __forceinline__ KvRow kv_row(const KvAttnArgs& a, const KvSeq& q, int
     return w;
 }
 
-// Four consecutive values; `vec`: rows start on 16 bytes.
-template <typename T>
-__device__ __forceinline__ float4 load4(const T* p, bool vec) {
-    T t[4];
-    if (vec) {
-        if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(t) = *reinterpret_cast<const uint4*>(p);
-        else *reinterpret_cast<uint2*>(t) = *reinterpret_cast<const uint2*>(p);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; i++) t[i] = p[i];
-    }
-    return make_float4(to_f32(t[0]), to_f32(t[1]), to_f32(t[2]), to_f32(t[3]));
-}
-template <typename T>
-__device__ __forceinline__ void store4(T* p, bool vec, float4 x) {
-    T t[4] = {from_f32<T>(x.x), from_f32<T>(x.y), from_f32<T>(x.z), from_f32<T>(x.w)};
-    if (vec) {
-        if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(p) = *reinterpret_cast<uint4*>(t);
-        else *reinterpret_cast<uint2*>(p) = *reinterpret_cast<uint2*>(t);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; i++) p[i] = t[i];
-    }
-}
-
 template <int HDP, int D, bool WIDE> struct KvaShape {
     static constexpr int kUnitLog = WIDE ? 3 : D == 2 ? 2 : 1, kUnit = 1 << kUnitLog;   // rows
     static constexpr int kSlot = kKvaT * HDP;

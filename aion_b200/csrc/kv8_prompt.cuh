@@ -201,13 +201,9 @@ __global__ void __launch_bounds__(kKvpThreads, 1) k_kv_prompt(const KvAttnArgs a
     const int h = blockIdx.y, place = gridDim.x - 1 - blockIdx.x;   // late rows, which see most, first
     int blk = 0, s = 0;
     {
-        int lo = 0, hi = a.r.n_seq - 1;   // places of a sequence: (rows before it / ROWS) + its number, on
+        // places of a sequence: (rows before it / ROWS) + its number, on
         auto first = [&](int i) { return (int)((long long)a.r.begin(i) * a.group / ROWS) + i; };
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if (first(mid) <= place) lo = mid;
-            else hi = mid - 1;
-        }
+        const int lo = kv_warp_find(a.r.n_seq, place, first);
         s = lo;
         blk = place - first(lo);
     }
