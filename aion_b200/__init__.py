@@ -515,40 +515,40 @@ class KV8Cache:
                       k.device.index, n_layers, n_pages, n_kv, page, hd, max_seqs, max_pages)
         self._p = ctypes.addressof(self._c)
         self._types = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+        self._dev, self._int = k.device.index, torch.int32
+        self._empty_like, self._new, self._lib = torch.empty_like, torch.empty, lib()
+        self._raw_stream = torch._C._cuda_getCurrentRawStream
         self._ws = {}   # bytes of workspace by (heads, sequences, rows)
-        if lib().aion_kv8_attention_workspace(self._p, n_kv, 1, 1) < 0:
+        if self._lib.aion_kv8_attention_workspace(self._p, n_kv, 1, 1) < 0:
             _check(3)
 
-    # -- arguments ----------------------------------------------------------
+    # -- arguments: calls take a few microseconds, so these checks are terse --
     def _stream(self, stream):
-        if stream is None:
-            import torch
-            return torch.cuda.current_stream(self.device).cuda_stream
-        return getattr(stream, "cuda_stream", stream)
+        return self._raw_stream(self._dev) if stream is None else getattr(stream, "cuda_stream", stream)
 
     def _empty(self, shape, dtype, stream):
         """A new tensor that belongs to the stream the call runs on."""
-        import torch
         if stream is None:
-            return torch.empty(shape, dtype=dtype, device=self.device)
+            return self._new(shape, dtype=dtype, device=self.device)
+        import torch
         if isinstance(stream, int):
             stream = torch.cuda.ExternalStream(stream, device=self.device)
         with torch.cuda.stream(stream):
             return torch.empty(shape, dtype=dtype, device=self.device)
 
     def _ints(self, name: str, t, n: int) -> int:
-        if t.dtype != self.tables.dtype or t.device != self.device or not t.is_contiguous() or t.numel() < n:
+        if t.dtype is not self._int or t.get_device() != self._dev or t.numel() < n or not t.is_contiguous():
             raise ValueError(f"{name}: expected a contiguous int32 tensor with >= {n} elements on {self.device}")
         return t.data_ptr()
 
     def _rows(self, name: str, t, n: int, heads: int):
         """(pointer, row stride) of an [n][heads][head_size] tensor whose rows are dense."""
-        if t.dtype not in self._types or t.device != self.device:
+        if t.get_device() != self._dev or t.dtype not in self._types:
             raise ValueError(f"{name}: expected an fp32, fp16 or bf16 tensor on {self.device}")
-        if tuple(t.shape) != (n, heads, self.head_size):
-            raise ValueError(f"{name}: expected shape {(n, heads, self.head_size)}, got {tuple(t.shape)}")
-        st = t.stride()
-        if (st[2] != 1 and self.head_size > 1) or (heads > 1 and st[1] != self.head_size):
+        sh, st, hd = t.shape, t.stride(), self.head_size
+        if len(sh) != 3 or sh[0] != n or sh[1] != heads or sh[2] != hd:
+            raise ValueError(f"{name}: expected shape {(n, heads, hd)}, got {tuple(sh)}")
+        if st[2] != 1 or (st[1] != hd and heads > 1):
             raise ValueError(f"{name}: the values of one token must be dense (strides {st})")
         return t.data_ptr(), st[0]
 
@@ -570,7 +570,7 @@ class KV8Cache:
         if k.dtype != v.dtype:
             raise ValueError("k and v differ in type")
         sp, pp, cp, n = self._seqs(seqs, pos0, cu, n_tok)
-        st = lib().aion_kv8_append(self._p, layer, kp, vp, self._types[k.dtype], ks, vs, sp, pp, cp, n, n_tok,
+        st = self._lib.aion_kv8_append(self._p, layer, kp, vp, self._types[k.dtype], ks, vs, sp, pp, cp, n, n_tok,
                                    self._stream(stream))
         if st:
             _check(st)
@@ -588,7 +588,7 @@ class KV8Cache:
         if k.dtype != v.dtype:
             raise ValueError("k and v differ in type")
         sp, pp, cp, n = self._seqs(seqs, pos0, cu, n_tok)
-        st = lib().aion_kv8_read(self._p, layer, kp, vp, self._types[k.dtype], ks, vs, sp, pp, cp, n, n_tok,
+        st = self._lib.aion_kv8_read(self._p, layer, kp, vp, self._types[k.dtype], ks, vs, sp, pp, cp, n, n_tok,
                                  self._stream(stream))
         if st:
             _check(st)
@@ -615,11 +615,11 @@ class KV8Cache:
         if ws is None:
             if len(self._ws) > 4096:   # ragged serving meets many shapes
                 self._ws.clear()
-            ws = self._ws[key] = lib().aion_kv8_attention_workspace(self._p, *key)
+            ws = self._ws[key] = self._lib.aion_kv8_attention_workspace(self._p, *key)
             if ws < 0:
                 _check(3)
         buf = self._empty((ws,), self.k.dtype, stream) if ws else None
-        st = lib().aion_kv8_attention(self._p, layer, qp, op, self._types[q.dtype], n_heads, qs, os_, scale, sp, pp, cp,
+        st = self._lib.aion_kv8_attention(self._p, layer, qp, op, self._types[q.dtype], n_heads, qs, os_, scale, sp, pp, cp,
                                       n, n_tok, buf.data_ptr() if ws else None, ws, self._stream(stream))
         if st:
             _check(st)
@@ -633,7 +633,7 @@ class KV8Cache:
         n = seqs.numel()
         if pos0 is None:
             pos0 = self._empty((n,), seqs.dtype, stream)
-        st = lib().aion_kv8_grow(self._p, self._ints("seqs", seqs, n), self._ints("n_new", n_new, n), n,
+        st = self._lib.aion_kv8_grow(self._p, self._ints("seqs", seqs, n), self._ints("n_new", n_new, n), n,
                                  self._ints("pos0", pos0, n), self._stream(stream))
         if st:
             _check(st)
@@ -643,7 +643,7 @@ class KV8Cache:
         """Slot dst[i] shares the pages of slot src[i]'s first keep[i] tokens
         (None: all of them) (aion_kv8_fork)."""
         n = src.numel()
-        st = lib().aion_kv8_fork(self._p, self._ints("src", src, n), self._ints("dst", dst, n),
+        st = self._lib.aion_kv8_fork(self._p, self._ints("src", src, n), self._ints("dst", dst, n),
                                  None if keep is None else self._ints("keep", keep, n), n, self._stream(stream))
         if st:
             _check(st)
@@ -652,7 +652,7 @@ class KV8Cache:
         """Slot seqs[i] keeps its first keep[i] tokens (None: none)
         (aion_kv8_trim)."""
         n = seqs.numel()
-        st = lib().aion_kv8_trim(self._p, self._ints("seqs", seqs, n),
+        st = self._lib.aion_kv8_trim(self._p, self._ints("seqs", seqs, n),
                                  None if keep is None else self._ints("keep", keep, n), n, self._stream(stream))
         if st:
             _check(st)
@@ -660,19 +660,19 @@ class KV8Cache:
     def compact(self, n_used=None, stream=None) -> None:
         """Moves pages until those in use come first; n_used (int32, one element)
         receives their number (aion_kv8_compact)."""
-        st = lib().aion_kv8_compact(self._p, None if n_used is None else self._ints("n_used", n_used, 1),
+        st = self._lib.aion_kv8_compact(self._p, None if n_used is None else self._ints("n_used", n_used, 1),
                                     self._stream(stream))
         if st:
             _check(st)
 
     def reset(self, stream=None) -> None:
         """Empties every slot and frees every page."""
-        _check(lib().aion_kv8_reset(self._p, self._stream(stream)))
+        _check(self._lib.aion_kv8_reset(self._p, self._stream(stream)))
 
     def status(self, stream=None) -> None:
         """Waits for the stream; raises AionError for what the calls before it
         refused on the device (aion_kv8_status)."""
-        _check(lib().aion_kv8_status(self._p, self._stream(stream)))
+        _check(self._lib.aion_kv8_status(self._p, self._stream(stream)))
 
 
 __all__ = ["AionError", "Config", "KV8Cache", "Model", "QMatrix", "checkpoint_bytes", "lib", "quantize_activations",
