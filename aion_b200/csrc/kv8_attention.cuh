@@ -147,6 +147,12 @@ __device__ __forceinline__ void kv_vet_seq(const KvAttnArgs& a, const KvSeq& q) 
     else if ((long long)q.p0 + q.cnt > q.len) kv_flag(a.c, KV_BAD_PAGE);
 }
 
+// x / d for x >= 0, d > 0; 64-bit division is a long sequence, so it is kept for what needs it.
+__device__ __forceinline__ long long kv_div(long long x, int d) {
+    if ((x >> 32) == 0) return (uint32_t)x / (uint32_t)d;
+    return x / d;
+}
+
 // A place in the line of groups.
 struct KvCursor {
     KvSeq q;
@@ -154,9 +160,9 @@ struct KvCursor {
     __device__ __forceinline__ void seek(const KvAttnArgs& a, int seq, long long rest) {
         s = seq;
         q = kv_seq(a, s);
-        const long long u = rest / q.ng;
+        const long long u = kv_div(rest, q.ng);
         g = (int)(rest - u * q.ng);
-        h = (int)(u / q.nrg);
+        h = (int)kv_div(u, q.nrg);
         rg = (int)(u - (long long)h * q.nrg);
     }
     __device__ __forceinline__ void next(const KvAttnArgs& a) {
@@ -196,7 +202,7 @@ template <int HDP, int D, bool WIDE> struct KvaShape {
     static constexpr int kWords = D == 2 && !WIDE ? 36 : 68;   // of a row of weights: 64 of them (16-bit for 4 rows x 2 digits), padded
     static_assert(kRing % 16 == 0 && kUnit * kWords * 4 <= kSlot && kPiece <= kRing && kPiece % 16 == 0, "the places of the weights and pieces");
     struct Info {   // of a piece; the unit's groups from the block's first one on
-        int begin, end, s, h, rg, valid;
+        int begin, end, s, h, rg, rows;   // rows 0: no piece
     };
     static constexpr int kQueue = (4 * 4 + 4 * 8) * 4;   // pages and scales of four groups
     static constexpr int kPieces = kKvaWarps * kRing, kQueues = kPieces + kKvaWarps * kPiece;
@@ -263,15 +269,17 @@ __global__ void __launch_bounds__(kKvaThreads, KvaShape<HDP, D, WIDE>::kBlocks) 
         return lo;
     };
     // a group for each warp at least: few blocks where there is little to do
-    const long long nb = min((long long)gridDim.x, (W + kKvaWarps - 1) / kKvaWarps);
-    long long b0 = blockIdx.x >= nb ? W : W * blockIdx.x / nb, b1 = blockIdx.x + 1 >= nb ? W : W * (blockIdx.x + 1) / nb;
+    const int nb = (int)min((long long)gridDim.x, (W + kKvaWarps - 1) / kKvaWarps);
+    const long long share = kv_div(W, max(nb, 1)), more = W - share * nb;   // the first `more` blocks take one group more
+    auto start = [&](int b) { return b >= nb ? W : share * b + min((long long)b, more); };
+    long long b0 = start(blockIdx.x), b1 = start(blockIdx.x + 1);
     if (a.whole) {   // up to the next unit's start
         if (threadIdx.x < 2) {
             long long v = threadIdx.x ? b1 : b0;
             if (v < W) {
                 const int s = find(v);
                 const long long ng = kv_seq(a, s).ng, rest = v - pre[s];
-                v = pre[s] + (rest + ng - 1) / ng * ng;
+                v = pre[s] + kv_div(rest + ng - 1, (int)ng) * ng;
             }
             s_range[threadIdx.x] = v;
         }
@@ -286,7 +294,7 @@ __global__ void __launch_bounds__(kKvaThreads, KvaShape<HDP, D, WIDE>::kBlocks) 
         const int s = find(w0);
         ahead.seek(a, s, w0 - pre[s]);
     }
-    if (lane < 2) info[2 * warp + lane].valid = 0;
+    if (lane < 2) info[2 * warp + lane].rows = 0;
     __syncthreads();   // the ring is free
 
     // ---- copies
@@ -472,7 +480,9 @@ __global__ void __launch_bounds__(kKvaThreads, KvaShape<HDP, D, WIDE>::kBlocks) 
             }
         }
         const int gg = it.g & 0x7FFFFFFF;
-        if (lane == 0) info[2 * warp + which] = {at - gg, at - gg + q.ng, it.s, it.h, it.rg, 1};
+        if (lane == 0)
+            info[2 * warp + which] = {at - gg, at - gg + q.ng, it.s, it.h, it.rg,
+                                      min(SH::kUnit, q.cnt * a.group - it.rg * SH::kUnit)};
     };
 
     // ---- the stretch.  Turn i uses group i; it also fetches V of i + 1, K of i + 2 and the pages of i + 3, and the
@@ -634,48 +644,52 @@ __global__ void __launch_bounds__(kKvaThreads, KvaShape<HDP, D, WIDE>::kBlocks) 
         parts[threadIdx.x].at = b0;
     }
     __syncthreads();
+    // Pieces in the line's order are 0..15 (a warp's first and last); the first piece of each unit leads.  Warps take
+    // (unit, row) in turn: lane i weighs piece i.
     const int nblk = (int)(b1 - b0);
+    const typename SH::Info mine_info = info[lane & 15];
+    const unsigned have = __ballot_sync(0xffffffffu, lane < 16 && mine_info.rows);
+    int task = 0;
 #pragma unroll 1
-    for (int first = warp; first < 2 * kKvaWarps; first += kKvaWarps) {
-        const typename SH::Info f = info[first];
-        if (!f.valid) continue;
-        int prev = first - 1;
-        while (prev >= 0 && !info[prev].valid) prev--;
-        if (prev >= 0 && info[prev].begin == f.begin) continue;   // the unit's first piece leads
-        const bool all = f.begin >= 0 && f.end <= nblk;
-        KvPart* part = all ? nullptr : parts + (f.begin <= 0 ? 0 : 1);
-        if (!all && lane == 0) {
-            part->begin = b0 + f.begin;
-            part->end = b0 + f.end;
-            part->s = f.s;
-            part->h = f.h;
-            part->rg = f.rg;
+    for (unsigned todo = have; todo;) {
+        const int lead = __ffs(todo) - 1;
+        const int begin = __shfl_sync(0xffffffffu, mine_info.begin, lead), end = __shfl_sync(0xffffffffu, mine_info.end, lead);
+        const unsigned group = __ballot_sync(0xffffffffu, lane < 16 && mine_info.rows && mine_info.begin == begin);
+        todo &= ~group;
+        const int us = __shfl_sync(0xffffffffu, mine_info.s, lead), uh = __shfl_sync(0xffffffffu, mine_info.h, lead),
+                  urg = __shfl_sync(0xffffffffu, mine_info.rg, lead);
+        const bool all = begin >= 0 && end <= nblk;
+        KvPart* part = all ? nullptr : parts + (begin <= 0 ? 0 : 1);
+        if (!all && threadIdx.x == 0) {
+            part->begin = b0 + begin;
+            part->end = b0 + end;
+            part->s = us;
+            part->h = uh;
+            part->rg = urg;
             part->valid = 1;
         }
-        const KvSeq q = kv_seq(a, f.s);
-        auto piece = [&](int i) {
-            return reinterpret_cast<const float*>(i & 1 ? smem + (i >> 1) * SH::kRing : smem + SH::kPieces + (i >> 1) * SH::kPiece);
-        };
+        const int rows = __shfl_sync(0xffffffffu, mine_info.rows, lead);
+        const float* piece = reinterpret_cast<const float*>(lane & 1 ? smem + ((lane >> 1) & 7) * SH::kRing
+                                                                     : smem + SH::kPieces + ((lane >> 1) & 7) * SH::kPiece);
 #pragma unroll 1
-        for (int r = 0; r < SH::kUnit; r++) {
-            const KvRow row = kv_row(a, q, f.h, f.rg, r);
-            if (row.out < 0) break;
-            float mx = -INFINITY, ls = 0.0f, os[HDP / 32];
-#pragma unroll 1
-            for (int i = first; i < 2 * kKvaWarps; i++)
-                if (info[i].valid && info[i].begin == f.begin) mx = fmaxf(mx, piece(i)[SH::kUnit * HDP + r]);
+        for (int r = 0; r < rows; r++, task++) {
+            if ((task & (kKvaWarps - 1)) != warp) continue;
+            const bool in = (group >> lane) & 1;
+            const float pm = in ? piece[SH::kUnit * HDP + r] : -INFINITY;
+            const float mx = warp_max(pm), wgt = pm == -INFINITY ? 0.0f : kv_exp2(pm - mx);
+            const float ls = warp_sum(in ? wgt * piece[SH::kUnit * HDP + SH::kUnit + r] : 0.0f);
+            float os[HDP / 32] = {};
+#pragma unroll 4
+            for (int i = 0; i < 16; i++) {
+                const float w = __shfl_sync(0xffffffffu, wgt, i);
+                if (!((group >> i) & 1)) continue;
+                const float* p = reinterpret_cast<const float*>(i & 1 ? smem + (i >> 1) * SH::kRing
+                                                                      : smem + SH::kPieces + (i >> 1) * SH::kPiece);
 #pragma unroll
-            for (int e = 0; e < HDP / 32; e++) os[e] = 0.0f;
-#pragma unroll 1
-            for (int i = first; i < 2 * kKvaWarps; i++) {
-                if (!info[i].valid || info[i].begin != f.begin) continue;
-                const float* p = piece(i);
-                const float pm = p[SH::kUnit * HDP + r], wgt = pm == -INFINITY ? 0.0f : kv_exp2(pm - mx);
-                ls += wgt * p[SH::kUnit * HDP + SH::kUnit + r];
-#pragma unroll
-                for (int e = 0; e < HDP / 32; e++) os[e] += wgt * p[r * HDP + lane + 32 * e];
+                for (int e = 0; e < HDP / 32; e++) os[e] += w * p[r * HDP + lane + 32 * e];
             }
             if (all) {
+                const KvRow row = kv_row(a, kv_seq(a, us), uh, urg, r);
                 const float inv = ls == 0.0f ? 0.0f : 1.0f / ls;
 #pragma unroll
                 for (int e = 0; e < HDP / 32; e++)
@@ -716,23 +730,32 @@ __global__ void __launch_bounds__(kKvJoinThreads) k_kv_attention_join(const KvAt
     if (!other)
         while (end < blocks && a.parts[2 * (size_t)end].valid && a.parts[2 * (size_t)end].begin == ubegin) end++;
     const KvSeq q = kv_seq(a, s);
+    const int np = end - (b - 1);
     for (int r = warp; r < 1 << a.unit_log; r += kKvJoinThreads / 32) {
         const KvRow row = kv_row(a, q, h, rg, r);
         if (row.out < 0) break;
-        float mx = head->m[r];
-        for (int i = b; i < end; i++) mx = fmaxf(mx, a.parts[2 * (size_t)i].m[r]);
-        float ls = 0.0f;
+        float mx = -INFINITY, ls = 0.0f;
         float4 os = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-        for (int i = b - 1; i < end; i++) {
-            const KvPart* p = i < b ? head : a.parts + 2 * (size_t)i;
-            const float pm = p->m[r], wgt = pm == -INFINITY ? 0.0f : kv_exp2(pm - mx);
-            const float4 x = *reinterpret_cast<const float4*>(&p->o[r][4 * lane]);
-            ls += wgt * p->l[r];
-            os.x += wgt * x.x;
-            os.y += wgt * x.y;
-            os.z += wgt * x.z;
-            os.w += wgt * x.w;
+        for (int base = 0; base < np; base += 32) {   // lane i weighs part base + i
+            const KvPart* p = base + lane == 0 ? head : p0 + 2 * (size_t)(base + lane);
+            const bool in = base + lane < np;
+            const float pm = in ? p->m[r] : -INFINITY, pl = in ? p->l[r] : 0.0f;
+            const float mn = fmaxf(mx, warp_max(pm)), wgt = pm == -INFINITY ? 0.0f : kv_exp2(pm - mn);
+            const float old = mx == -INFINITY ? 0.0f : kv_exp2(mx - mn);
+            mx = mn;
+            ls = ls * old + warp_sum(wgt * pl);
+            os = make_float4(os.x * old, os.y * old, os.z * old, os.w * old);
+            const int n = min(np - base, 32);
+#pragma unroll 8
+            for (int i = 0; i < n; i++) {
+                const KvPart* pi = base + i == 0 ? head : p0 + 2 * (size_t)(base + i);
+                const float w = __shfl_sync(0xffffffffu, wgt, i);
+                const float4 x = *reinterpret_cast<const float4*>(&pi->o[r][4 * lane]);
+                os.x += w * x.x;
+                os.y += w * x.y;
+                os.z += w * x.z;
+                os.w += w * x.w;
+            }
         }
         const float inv = ls == 0.0f ? 0.0f : 1.0f / ls;
         if (4 * lane < a.c.hd)
