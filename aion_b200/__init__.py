@@ -137,6 +137,7 @@ def lib() -> ctypes.CDLL:
         "aion_kv8_attention": (I32, [VP, I32, VP, VP, I32, I32, I64, I64, F, VP, VP, VP, I32, I32, VP, I64, VP]),
         "aion_kv8_attention_workspace": (I64, [VP, I32, I32, I32]),
         "aion_kv8_status": (I32, [VP, VP]),
+        "aion_extend": (I32, [VP, VP, VP, VP, VP, I32, VP]),
         "aion_quantize_buffer": (None, [VP, VP, VP, I64]),
         "aion_checkpoint_bytes": (I64, [P(I32), ctypes.c_int]),
         "aion_quantize_file": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_char_p, ctypes.c_int, ctypes.c_char_p,
@@ -329,6 +330,25 @@ class Model:
         _check(lib().aion_decode_batch(self._h, f.size, steps, _ptr(f), _ptr(p), _ptr(toks),
                                        _ptr(lg) if lg is not None else None), self._h)
         return toks, lg
+
+    def extend(self, cache: "KV8Cache", seqs, tokens, want_logits: bool = True):
+        """Runs tokens[i] (one list of token ids a sequence) behind what slot
+        seqs[i] of the 8-bit paged cache holds; returns the logits of each
+        sequence's last token, [len(seqs)][vocab], or None (aion_extend).
+        Work on the cache in torch's current stream is waited for; other
+        streams' has to be complete."""
+        import torch
+        new = [np.ascontiguousarray(t, dtype=np.int32).ravel() for t in tokens]
+        s = np.ascontiguousarray(seqs, dtype=np.int32).ravel()
+        if s.size != len(new):
+            raise ValueError("seqs and tokens differ in length")
+        n = np.array([t.size for t in new], np.int32)
+        flat = np.concatenate(new) if new else np.empty(0, np.int32)
+        out = np.empty((s.size, self.config.vocab_size), np.float32) if want_logits else None
+        torch.cuda.current_stream(cache.device).synchronize()
+        _check(lib().aion_extend(self._h, cache._p, _ptr(s), _ptr(n), _ptr(flat), s.size,
+                                 _ptr(out) if out is not None else None), self._h)
+        return out
 
     def set_sampler(self, temperature: float = 0.0, top_p: float = 1.0, top_k: int = 0, seed: int = 0) -> None:
         """Next-token rule of the decode calls: greedy when temperature <= 0,

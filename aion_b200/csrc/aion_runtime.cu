@@ -297,12 +297,14 @@ struct aion_ctx {
     int nseq = 1;                  // sequences (KV caches) held; opts.max_batch
     int cur_seq = 0;               // the sequence decode / forward calls run on
     size_t kv_seq = 0;             // floats per sequence in kcache / vcache
-    struct PrefillBufs {           // grown on demand by aion_prefill
+    struct PrefillBufs {           // grown on demand by aion_prefill and aion_extend
         __nv_bfloat16 *a = nullptr, *b = nullptr;
         float *c = nullptr, *x = nullptr, *q = nullptr;
         int32_t* tok = nullptr;
         int* map = nullptr;
-        size_t a_cap = 0, b_cap = 0, c_cap = 0, x_cap = 0, q_cap = 0, tok_cap = 0, map_cap = 0;
+        int32_t* seq = nullptr;    // aion_extend: slots, new tokens, positions, row offsets, row positions
+        void* ws = nullptr;        // its attention's workspace
+        size_t a_cap = 0, b_cap = 0, c_cap = 0, x_cap = 0, q_cap = 0, tok_cap = 0, map_cap = 0, seq_cap = 0, ws_cap = 0;
     } pf;
     struct BatchBufs {             // lock-step batched decode, allocated on first use
         float *x = nullptr, *q = nullptr, *att = nullptr, *logits = nullptr;
@@ -487,7 +489,7 @@ static void ctx_destroy(aion_ctx* c) {
     if (c->peers_dev) cudaFree(c->peers_dev);
     if (c->xr) cudaFree(c->xr);
     for (void* p : {(void*)c->pf.a, (void*)c->pf.b, (void*)c->pf.c, (void*)c->pf.x, (void*)c->pf.q,
-                    (void*)c->pf.tok, (void*)c->pf.map})
+                    (void*)c->pf.tok, (void*)c->pf.map, (void*)c->pf.seq, c->pf.ws})
         if (p) cudaFree(p);
     for (void* p : {(void*)c->bt.x, (void*)c->bt.q, (void*)c->bt.att, (void*)c->bt.dg, (void*)c->bt.logits,
                     (void*)c->bt.part, (void*)c->bt.ssq, (void*)c->bt.argmax, (void*)c->bt.first, (void*)c->bt.pos0, (void*)c->bt.tokens})
@@ -1329,6 +1331,28 @@ static aion_status pf_matmul(aion_ctx* c, const MatDesc& w, long long mpad, long
     return s;
 }
 
+// The operand buffers of a pass over mrows rows with the logits of n_seq of them.
+static aion_status pf_reserve(aion_ctx* c, long long mrows, long long n_seq) {
+    const long long dim = c->dim, hid = c->hidden, kv = c->kv_dim;
+    const long long mpad = round_up(mrows, kGemmBM), kpd = round_up(dim, kGemmBK), kph = round_up(hid, kGemmBK);
+    const long long np_max = std::max({round_up(dim + 2 * kv, kGemmBN), round_up(2 * hid, kGemmBN),
+                                       round_up(dim, kGemmBN)});
+    const long long np_cls = round_up(c->vocab, kGemmBN), mcls = round_up(n_seq, kGemmBM);
+    const long long kmax = std::max(kpd, kph);
+    const size_t a_bytes = (size_t)std::max(mpad, mcls) * 3 * kmax * 2;
+    const size_t b_bytes = (size_t)std::max({np_max * 3 * kpd, round_up(dim, kGemmBN) * 3 * kph, np_cls * 3 * kpd}) * 2;
+    const size_t c_bytes = (size_t)std::max(mpad * np_max, mcls * np_cls) * 4;
+    auto& pf = c->pf;
+    CK_RET(&c->err, pf_grow((void**)&pf.a, &pf.a_cap, a_bytes));
+    CK_RET(&c->err, pf_grow((void**)&pf.b, &pf.b_cap, b_bytes));
+    CK_RET(&c->err, pf_grow((void**)&pf.c, &pf.c_cap, c_bytes));
+    CK_RET(&c->err, pf_grow((void**)&pf.x, &pf.x_cap, (size_t)mrows * dim * 4));
+    CK_RET(&c->err, pf_grow((void**)&pf.q, &pf.q_cap, (size_t)mrows * dim * 4));
+    CK_RET(&c->err, pf_grow((void**)&pf.tok, &pf.tok_cap, (size_t)mrows * 4));
+    CK_RET(&c->err, pf_grow((void**)&pf.map, &pf.map_cap, (size_t)mcls * 4));
+    return AION_OK;
+}
+
 extern "C" AION_API aion_status aion_prefill(aion_ctx* c, const int32_t* tokens, int32_t n_seq, int32_t n_tok,
                                              float* logits_host) {
     if (!c || !tokens || n_seq < 1 || n_tok < 1) return AION_ERR_ARG;
@@ -1348,23 +1372,11 @@ extern "C" AION_API aion_status aion_prefill(aion_ctx* c, const int32_t* tokens,
         }
     CK_RET(&c->err, cudaSetDevice(c->dev));
     const long long dim = c->dim, hid = c->hidden, kv = c->kv_dim, L = c->L;
-    const long long mrows = (long long)n_seq * n_tok, mpad = round_up(mrows, kGemmBM);
+    const long long mrows = (long long)n_seq * n_tok, mpad = round_up(mrows, kGemmBM), mcls = round_up(n_seq, kGemmBM);
     const long long kpd = round_up(dim, kGemmBK), kph = round_up(hid, kGemmBK);
-    const long long np_max = std::max({round_up(dim + 2 * kv, kGemmBN), round_up(2 * hid, kGemmBN),
-                                       round_up(dim, kGemmBN)});
-    const long long np_cls = round_up(c->vocab, kGemmBN), mcls = round_up(n_seq, kGemmBM);
-    const long long kmax = std::max(kpd, kph);
-    const size_t a_bytes = (size_t)std::max(mpad, mcls) * 3 * kmax * 2;
-    const size_t b_bytes = (size_t)std::max({np_max * 3 * kpd, round_up(dim, kGemmBN) * 3 * kph, np_cls * 3 * kpd}) * 2;
-    const size_t c_bytes = (size_t)std::max(mpad * np_max, mcls * np_cls) * 4;
     auto& pf = c->pf;
-    CK_RET(&c->err, pf_grow((void**)&pf.a, &pf.a_cap, a_bytes));
-    CK_RET(&c->err, pf_grow((void**)&pf.b, &pf.b_cap, b_bytes));
-    CK_RET(&c->err, pf_grow((void**)&pf.c, &pf.c_cap, c_bytes));
-    CK_RET(&c->err, pf_grow((void**)&pf.x, &pf.x_cap, (size_t)mrows * dim * 4));
-    CK_RET(&c->err, pf_grow((void**)&pf.q, &pf.q_cap, (size_t)mrows * dim * 4));
-    CK_RET(&c->err, pf_grow((void**)&pf.tok, &pf.tok_cap, (size_t)mrows * 4));
-    CK_RET(&c->err, pf_grow((void**)&pf.map, &pf.map_cap, (size_t)mcls * 4));
+    const aion_status rs = pf_reserve(c, mrows, n_seq);
+    if (rs != AION_OK) return rs;
     CK_RET(&c->err, cudaMemcpyAsync(pf.tok, tokens, (size_t)mrows * 4, cudaMemcpyHostToDevice, c->stream));
     std::vector<int> map(n_seq);
     for (int s = 0; s < n_seq; s++) map[s] = s * n_tok + n_tok - 1;
@@ -1435,6 +1447,149 @@ extern "C" AION_API aion_status aion_prefill(aion_ctx* c, const int32_t* tokens,
         CK_RET(&c->err, cudaMemcpy2DAsync(logits_host, (size_t)c->vocab * 4, pf.c, (size_t)np * 4,
                                           (size_t)c->vocab * 4, (size_t)n_seq, cudaMemcpyDeviceToHost, c->stream));
     CK_RET(&c->err, cudaStreamSynchronize(c->stream));
+    return check_device_error(c);
+}
+
+// ---------------------------------------------------------------------------
+// New tokens of several sequences against an 8-bit paged cache (aion_kv8)
+// ---------------------------------------------------------------------------
+// Gives back what aion_kv8_grow granted: every granted slot to its length before.
+static void extend_undo(aion_ctx* c, const aion_kv8* kv, const int32_t* seqs, const std::vector<int32_t>& pos0) {
+    std::vector<int32_t> list, keep;
+    for (size_t i = 0; i < pos0.size(); i++)
+        if (pos0[i] >= 0) {
+            list.push_back(seqs[i]);
+            keep.push_back(pos0[i]);
+        }
+    const size_t n = list.size();
+    list.insert(list.end(), keep.begin(), keep.end());
+    if (n && cudaMemcpyAsync(c->pf.seq, list.data(), list.size() * 4, cudaMemcpyHostToDevice, c->stream) == cudaSuccess)
+        aion_kv8_trim(kv, c->pf.seq, c->pf.seq + n, (int32_t)n, c->stream);
+    cudaStreamSynchronize(c->stream);
+    aion_kv8_status(kv, c->stream);   // the refusal is this call's to report
+}
+
+extern "C" AION_API aion_status aion_extend(aion_ctx* c, const aion_kv8* kv, const int32_t* seqs, const int32_t* n_new,
+                                            const int32_t* tokens, int32_t n_seq, float* logits_host) {
+    if (!c || !kv || !seqs || !n_new || !tokens || n_seq < 1) return AION_ERR_ARG;
+    if (c->tp_n > 1 || c->mode == MODE_F32) {
+        set_err(&c->err, "aion_extend needs an int4 file on one GPU");
+        return AION_ERR_STATE;
+    }
+    if (kv->device != c->dev || kv->n_layers != c->L || kv->n_kv_heads != c->nkv || kv->head_size != c->hs) {
+        set_err(&c->err, "aion_extend: the cache (%d layers, %d K/V heads of %d, device %d) is not of this model's shape", kv->n_layers,
+                kv->n_kv_heads, kv->head_size, kv->device);
+        return AION_ERR_SHAPE;
+    }
+    if (n_seq > 1024) {
+        set_err(&c->err, "aion_extend: %d sequences (at most 1024)", n_seq);
+        return AION_ERR_ARG;
+    }
+    long long mrows = 0;
+    std::vector<int32_t> cu(1, 0);
+    std::vector<char> seen((size_t)std::max(kv->max_seqs, 0));
+    for (int i = 0; i < n_seq; i++) {
+        if (seqs[i] < 0 || seqs[i] >= kv->max_seqs || seen[seqs[i]] || n_new[i] < 1) {
+            set_err(&c->err, "aion_extend: sequence %d (slot %d, %d tokens) is out of range or names a slot twice", i, seqs[i],
+                    n_new[i]);
+            return AION_ERR_ARG;
+        }
+        seen[seqs[i]] = 1;
+        mrows += n_new[i];
+        if (mrows > (1 << 24)) {
+            set_err(&c->err, "aion_extend: more than %d tokens", 1 << 24);
+            return AION_ERR_ARG;
+        }
+        cu.push_back((int32_t)mrows);
+    }
+    for (long long i = 0; i < mrows; i++)
+        if (tokens[i] < 0 || tokens[i] >= c->vocab) {
+            set_err(&c->err, "aion_extend: token %d at %lld out of range", tokens[i], i);
+            return AION_ERR_ARG;
+        }
+    CK_RET(&c->err, cudaSetDevice(c->dev));
+    const long long dim = c->dim, hid = c->hidden, kvd = c->kv_dim, mpad = round_up(mrows, kGemmBM);
+    const long long kpd = round_up(dim, kGemmBK), kph = round_up(hid, kGemmBK), mcls = round_up(n_seq, kGemmBM);
+    aion_status st = pf_reserve(c, mrows, n_seq);
+    if (st != AION_OK) return st;
+    auto& pf = c->pf;
+    const int64_t ws = aion_kv8_attention_workspace(kv, (int32_t)c->nh, n_seq, (int32_t)mrows);
+    auto kv_fail = [&](aion_status s) {
+        c->err = g_thread_err;
+        return s;
+    };
+    if (ws < 0) return kv_fail(AION_ERR_SHAPE);
+    CK_RET(&c->err, pf_grow(&pf.ws, &pf.ws_cap, (size_t)std::max<int64_t>(ws, 16)));
+    CK_RET(&c->err, pf_grow((void**)&pf.seq, &pf.seq_cap, (size_t)(4 * n_seq + 1 + mrows) * 4));
+    int32_t *d_seqs = pf.seq, *d_new = d_seqs + n_seq, *d_pos0 = d_new + n_seq, *d_cu = d_pos0 + n_seq, *d_pos = d_cu + n_seq + 1;
+    const cudaStream_t sm = c->stream;
+    CK_RET(&c->err, cudaMemcpyAsync(d_seqs, seqs, n_seq * 4, cudaMemcpyHostToDevice, sm));
+    CK_RET(&c->err, cudaMemcpyAsync(d_new, n_new, n_seq * 4, cudaMemcpyHostToDevice, sm));
+    CK_RET(&c->err, cudaMemcpyAsync(d_cu, cu.data(), cu.size() * 4, cudaMemcpyHostToDevice, sm));
+    CK_RET(&c->err, cudaMemcpyAsync(pf.tok, tokens, (size_t)mrows * 4, cudaMemcpyHostToDevice, sm));
+    st = aion_kv8_grow(kv, d_seqs, d_new, n_seq, d_pos0, sm);
+    if (st != AION_OK) return kv_fail(st);
+    std::vector<int32_t> pos0(n_seq);
+    CK_RET(&c->err, cudaMemcpyAsync(pos0.data(), d_pos0, n_seq * 4, cudaMemcpyDeviceToHost, sm));
+    CK_RET(&c->err, cudaStreamSynchronize(sm));
+    std::vector<int32_t> pos((size_t)mrows), map(n_seq);
+    for (int i = 0; i < n_seq; i++) {
+        if (pos0[i] < 0 || (long long)pos0[i] + n_new[i] > c->seq) {
+            const bool full = pos0[i] < 0;
+            if (full)
+                set_err(&c->err, "aion_extend: the cache has no room for sequence %d (slot %d, %d tokens)", i, seqs[i], n_new[i]);
+            else
+                set_err(&c->err, "aion_extend: sequence %d would reach position %lld of %lld", i, (long long)pos0[i] + n_new[i],
+                        (long long)c->seq);
+            extend_undo(c, kv, seqs, pos0);
+            return full ? AION_ERR_OOM : AION_ERR_ARG;
+        }
+        for (int t = 0; t < n_new[i]; t++) pos[(size_t)cu[i] + t] = pos0[i] + t;
+        map[i] = cu[i + 1] - 1;
+    }
+    CK_RET(&c->err, cudaMemcpyAsync(d_pos, pos.data(), (size_t)mrows * 4, cudaMemcpyHostToDevice, sm));
+    CK_RET(&c->err, cudaMemcpyAsync(pf.map, map.data(), n_seq * 4, cudaMemcpyHostToDevice, sm));
+
+    const unsigned rows = (unsigned)mrows, padded = (unsigned)mpad;
+    k_pf_embed<<<rows, 256, 0, sm>>>(pf.tok, (int)mrows, c->emb, (int)dim, pf.x);
+    CK_RET(&c->err, cudaGetLastError());
+    for (int l = 0; l < (int)c->L; l++) {
+        long long np = 0;
+        k_pf_norm_split<<<padded, 256, 0, sm>>>(pf.x, nullptr, (int)mrows, (int)dim, (int)kpd, c->rms_att + l * dim, pf.a);
+        st = pf_matmul(c, c->qkv[l], mpad, kpd, &np);
+        if (st != AION_OK) return st;
+        k_pf_rope_rows<<<rows, 256, 0, sm>>>(pf.c, (int)np, (int)mrows, d_pos, (int)dim, (int)kvd, (int)c->hs, c->freq_re,
+                                            c->freq_im);
+        CK_RET(&c->err, cudaGetLastError());
+        st = aion_kv8_append(kv, l, pf.c + dim, pf.c + dim + kvd, AION_F32, np, np, d_seqs, d_pos0, d_cu, n_seq,
+                             (int32_t)mrows, sm);
+        if (st == AION_OK)
+            st = aion_kv8_attention(kv, l, pf.c, pf.q, AION_F32, (int32_t)c->nh, np, dim, 0.0f, d_seqs, d_pos0, d_cu, n_seq,
+                                    (int32_t)mrows, pf.ws, ws, sm);
+        if (st != AION_OK) return kv_fail(st);
+        k_pf_split<<<padded, 256, 0, sm>>>(pf.q, (int)mrows, (int)dim, (int)kpd, pf.a);
+        st = pf_matmul(c, c->wo[l], mpad, kpd, &np);
+        if (st != AION_OK) return st;
+        k_pf_residual<<<rows, 256, 0, sm>>>(pf.x, pf.c, (int)np, (int)mrows, (int)dim);
+        k_pf_norm_split<<<padded, 256, 0, sm>>>(pf.x, nullptr, (int)mrows, (int)dim, (int)kpd, c->rms_ffn + l * dim, pf.a);
+        st = pf_matmul(c, c->w13[l], mpad, kpd, &np);
+        if (st != AION_OK) return st;
+        k_pf_swiglu_split<<<padded, 256, 0, sm>>>(pf.c, (int)np, (int)mrows, (int)hid, (int)kph, pf.a);
+        st = pf_matmul(c, c->w2[l], mpad, kph, &np);
+        if (st != AION_OK) return st;
+        k_pf_residual<<<rows, 256, 0, sm>>>(pf.x, pf.c, (int)np, (int)mrows, (int)dim);
+        CK_RET(&c->err, cudaGetLastError());
+    }
+    if (logits_host) {
+        k_pf_norm_split<<<(unsigned)mcls, 256, 0, sm>>>(pf.x, pf.map, n_seq, (int)dim, (int)kpd, c->rms_final, pf.a);
+        long long np = 0;
+        st = pf_matmul(c, c->emb, mcls, kpd, &np);
+        if (st != AION_OK) return st;
+        CK_RET(&c->err, cudaMemcpy2DAsync(logits_host, (size_t)c->vocab * 4, pf.c, (size_t)np * 4, (size_t)c->vocab * 4,
+                                          (size_t)n_seq, cudaMemcpyDeviceToHost, sm));
+    }
+    st = aion_kv8_status(kv, sm);
+    if (st != AION_OK) return kv_fail(st);
     return check_device_error(c);
 }
 

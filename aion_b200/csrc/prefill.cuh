@@ -415,6 +415,35 @@ __global__ void __launch_bounds__(kPfAttnThreads, 1) k_pf_attention(PfAttnArgs a
     }
 }
 
+// QKV output rows whose positions are given: q and K rotated in place
+// (src/kernel_simd.c:1068-1085); V stays.
+__global__ void k_pf_rope_rows(float* c, int ldc, int mrows, const int32_t* pos, int dim, int kv_dim, int hs,
+                               const float* freq_re, const float* freq_im) {
+    const int m = blockIdx.x;
+    if (m >= mrows) return;
+    float* cr = c + (size_t)m * ldc;
+    const size_t f = (size_t)pos[m] * (hs / 2);
+    for (int i = 2 * threadIdx.x; i < dim + kv_dim; i += 2 * blockDim.x) {
+        const int hd = (i < dim ? i : i - dim) % hs;
+        const float fr = freq_re[f + hd / 2], fi = freq_im[f + hd / 2];
+        const float v0 = cr[i], v1 = cr[i + 1];
+        cr[i] = __fsub_rn(__fmul_rn(v0, fr), __fmul_rn(v1, fi));
+        cr[i + 1] = __fadd_rn(__fmul_rn(v0, fi), __fmul_rn(v1, fr));
+    }
+}
+
+// A operand of rows as they are; rows >= mrows are zero.
+__global__ void k_pf_split(const float* x, int mrows, int k, int kp, __nv_bfloat16* out) {
+    const int m = blockIdx.x;
+    __nv_bfloat16* row = out + (size_t)m * 3 * kp;
+    for (int i = 8 * threadIdx.x; i < kp; i += 8 * blockDim.x) {
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] = m < mrows && i + e < k ? x[(size_t)m * k + i + e] : 0.0f;
+        split8_store<false>(row, kp, i, v);
+    }
+}
+
 // x[m][0:dim] += c[m][0:dim] (residual, src/kernel_simd.c:1126,1153).
 __global__ void k_pf_residual(float* x, const float* c, int ldc, int mrows, int dim) {
     const int m = blockIdx.x;

@@ -443,6 +443,24 @@ AION_API int64_t aion_kv8_attention_workspace(const aion_kv8* kv, int32_t n_head
  * of pages); the first of these that applies. */
 AION_API aion_status aion_kv8_status(const aion_kv8* kv, void* stream);
 
+/* Model level: runs new tokens of n_seq sequences (n_seq <= 1024) through the
+ * model against an 8-bit paged cache of the model's shape on the context's
+ * device (n_layers, n_kv_heads, head_size of the checkpoint).  Sequence i
+ * continues slot seqs[i] with n_new[i] >= 1 tokens; `tokens` holds all of
+ * them, sequence by sequence (all host memory).  Equivalent to transformer()
+ * (src/kernel_simd.c:1014) for each token at the slot's next position, with
+ * K and V rows held in 8 bits: prompts in chunks, single steps and drafts of
+ * sequences of different lengths in one call, on prefixes that
+ * aion_kv8_fork shares.  Products as in aion_prefill.  The slots grow by
+ * their tokens; logits_host[n_seq][vocab] (may be NULL) receives the logits
+ * of each sequence's last token.  Needs an int4 file and tp_size 1; W4A8
+ * contexts run the same products.  AION_ERR_OOM when the cache has no room
+ * for a sequence, AION_ERR_ARG when one would pass the checkpoint's seq_len:
+ * every slot is then as long as before.  Waits for its own work; what other
+ * streams do to the cache has to be complete before the call. */
+AION_API aion_status aion_extend(aion_ctx* ctx, const aion_kv8* kv, const int32_t* seqs, const int32_t* n_new,
+                                 const int32_t* tokens, int32_t n_seq, float* logits_host);
+
 /* ---------------------------------------------------------------------------
  * Checkpoint tools (host)
  * ------------------------------------------------------------------------- */
