@@ -275,55 +275,46 @@ __global__ void __launch_bounds__(kKvpThreads, 1) k_kv_prompt(const KvAttnArgs a
         const int tok = i / a.group, head = h * a.group + (i - tok * a.group);
         const bool live_row = i < total && 128 * tile + r < rows;
         const int lim = live_row ? (int)min((long long)q.p0 + tok, (long long)q.len - 1) : -1;
-        // the query row to shared memory
-        float up = 1.0f, rs;
+        // The warp's 32 query rows to shared memory, a row at a time so that its loads are one line after the other; lane l
+        // has dimensions 4 l..+3, and keeps what row l's scores are scaled by.
+        float rs = 1.0f;
         bool bad = false;
         {
-            const T* src = (const T*)a.q + (q.t0 + tok) * a.q_stride + (long long)head * c.hd;
+            const long long mine = live_row ? (q.t0 + tok) * a.q_stride + (long long)head * c.hd : -1;
             const float sign = a.scale < 0.0f ? -1.0f : 1.0f;
-            float top = 0.0f;
-            if (live_row) {
-                for (int d = 0; d < c.hd; d += 16) {
-                    float x[16];
-                    load16(src + d, a.vec_q, x);
-#pragma unroll
-                    for (int e = 0; e < 16; e++) {
-                        const float b = fabsf(x[e]);
-                        bad = bad || !(b <= 3.402823466e38f);
-                        top = fmaxf(top, b);
-                    }
-                }
-                if (!std::is_same<T, __half>::value) {   // the largest to 2^14..2^15
-                    const int e = top > 0.0f && !bad ? max(min(14 - ilogbf(top), 126), -126) : 0;
-                    up = __int_as_float((127 + e) << 23);
-                }
-            }
-            rs = bad ? 1.0f : fabsf(a.scale) / up;
-            for (int d = 0; d < c.hd; d += 16) {
-                float x[16];
-                if (live_row && !bad) {
-                    load16(src + d, a.vec_q, x);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 16; e++) x[e] = 0.0f;
-                }
-                uint32_t hi[8], lo[8];
+            const bool in = 4 * lane < c.hd;
+#pragma unroll 1
+            for (int r0 = 0; r0 < 32; r0 += 8) {
+                float4 v[8];
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
-                    const float x0 = x[2 * e] * up * sign, x1 = x[2 * e + 1] * up * sign;
-                    hi[e] = half2_bits(x0, x1);
-                    if (TERMS == 2) {
-                        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi[e]));
-                        lo[e] = half2_bits(x0 - f.x, x1 - f.y);
-                    }
+                    const long long from = __shfl_sync(0xffffffffu, mine, r0 + e);
+                    v[e] = from >= 0 && in ? load4((const T*)a.q + from + 4 * lane, a.vec_q) : make_float4(0, 0, 0, 0);
                 }
 #pragma unroll
-                for (int p = 0; p < 2; p++) {
-                    unsigned char* to = qs + tile * TERMS * kKvpQ + kvp_piece(128, r, d / 8 + p);
-                    *reinterpret_cast<uint4*>(to) = make_uint4(hi[4 * p], hi[4 * p + 1], hi[4 * p + 2], hi[4 * p + 3]);
-                    if (TERMS == 2)
-                        *reinterpret_cast<uint4*>(to + kKvpQ) =
-                            make_uint4(lo[4 * p], lo[4 * p + 1], lo[4 * p + 2], lo[4 * p + 3]);
+                for (int e = 0; e < 8; e++) {
+                    const uint32_t top = __reduce_max_sync(0xffffffffu, kv_top4(0, v[e]));
+                    const bool off = top >= 0x7F800000u;
+                    float up = 1.0f;   // the largest to 2^14..2^15, as far as a factor of 2^126 goes
+                    if (!std::is_same<T, __half>::value && top != 0 && !off)
+                        up = __uint_as_float((uint32_t)(127 + min(14 + 127 - (int)(top >> 23), 126)) << 23);
+                    const float f = off ? 0.0f : up * sign;
+                    if (off) v[e] = make_float4(0, 0, 0, 0);
+                    const float x0 = v[e].x * f, x1 = v[e].y * f, x2 = v[e].z * f, x3 = v[e].w * f;
+                    const uint2 hi = make_uint2(half2_bits(x0, x1), half2_bits(x2, x3));
+                    unsigned char* to = qs + tile * TERMS * kKvpQ + kvp_piece(128, 32 * (warp & 3) + r0 + e, lane >> 1) + 8 * (lane & 1);
+                    if (in) *reinterpret_cast<uint2*>(to) = hi;
+                    if (TERMS == 2) {
+                        const float2 a0 = __half22float2(*reinterpret_cast<const __half2*>(&hi.x)),
+                                     a1 = __half22float2(*reinterpret_cast<const __half2*>(&hi.y));
+                        if (in)
+                            *reinterpret_cast<uint2*>(to + kKvpQ) =
+                                make_uint2(half2_bits(x0 - a0.x, x1 - a0.y), half2_bits(x2 - a1.x, x3 - a1.y));
+                    }
+                    if (lane == r0 + e) {
+                        rs = off ? 1.0f : fabsf(a.scale) / up;
+                        bad = off;
+                    }
                 }
             }
         }
