@@ -47,7 +47,7 @@ constexpr int kKvpQ = 128 * 128 * 2;        // a query operand: 128 rows of two 
 constexpr int kKvpStage = 64 * 128 * 2;     // a key tile's K (64 rows, two halves) or V (up to 128 dimensions x 64 tokens)
 constexpr int kKvpRaw = 64 * 128;           // a key tile's K or V as the cache holds it
 constexpr int kKvpSmem = 2 * kKvpQ + 8 * kKvpStage + 4 * kKvpRaw + 1024;
-constexpr uint32_t kKvpWaitLimit = 1u << 20;
+constexpr uint32_t kKvpWaitLimit = 20000;
 
 // Registers a thread, by warpgroup; at launch all have 96 (640 threads).
 constexpr int kKvpRegsSoft = 144, kKvpRegsConv = 72, kKvpRegsMma = 40;
@@ -160,12 +160,22 @@ __device__ __forceinline__ int kvp_piece(int rows, int row, int ch) {
     return (ch >> 3) * rows * 128 + row * 128 + (((ch & 7) ^ (row & 7)) << 4);
 }
 
-// Wait that gives up when the block has failed or after kKvpWaitLimit polls.
+// Wait that gives up when the block has failed or after about two seconds.  A
+// poll sleeps for up to 100 us, so that waiting warps leave the issue slots and
+// the shared-memory pipe to the others.
 __device__ __forceinline__ bool kvp_wait(uint64_t* bar, uint32_t parity, volatile int* fail) {
     const uint32_t b = smem_addr(bar);
     for (uint32_t i = 0; i < kKvpWaitLimit; i++) {
-        if (mbar_try_wait(b, parity)) return true;
-        if ((i & 255u) == 255u && *fail) return false;
+        uint32_t done;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 100000;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(done)
+            : "r"(b), "r"(parity)
+            : "memory");
+        if (done) return true;
+        if (*fail) return false;
     }
     *fail = 1;
     return false;
@@ -283,40 +293,56 @@ __global__ void __launch_bounds__(kKvpThreads, 1) k_kv_prompt(const KvAttnArgs a
             const long long mine = live_row ? (q.t0 + tok) * a.q_stride + (long long)head * c.hd : -1;
             const float sign = a.scale < 0.0f ? -1.0f : 1.0f;
             const bool in = 4 * lane < c.hd;
-#pragma unroll 1
-            for (int r0 = 0; r0 < 32; r0 += 8) {
-                float4 v[8];
+            // Lanes past the head size bring zeros, which no MMA reads.
+            auto load = [&](int r0, float4 (&v)[4], auto vec) {
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
+                for (int e = 0; e < 4; e++) {
                     const long long from = __shfl_sync(0xffffffffu, mine, r0 + e);
-                    v[e] = from >= 0 && in ? load4((const T*)a.q + from + 4 * lane, a.vec_q) : make_float4(0, 0, 0, 0);
+                    v[e] = from >= 0 && in ? load4((const T*)a.q + from + 4 * lane, vec.value) : make_float4(0, 0, 0, 0);
                 }
+            };
+            unsigned char* to0 = qs + tile * TERMS * kKvpQ + kvp_piece(128, 32 * (warp & 3), lane >> 1) + 8 * (lane & 1);
+            auto put = [&](int r0, const float4 (&v)[4]) {
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
+                for (int e = 0; e < 4; e++) {
                     const uint32_t top = __reduce_max_sync(0xffffffffu, kv_top4(0, v[e]));
                     const bool off = top >= 0x7F800000u;
                     float up = 1.0f;   // the largest to 2^14..2^15, as far as a factor of 2^126 goes
                     if (!std::is_same<T, __half>::value && top != 0 && !off)
                         up = __uint_as_float((uint32_t)(127 + min(14 + 127 - (int)(top >> 23), 126)) << 23);
-                    const float f = off ? 0.0f : up * sign;
-                    if (off) v[e] = make_float4(0, 0, 0, 0);
-                    const float x0 = v[e].x * f, x1 = v[e].y * f, x2 = v[e].z * f, x3 = v[e].w * f;
+                    const float f = up * sign;
+                    const float x0 = off ? 0.0f : v[e].x * f, x1 = off ? 0.0f : v[e].y * f, x2 = off ? 0.0f : v[e].z * f,
+                                x3 = off ? 0.0f : v[e].w * f;
                     const uint2 hi = make_uint2(half2_bits(x0, x1), half2_bits(x2, x3));
-                    unsigned char* to = qs + tile * TERMS * kKvpQ + kvp_piece(128, 32 * (warp & 3) + r0 + e, lane >> 1) + 8 * (lane & 1);
-                    if (in) *reinterpret_cast<uint2*>(to) = hi;
+                    // row r's pieces are swizzled with r & 7, which to0 has for row 0
+                    const int row = r0 + e;
+                    unsigned char* to = reinterpret_cast<unsigned char*>(reinterpret_cast<uintptr_t>(to0) ^ ((row & 7) << 4)) + row * 128;
+                    *reinterpret_cast<uint2*>(to) = hi;
                     if (TERMS == 2) {
                         const float2 a0 = __half22float2(*reinterpret_cast<const __half2*>(&hi.x)),
                                      a1 = __half22float2(*reinterpret_cast<const __half2*>(&hi.y));
-                        if (in)
-                            *reinterpret_cast<uint2*>(to + kKvpQ) =
-                                make_uint2(half2_bits(x0 - a0.x, x1 - a0.y), half2_bits(x2 - a1.x, x3 - a1.y));
+                        *reinterpret_cast<uint2*>(to + kKvpQ) =
+                            make_uint2(half2_bits(x0 - a0.x, x1 - a0.y), half2_bits(x2 - a1.x, x3 - a1.y));
                     }
-                    if (lane == r0 + e) {
+                    if (lane == row) {
                         rs = off ? 1.0f : fabsf(a.scale) / up;
                         bad = off;
                     }
                 }
-            }
+            };
+            auto bring = [&](auto vec) {
+                float4 va[4], vb[4];
+                load(0, va, vec);
+#pragma unroll 1
+                for (int r0 = 0; r0 < 32; r0 += 8) {
+                    load(r0 + 4, vb, vec);
+                    put(r0, va);
+                    load(min(r0 + 8, 28), va, vec);
+                    put(r0 + 4, vb);
+                }
+            };
+            if (a.vec_q) bring(std::true_type{});
+            else bring(std::false_type{});
         }
         fence_smem_async();
         __syncwarp();
@@ -643,7 +669,7 @@ __global__ void __launch_bounds__(kKvpThreads, 1) k_kv_prompt(const KvAttnArgs a
     tc_fence_before();
     __syncthreads();
     if (warp == 16) {
-        mbar_wait(smem_addr(&done_bar), 0, kKvpWaitLimit);   // every MMA issued is complete
+        mbar_wait(smem_addr(&done_bar), 0, 1u << 20);   // every MMA issued is complete
         __syncwarp();
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
