@@ -4,6 +4,8 @@
 
 #include <stddef.h>
 
+#include <type_traits>
+
 #include "kv8.cuh"
 
 namespace aion {
@@ -368,17 +370,24 @@ __global__ void __launch_bounds__(kKvaThreads, KvaShape<HDP, D, WIDE>::kBlocks) 
         float4 v[KS][2];
         float top = 0.0f;
         bool bad = false;
+        const T* src = (const T*)a.q + row.q;
+        const int end = row.lim >= 0 ? c.hd : 0;
+        auto load = [&](auto vec) {
 #pragma unroll
-        for (int k = 0; k < KS; k++)
+            for (int k = 0; k < KS; k++)
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const int d0 = 32 * k + 16 * i + 4 * t;
-                v[k][i] = row.lim >= 0 && d0 < c.hd ? load4((const T*)a.q + row.q + d0, a.vec_q) : make_float4(0, 0, 0, 0);
-                const float b = fmaxf(fmaxf(fabsf(v[k][i].x), fabsf(v[k][i].y)), fmaxf(fabsf(v[k][i].z), fabsf(v[k][i].w)));
-                const float sum = (v[k][i].x + v[k][i].y) + (v[k][i].z + v[k][i].w);
-                bad = bad || !(b <= 3.402823466e38f) || sum != sum;   // max leaves a NaN out, a sum does not
-                top = fmaxf(top, b);
-            }
+                for (int i = 0; i < 2; i++) {
+                    const int d0 = 32 * k + 16 * i + 4 * t;
+                    v[k][i] = d0 < end ? load4(src + d0, vec.value) : make_float4(0, 0, 0, 0);
+                }
+        };
+        if (a.vec_q) load(std::true_type{});
+        else load(std::false_type{});
+        uint32_t high = 0;
+#pragma unroll
+        for (int k = 0; k < KS; k++) high = kv_top4(kv_top4(high, v[k][0]), v[k][1]);
+        bad = high >= 0x7F800000u;
+        top = __uint_as_float(high);
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
         bad = (__ballot_sync(0xffffffffu, bad) >> (4 * g)) & 15;

@@ -458,18 +458,18 @@ __global__ void __launch_bounds__(kKvpThreads, 1) k_kv_prompt(const KvAttnArgs a
         if (ok && (tile < nq)) {
             const float f = l == 0.0f ? 0.0f : vref * 0.0078125f / l;
             T* dst = (T*)a.out + (q.t0 + tok) * a.out_stride + (long long)head * c.hd;
-            for (int b = 0; b < c.hd; b += 16) {
-                float x[16];
-                if (mine > 0) {
-                    tmem_ld16(to + b, x);
-                } else {
+            auto put = [&](auto vec) {
+#pragma unroll 1
+                for (int b = 0; b < c.hd; b += 16) {
+                    float x[16];
+                    if (mine > 0) tmem_ld16(to + b, x);
 #pragma unroll
-                    for (int e = 0; e < 16; e++) x[e] = 0.0f;
+                    for (int e = 0; e < 16; e++) x[e] = l == 0.0f || mine == 0 ? 0.0f : x[e] * f;
+                    if (live_row) store16(dst + b, vec.value, x);
                 }
-#pragma unroll
-                for (int e = 0; e < 16; e++) x[e] = l == 0.0f ? 0.0f : x[e] * f;
-                if (live_row) store16(dst + b, a.vec_out, x);
-            }
+            };
+            if (a.vec_out) put(std::true_type{});
+            else put(std::false_type{});
         }
         tc_fence_before();
     } else if (warp < 16) {
