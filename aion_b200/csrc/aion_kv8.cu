@@ -429,8 +429,8 @@ static cudaError_t launch_prompt(const KvAttnArgs& a, int dev, cudaStream_t st) 
         if (e != cudaSuccess) return e;
         opted.fetch_or(bit);
     }
-    const int64_t places = (int64_t)a.r.n_tok * a.group / 256 + a.r.n_seq;
-    k_kv_prompt<T><<<dim3((unsigned)places, a.c.nkv), kKvpThreads, kKvpSmem, st>>>(a);
+    const int64_t blocks = ((int64_t)a.r.n_tok * a.group / 256 + a.r.n_seq) * a.c.nkv;
+    k_kv_prompt<T><<<(unsigned)blocks, kKvpThreads, kKvpSmem, st>>>(a);
     return cudaGetLastError();
 }
 
@@ -442,7 +442,8 @@ extern "C" AION_API aion_status aion_kv8_attention(const aion_kv8* kv, int32_t l
     const char* what = "aion_kv8_attention";
     aion_status s = check_rows(kv, layer, type, seqs, pos0, cu, n_seq, n_tok, what);
     if (s != AION_OK) return s;
-    if (n_heads < 1 || n_heads % kv->n_kv_heads || (int64_t)n_tok * (n_heads / kv->n_kv_heads) > (1 << 30)) {
+    if (n_heads < 1 || n_heads % kv->n_kv_heads || (int64_t)n_tok * (n_heads / kv->n_kv_heads) > (1 << 30) ||
+        ((int64_t)n_tok * n_heads / 256 + (int64_t)(n_seq + 1) * kv->n_kv_heads) >> 31) {
         aion_thread_error("%s: %d query heads for %d K/V heads, %d rows", what, n_heads, kv->n_kv_heads, n_tok);
         return AION_ERR_SHAPE;
     }

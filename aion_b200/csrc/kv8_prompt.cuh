@@ -208,7 +208,7 @@ __global__ void __launch_bounds__(kKvpThreads, 1) k_kv_prompt(const KvAttnArgs a
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     // ---- the block's rows
-    const int h = blockIdx.y, place = gridDim.x - 1 - blockIdx.x;   // late rows, which see most, first
+    const int h = blockIdx.x % c.nkv, place = (gridDim.x - 1 - blockIdx.x) / c.nkv;   // late rows, which see most, first, in all heads
     int blk = 0, s = 0;
     {
         // places of a sequence: (rows before it / ROWS) + its number, on
