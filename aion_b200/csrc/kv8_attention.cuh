@@ -342,11 +342,10 @@ __global__ void __launch_bounds__(kKvaThreads, KvaShape<HDP, D, WIDE>::kBlocks) 
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             const long long from = __shfl_sync(0xffffffffu, at, j);
-            if (from < 0) continue;
             const int8_t* src = pool + from + 16 * lane;
 #pragma unroll
             for (int e = 0; e < NE; e++)
-                if (lane + 32 * e < c.hd)
+                if (from >= 0 && lane + 32 * e < c.hd)
                     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + j * 16 * HDP + dst[e]),
                                  "l"(src + 512 * e)
                                  : "memory");
@@ -530,7 +529,6 @@ __global__ void __launch_bounds__(kKvaThreads, KvaShape<HDP, D, WIDE>::kBlocks) 
                     for (int d = 0; d < ND; d++) acc[d][0] = acc[d][1] = acc[d][2] = acc[d][3] = 0;
 #pragma unroll
                     for (int k = 0; k < KS; k++) {
-                        if (32 * k >= c.hd) break;
                         uint32_t f[4];
                         ldsm_rows(f, ks + 16 * j * HDP + place(lane & 15, 2 * k + (lane >> 4)));
 #pragma unroll
@@ -608,7 +606,6 @@ __global__ void __launch_bounds__(kKvaThreads, KvaShape<HDP, D, WIDE>::kBlocks) 
                 const uint32_t v8 = smem_addr(ring + vslot * SH::kSlot);
 #pragma unroll
                 for (int mt = 0; mt < MT; mt++) {
-                    if (16 * mt >= c.hd) break;
                     int acc[ND][4];
 #pragma unroll
                     for (int d = 0; d < ND; d++) acc[d][0] = acc[d][1] = acc[d][2] = acc[d][3] = 0;
