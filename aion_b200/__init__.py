@@ -538,8 +538,8 @@ class KV8Cache:
         self._dev, self._int = k.device.index, torch.int32
         self._empty_like, self._new, self._lib = torch.empty_like, torch.empty, lib()
         self._raw_stream = torch._C._cuda_getCurrentRawStream
-        self._ws = {}   # bytes of workspace by (heads, sequences, rows)
-        if self._lib.aion_kv8_attention_workspace(self._p, n_kv, 1, 1) < 0:
+        self._ws = self._lib.aion_kv8_attention_workspace(self._p, n_kv, 1, 1)   # bytes that serve any call
+        if self._ws < 0:
             _check(3)
 
     # -- arguments: calls take a few microseconds, so these checks are terse --
@@ -630,14 +630,7 @@ class KV8Cache:
             scale = 0.0
         elif scale == 0.0:
             raise ValueError("a scale of 0 stands for the default: pass None")
-        key = (n_heads, n, n_tok)
-        ws = self._ws.get(key)
-        if ws is None:
-            if len(self._ws) > 4096:   # ragged serving meets many shapes
-                self._ws.clear()
-            ws = self._ws[key] = self._lib.aion_kv8_attention_workspace(self._p, *key)
-            if ws < 0:
-                _check(3)
+        ws = self._ws
         buf = self._empty((ws,), self.k.dtype, stream) if ws else None
         st = self._lib.aion_kv8_attention(self._p, layer, qp, op, self._types[q.dtype], n_heads, qs, os_, scale, sp, pp, cp,
                                       n, n_tok, buf.data_ptr() if ws else None, ws, self._stream(stream))

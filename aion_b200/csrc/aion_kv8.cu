@@ -373,14 +373,30 @@ extern "C" AION_API aion_status aion_kv8_read(const aion_kv8* kv, int32_t layer,
 // ---------------------------------------------------------------------------
 // Attention
 // ---------------------------------------------------------------------------
-// Rows of a K/V head (tokens x query heads) from which a sequence, on average,
-// goes to the tiles of 128 rows.
-constexpr int kTileRows = 32;
-static bool attention_tiles(int n_seq, int n_tok, int group) { return (int64_t)n_tok * group >= (int64_t)kTileRows * n_seq; }
+// Which kernel.  k_kv_attention streams a sequence's keys once for each 8 rows
+// of a K/V head (rows: tokens x query heads), spread over the whole card;
+// k_kv_prompt once for each 256 rows, from one SM.  Per 64 keys the first takes
+// the SM about 0.4 us a unit of 8 rows, the second 1.3 to 2.2 us a block of
+// 256, whatever there is in it, so the tiles win from about 4 units an SM and
+// wave of blocks on.  Measured, us of tiles / of streams, hd 128, page 64:
+//   fp32, 32 K/V heads, 4 x 4096 keys   16 rows 131 / 71, 32: 131 / 113, 64: 132 / 196
+//   bf16, 8 K/V heads, 16 x 4096 keys   16 rows 104 / 69, 32: 105 / 110, 64: 104 / 187
+//   bf16, 8 K/V heads, 1 x 32768 keys   256 rows 733 / 318, 512: 768 / 605, 1024: 770 / 1170
+// and within 4% of the better one from 4096 keys on over 90 such shapes (20% at 512 keys).
+constexpr int kTileUnits = 4;
+static bool attention_tiles(const aion_kv8* kv, int n_seq, int n_tok, int group) {
+    const int64_t rows = ((int64_t)n_tok * group + n_seq - 1) / n_seq, lines = (int64_t)n_seq * kv->n_kv_heads;
+    const int64_t sms = sm_count(kv->device), waves = (lines * ((rows + 255) / 256) + sms - 1) / sms;
+    return lines * ((rows + 7) / 8) >= kTileUnits * sms * waves;
+}
 
-// Units of at most this many groups of 64 keys go to one block whole: no join
-// launch.
-constexpr int kWholeGroups = 8;
+// Where a sequence holds at most this many groups of 64 keys, its units go to
+// one block whole: no join launch.  us, cut / whole, fp32 steps of full
+// sequences: 32 x 32 heads of 128 and 512 keys 48.1 / 43.4, 1024 keys 73.7 /
+// 70.5; 6 heads of 48 and 512 keys 15.9 / 13.8, 1024 keys 17.5 / 16.1, 2048
+// keys 19.5 / 20.4; 1 x 8 heads of 128 (groups of 4) 1024 keys 19.9 / 18.7,
+// 2048 keys 21.5 / 24.6.
+constexpr int kWholeGroups = 16;
 static bool attention_whole(const aion_kv8* kv) {
     return (int64_t)kv->max_pages * kv->page_tokens <= kWholeGroups * kKvaT;
 }
@@ -389,7 +405,6 @@ extern "C" AION_API int64_t aion_kv8_attention_workspace(const aion_kv8* kv, int
                                                          int32_t n_tok) {
     if (check_shape(kv, "aion_kv8_attention_workspace") != AION_OK) return -1;
     if (n_heads < 1 || n_heads % kv->n_kv_heads || n_seq < 0 || n_tok < 0) return -1;
-    if (attention_tiles(n_seq, n_tok, n_heads / kv->n_kv_heads)) return 0;
     return attention_whole(kv) ? 0 : (int64_t)sm_count(kv->device) * 2 * 2 * sizeof(KvPart);   // two blocks an SM at most
 }
 
@@ -414,7 +429,11 @@ static cudaError_t launch_attention(KvAttnArgs a, int dev, cudaStream_t st) {
 }
 template <typename T, int D>
 static cudaError_t launch_attention_of(const KvAttnArgs& a, int rows, int dev, cudaStream_t st) {
-    const bool wide = rows > (D == 2 ? 4 : 2);
+    // Units of 8 rows, or of 4 (16-bit rows) or 2 (fp32), whose turns are shorter but which read the keys anew.
+    // us, wide / narrow, 8 K/V heads, 1 x 32768 keys and 16 x 2048: bf16 4 rows 38.6 / 36.3 and 35.8 / 32.0, 8 rows
+    // 44.0 / 39.9 and 38.8 / 39.9, 12 rows 47.0 / 48.1 and 46.1 / 44.0, 16 rows 47.9 / 50.2 and 47.7 / 53.0; fp32
+    // 2 rows 39.8 / 35.9 and 35.5 / 31.9, 3 rows 39.9 / 39.9 and 35.8 / 39.1, 8 rows 45.9 / 50.5 and 39.4 / 52.4.
+    const bool wide = rows > (D == 2 ? 8 : 2);
     if (a.c.hd > 64) return wide ? launch_attention<T, 128, D, true>(a, dev, st) : launch_attention<T, 128, D, false>(a, dev, st);
     return wide ? launch_attention<T, 64, D, true>(a, dev, st) : launch_attention<T, 64, D, false>(a, dev, st);
 }
@@ -457,7 +476,8 @@ extern "C" AION_API aion_status aion_kv8_attention(const aion_kv8* kv, int32_t l
     const char *q0 = (const char*)q, *q1 = q0 + (last * q_stride + width) * el;
     const char *o0 = (const char*)out, *o1 = o0 + (last * out_stride + width) * el;
     KV_ARG(q1 <= o0 || o1 <= q0, "%s: q and out overlap", what);
-    const int64_t need = aion_kv8_attention_workspace(kv, n_heads, n_seq, n_tok);
+    const bool tiles = attention_tiles(kv, n_seq, n_tok, n_heads / kv->n_kv_heads);
+    const int64_t need = tiles ? 0 : aion_kv8_attention_workspace(kv, n_heads, n_seq, n_tok);
     KV_ARG(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0),
            "%s: needs %lld bytes of 16-byte aligned workspace, got %lld", what, (long long)need,
            (long long)(workspace ? workspace_bytes : 0));
@@ -480,7 +500,7 @@ extern "C" AION_API aion_status aion_kv8_attention(const aion_kv8* kv, int32_t l
     a.parts = (KvPart*)workspace;
     a.unit_log = 0;
     const cudaStream_t st = (cudaStream_t)stream;
-    if (attention_tiles(n_seq, n_tok, a.group)) {
+    if (tiles) {
         if (type == AION_F32) KV_CUDA((launch_prompt<float>(a, kv->device, st)));
         else if (type == AION_F16) KV_CUDA((launch_prompt<__half>(a, kv->device, st)));
         else KV_CUDA((launch_prompt<__nv_bfloat16>(a, kv->device, st)));

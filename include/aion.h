@@ -423,16 +423,21 @@ AION_API aion_status aion_kv8_read(const aion_kv8* kv, int32_t layer, void* k, v
  * rows of `type`, q_stride / out_stride elements apart, and do not overlap.
  * scale 0: 1 / sqrt(head_size).  A sequence with pos0[i] < 0 gets zeros;
  * positions whose page is missing are left out; rows from cu[n_seq] on are
- * left as they were.  Scores, softmax and sums are exact integer dots of
- * fixed-point digits (24 bits for fp32 rows, 16 for 16-bit rows, relative to
- * the largest of a row) joined in fp32; out is rounded once.
+ * left as they were.  The products are exact, the softmax and the sums fp32,
+ * and out is rounded once.  What is rounded before: where a K/V head has few
+ * rows, queries and weights to fixed point (24 bits for fp32 rows, 16 for
+ * 16-bit rows, relative to the largest of a row, or of 64 weights); where it
+ * has many, fp32 queries and weights to 22 bits, weights of 16-bit rows to
+ * fp16.
  * `workspace`: aion_kv8_attention_workspace bytes of device memory, 16-byte
  * aligned, that no other call in flight uses (NULL when that is 0). */
 AION_API aion_status aion_kv8_attention(const aion_kv8* kv, int32_t layer, const void* q, void* out, int32_t type,
                                         int32_t n_heads, int64_t q_stride, int64_t out_stride, float scale,
                                         const int32_t* seqs, const int32_t* pos0, const int32_t* cu, int32_t n_seq,
                                         int32_t n_tok, void* workspace, int64_t workspace_bytes, void* stream);
-/* Workspace bytes of such a call; -1 when the shape is not supported. */
+/* Workspace bytes that serve every such call of a cache, whatever its rows
+ * (a call that has no use for it takes NULL, too); -1 when the shape is not
+ * supported. */
 AION_API int64_t aion_kv8_attention_workspace(const aion_kv8* kv, int32_t n_heads, int32_t n_seq, int32_t n_tok);
 
 /* Waits for `stream`, then reports and clears what the calls enqueued before

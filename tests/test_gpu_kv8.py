@@ -373,6 +373,131 @@ def test_attention_strides_and_out(cuda):
 
 
 # ---------------------------------------------------------------------------
+# Many rows a sequence: tiles of 128 rows.  Calls come here from 592 units of 8
+# rows on (sequences x K/V heads x rows / 8).  Weights of 16-bit rows are fp16:
+# half a step of 2^-11 of each, so 2^-11 of the largest value in all; fp32
+# queries and weights have 22 bits, which the digits' bounds hold.
+# ---------------------------------------------------------------------------
+def check_tiles(p, q, seqs, pos0, counts, name, scale=None, with_cu=True, out=None):
+    lines, rows = len(seqs) * p.r.k.shape[2], -(-sum(counts) * (q.shape[1] // p.r.k.shape[2]) // len(seqs))
+    assert lines * -(-rows // 8) >= 592 and lines * -(-rows // 256) <= 132   # one wave of blocks
+    cu = [0] + np.cumsum(counts).tolist()
+    got = p.c.attention(0, q, p.ints(seqs), p.ints(pos0), p.ints(cu) if with_cu else None, scale, out)
+    want, info = p.r.attention(0, q[:cu[-1]].float().cpu().numpy(), seqs, pos0, cu, scale)
+    got = got.float().cpu().numpy()[:cu[-1]].astype(np.float64)
+    sc = abs(scale) if scale else 1 / np.sqrt(q.shape[2])
+    u2 = 2.0 ** -20 if name == "f32" else 2.0 ** -16
+    qm, ks, vm, seen = (info[..., i] for i in range(4))
+    tol = (2 * (sc * qm * ks * u2 + 2.0 ** -20) + 64 * u2 / 8 + 2.0 ** -22 * (seen / 64 + 4)) * vm
+    tol += (0 if name == "f32" else 2.0 ** -11) * vm
+    tol = tol[..., None] + {"f32": 2.0 ** -24, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}[name] * np.abs(want) + 2.0 ** -24
+    err = np.abs(got - want)
+    assert np.isfinite(got).all()
+    assert (err <= tol).all(), f"worst {float((err / tol).max())} of the tolerance"
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("n_kv,group,hd,page,counts,before", [
+    (16, 1, 64, 16, [90, 1, 130, 77], [0, 40, 7, 100]),
+    (8, 2, 128, 64, [257, 30, 5, 1], [130, 0, 61, 200]),
+    (8, 4, 48, 32, [37, 64, 129, 1], [0, 3, 70, 11]),
+    (4, 8, 96, 128, [133, 2, 90], [100, 0, 1]),
+    (2, 16, 16, 16, [240], [17]),
+    (40, 1, 80, 64, [129, 127], [0, 513]),
+    (3, 7, 112, 32, [0, 300, 0, 210], [0, 1, 5, 64])])
+def test_attention_of_many_rows(cuda, name, n_kv, group, hd, page, counts, before):
+    dt = dtype_of(cuda, name)
+    n = len(counts)
+    p = Pair(cuda, 1, 120, n_kv, hd, n + 1, 64, page, seed=n + hd)
+    p.fill([a + b for a, b in zip(counts, before)], dt)
+    check_tiles(p, p.rows(sum(counts), n_kv * group, dt), list(range(n)), before, counts, name)
+    p.c.status()
+
+
+@pytest.mark.parametrize("name", TYPES)
+def test_attention_of_single_tokens_with_many_heads(cuda, name):
+    dt = dtype_of(cuda, name)
+    p = Pair(cuda, 1, 120, 2, 16, 17, 8, 16, seed=3)
+    lens = [1, 2, 15, 16, 17, 63, 64, 65, 127, 128, 100, 99, 33, 5, 80, 70]
+    p.fill(lens, dt)
+    check_tiles(p, p.rows(16, 320, dt), list(range(16)), [n - 1 for n in lens], [1] * 16, name, with_cu=False)
+    p.c.status()
+
+
+@pytest.mark.parametrize("spread,scale", [(0.0, None), (1e-3, None), (30.0, None), (1e4, None), (1.0, -0.3), (1.0, 3.0)])
+def test_many_rows_of_flat_and_peaked_scores(cuda, spread, scale):
+    p = Pair(cuda, 1, 40, 16, 32, 2, 40, 16, seed=1)
+    p.fill([320], cuda.float32)
+    check_tiles(p, p.rows(320, 16, cuda.float32, spread), [0], [0], [320], "f32", scale)
+
+
+@pytest.mark.parametrize("name,off", [("f32", 33), ("f16", 1), ("bf16", 3)])
+def test_many_rows_with_strides(cuda, name, off):
+    dt = dtype_of(cuda, name)
+    p = Pair(cuda, 1, 40, 16, 32, 2, 40, 16, seed=2)
+    p.fill([330], dt)
+    q = p.rows(320, 20, dt).flatten(1)[:, off:off + 512].unflatten(1, (16, 32))
+    out = cuda.zeros(320, 521, device="cuda", dtype=dt)[:, 1:513].unflatten(1, (16, 32))
+    check_tiles(p, q, [0], [10], [320], name, out=out)
+
+
+def test_many_rows_that_see_nothing_and_what_poisons_them(cuda):
+    import aion_b200 as A
+    p = Pair(cuda, 1, 40, 16, 64, 6, 8, 32, seed=4)
+    p.fill([186, 95, 0, 5], cuda.float32)
+    q = p.rows(320, 16, cuda.float32)
+    q[10, 5, 3] = float("nan")
+    q[11, 6, 3] = float("-inf")
+    clean = p.r.attention(0, q.cpu().numpy(), [0], [46], [0, 140])[0][:140]
+    p.c.v_scale[0, p.c.tables[0, 4].long(), 3] = float("nan")   # slot 0, positions 128..159, head 3
+    p.c.k_scale[0, p.c.tables[0, 5].long(), 2] = float("nan")   # 160.., head 2
+    p.c.tables[1, 1] = -1                                       # slot 1, positions 32..63
+    out = cuda.full((320, 16, 64), 3.0, device="cuda")
+    # slot 0: 140 rows; 80 of a refused sequence; slot 3: none; slot 1: 90; 10 behind the last sequence
+    p.c.attention(0, q, p.ints([0, 2, 3, 1]), p.ints([46, -1, 5, 5]), p.ints([0, 140, 220, 220, 310]), out=out)
+    with pytest.raises(A.AionError) as e:
+        p.c.status()
+    assert e.value.code == "STATE"
+    got = out.cpu().numpy()
+    assert (got[140:220] == 0).all() and (got[310:] == 3).all()
+    nan = np.zeros((140, 16), bool)
+    nan[10, 5] = nan[11, 6] = True
+    nan[128 - 46:, 3] = True
+    nan[160 - 46:, 2] = True
+    assert (np.isnan(got[:140]).all(-1) == nan).all() and (np.isnan(got[:140]).any(-1) == nan).all()
+    assert np.abs(got[:140] - clean)[~nan].max() < 1e-4
+    k, v = p.r.rows(0, 1, 95)
+    k, v = (np.delete(x, slice(32, 64), 0) for x in (k, v))
+    for r in (0, 20, 31, 57, 58, 59, 89):
+        seen = r + 6 if r + 6 <= 32 else 32 + max(r + 6 - 64, 0)
+        for h in range(16):
+            x = k[:seen, h] @ q[220 + r, h].cpu().numpy().astype(np.float64) / 8
+            w = np.exp(x - x.max())
+            assert np.abs(got[220 + r, h] - w @ v[:seen, h] / w.sum()).max() < 1e-4
+
+
+def test_many_rows_captured_and_replayed(cuda):
+    p = Pair(cuda, 1, 40, 16, 64, 3, 20, 32, seed=5)
+    p.fill([400, 300], cuda.bfloat16)
+    q = p.rows(300, 16, cuda.bfloat16)
+    seqs, pos0, cu = p.ints([0, 1]), p.ints([0, 0]), p.ints([0, 150, 300])
+    side = cuda.cuda.Stream()
+    side.wait_stream(cuda.cuda.current_stream())
+    graph = cuda.cuda.CUDAGraph()
+    with cuda.cuda.graph(graph, stream=side):
+        out = p.c.attention(0, q, seqs, pos0, cu)
+    for at, rows in (([0, 0], 150), ([200, 100], 200), ([100, -1], 100)):
+        pos0.copy_(p.ints(at))
+        cu.copy_(p.ints([0, rows, 300]))
+        out.fill_(5)
+        graph.replay()
+        first = out.clone()
+        graph.replay()
+        eager = p.c.attention(0, q, seqs, pos0, cu)
+        assert cuda.equal(first, out) and cuda.equal(eager, out)
+
+
+# ---------------------------------------------------------------------------
 # Entries that are refused on the device
 # ---------------------------------------------------------------------------
 def test_bad_entries_are_skipped_and_reported(cuda):

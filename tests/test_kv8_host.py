@@ -163,3 +163,14 @@ def test_empty_calls_do_nothing(built):
     assert L.aion_kv8_grow(p, None, None, 0, None, None) == 0
     assert L.aion_kv8_fork(p, None, None, None, 0, None) == 0
     assert L.aion_kv8_trim(p, None, None, 0, None) == 0
+
+
+def test_one_workspace_serves_every_call(built):
+    """Its size depends on the cache alone, and is 0 where a sequence holds no more than 1024 tokens."""
+    import aion_b200 as A
+    kv = view(page_tokens=64, max_pages=17)
+    sizes = {A.lib().aion_kv8_attention_workspace(ctypes.addressof(kv), heads, n, rows)
+             for heads in (4, 64) for n, rows in ((1, 1), (3, 3), (2, 900), (1, 1 << 20), (0, 0))}
+    assert len(sizes) == 1 and sizes.pop() > 0
+    kv = view(page_tokens=64, max_pages=16)
+    assert A.lib().aion_kv8_attention_workspace(ctypes.addressof(kv), 4, 2, 2) == 0
