@@ -232,6 +232,13 @@ __global__ void __launch_bounds__(kKvpThreads, 1) k_kv_prompt(const KvAttnArgs a
     }
     const int ntiles = nt[nq - 1];
 
+    if (warp < 8) {   // the query rows to L2 while the block is set up
+        const int i = row0 + 32 * warp + lane, tok = i / a.group;
+        if (i < row0 + rows) {
+            const T* src = (const T*)a.q + (q.t0 + tok) * a.q_stride + (long long)(h * a.group + i - tok * a.group) * c.hd;
+            for (int d = 0; d < c.hd; d += 128 / (int)sizeof(T)) asm volatile("prefetch.global.L2 [%0];" ::"l"(src + d));
+        }
+    }
     if (threadIdx.x == 0) {
         kv_vet_seq(a, q);
         mbar_init(smem_addr(&q_full), 4 * NQ);
@@ -458,18 +465,50 @@ __global__ void __launch_bounds__(kKvpThreads, 1) k_kv_prompt(const KvAttnArgs a
         if (ok && (tile < nq)) {
             const float f = l == 0.0f ? 0.0f : vref * 0.0078125f / l;
             T* dst = (T*)a.out + (q.t0 + tok) * a.out_stride + (long long)head * c.hd;
-            auto put = [&](auto vec) {
+            if (a.vec_out) {
+                // Through the place of the tile's queries, which no MMA reads any more, 16 bytes a piece: a store then
+                // covers whole rows (a thread's own row is 16-byte pieces of 32 rows to a store).
+                constexpr int PR = 128 * (int)sizeof(T) / 16, RI = 32 / PR;   // pieces of a row, rows a store
+                constexpr int PV = 16 / (int)sizeof(T);                       // values of a piece
+                unsigned char* st = qs + tile * TERMS * kKvpQ + (warp & 3) * 32 * PR * 16;
+                // without keys no MMA has waited for all four warps' queries
+                if (mine == 0) asm volatile("bar.sync %0, 128;" ::"r"(1 + tile) : "memory");
 #pragma unroll 1
                 for (int b = 0; b < c.hd; b += 16) {
                     float x[16];
                     if (mine > 0) tmem_ld16(to + b, x);
 #pragma unroll
                     for (int e = 0; e < 16; e++) x[e] = l == 0.0f || mine == 0 ? 0.0f : x[e] * f;
-                    if (live_row) store16(dst + b, vec.value, x);
+#pragma unroll
+                    for (int e = 0; e < 16 / PV; e++) {
+                        T y[PV];
+#pragma unroll
+                        for (int i = 0; i < PV; i++) y[i] = from_f32<T>(x[PV * e + i]);
+                        *reinterpret_cast<uint4*>(st + lane * PR * 16 + (((b / PV + e) ^ (lane & (PR - 1))) << 4)) =
+                            *reinterpret_cast<const uint4*>(y);
+                    }
                 }
-            };
-            if (a.vec_out) put(std::true_type{});
-            else put(std::false_type{});
+                __syncwarp();
+                const long long at = live_row ? dst - (T*)a.out : -1;
+                const int piece = lane & (PR - 1);
+                const bool in = piece * PV < c.hd;
+#pragma unroll 4
+                for (int r0 = 0; r0 < 32; r0 += RI) {
+                    const int row = r0 + lane / PR;
+                    const long long to_row = __shfl_sync(0xffffffffu, at, row);
+                    const uint4 y = *reinterpret_cast<const uint4*>(st + row * PR * 16 + ((piece ^ (row & (PR - 1))) << 4));
+                    if (to_row >= 0 && in) *reinterpret_cast<uint4*>((T*)a.out + to_row + piece * PV) = y;
+                }
+            } else {
+#pragma unroll 1
+                for (int b = 0; b < c.hd; b += 16) {
+                    float x[16];
+                    if (mine > 0) tmem_ld16(to + b, x);
+#pragma unroll
+                    for (int e = 0; e < 16; e++) x[e] = l == 0.0f || mine == 0 ? 0.0f : x[e] * f;
+                    if (live_row) store16(dst + b, false, x);
+                }
+            }
         }
         tc_fence_before();
     } else if (warp < 16) {
