@@ -22,6 +22,7 @@
 #include <mutex>
 #include <string>
 #include <thread>
+#include <new>
 #include <vector>
 
 #include <cudaTypedefs.h>
@@ -1469,9 +1470,8 @@ static void extend_undo(aion_ctx* c, const aion_kv8* kv, const int32_t* seqs, co
     aion_kv8_status(kv, c->stream);   // the refusal is this call's to report
 }
 
-extern "C" AION_API aion_status aion_extend(aion_ctx* c, const aion_kv8* kv, const int32_t* seqs, const int32_t* n_new,
-                                            const int32_t* tokens, int32_t n_seq, float* logits_host) {
-    if (!c || !kv || !seqs || !n_new || !tokens || n_seq < 1) return AION_ERR_ARG;
+static aion_status extend(aion_ctx* c, const aion_kv8* kv, const int32_t* seqs, const int32_t* n_new,
+                          const int32_t* tokens, int32_t n_seq, float* logits_host) {
     if (c->tp_n > 1 || c->mode == MODE_F32) {
         set_err(&c->err, "aion_extend needs an int4 file on one GPU");
         return AION_ERR_STATE;
@@ -1485,9 +1485,15 @@ extern "C" AION_API aion_status aion_extend(aion_ctx* c, const aion_kv8* kv, con
         set_err(&c->err, "aion_extend: %d sequences (at most 1024)", n_seq);
         return AION_ERR_ARG;
     }
+    auto kv_fail = [&](aion_status s) {
+        c->err = g_thread_err;
+        return s;
+    };
+    const int64_t ws = aion_kv8_attention_workspace(kv, (int32_t)c->nh, n_seq, n_seq);
+    if (ws < 0) return kv_fail(AION_ERR_SHAPE);
     long long mrows = 0;
     std::vector<int32_t> cu(1, 0);
-    std::vector<char> seen((size_t)std::max(kv->max_seqs, 0));
+    std::vector<char> seen((size_t)kv->max_seqs);
     for (int i = 0; i < n_seq; i++) {
         if (seqs[i] < 0 || seqs[i] >= kv->max_seqs || seen[seqs[i]] || n_new[i] < 1) {
             set_err(&c->err, "aion_extend: sequence %d (slot %d, %d tokens) is out of range or names a slot twice", i, seqs[i],
@@ -1510,15 +1516,12 @@ extern "C" AION_API aion_status aion_extend(aion_ctx* c, const aion_kv8* kv, con
     CK_RET(&c->err, cudaSetDevice(c->dev));
     const long long dim = c->dim, hid = c->hidden, kvd = c->kv_dim, mpad = round_up(mrows, kGemmBM);
     const long long kpd = round_up(dim, kGemmBK), kph = round_up(hid, kGemmBK), mcls = round_up(n_seq, kGemmBM);
-    aion_status st = pf_reserve(c, mrows, n_seq);
+    // What earlier calls have left to report is reported before anything grows.
+    aion_status st = aion_kv8_status(kv, c->stream);
+    if (st != AION_OK) return kv_fail(st);
+    st = pf_reserve(c, mrows, n_seq);
     if (st != AION_OK) return st;
     auto& pf = c->pf;
-    const int64_t ws = aion_kv8_attention_workspace(kv, (int32_t)c->nh, n_seq, (int32_t)mrows);
-    auto kv_fail = [&](aion_status s) {
-        c->err = g_thread_err;
-        return s;
-    };
-    if (ws < 0) return kv_fail(AION_ERR_SHAPE);
     CK_RET(&c->err, pf_grow(&pf.ws, &pf.ws_cap, (size_t)std::max<int64_t>(ws, 16)));
     CK_RET(&c->err, pf_grow((void**)&pf.seq, &pf.seq_cap, (size_t)(4 * n_seq + 1 + mrows) * 4));
     int32_t *d_seqs = pf.seq, *d_new = d_seqs + n_seq, *d_pos0 = d_new + n_seq, *d_cu = d_pos0 + n_seq, *d_pos = d_cu + n_seq + 1;
@@ -1591,6 +1594,17 @@ extern "C" AION_API aion_status aion_extend(aion_ctx* c, const aion_kv8* kv, con
     st = aion_kv8_status(kv, sm);
     if (st != AION_OK) return kv_fail(st);
     return check_device_error(c);
+}
+
+extern "C" AION_API aion_status aion_extend(aion_ctx* c, const aion_kv8* kv, const int32_t* seqs, const int32_t* n_new,
+                                            const int32_t* tokens, int32_t n_seq, float* logits_host) {
+    if (!c || !kv || !seqs || !n_new || !tokens || n_seq < 1) return AION_ERR_ARG;
+    try {
+        return extend(c, kv, seqs, n_new, tokens, n_seq, logits_host);
+    } catch (const std::bad_alloc&) {
+        set_err(&c->err, "aion_extend: no host memory for its lists");
+        return AION_ERR_OOM;
+    }
 }
 
 // ---------------------------------------------------------------------------

@@ -41,6 +41,13 @@ namespace aion {
 // l is kept in fp32 from the unrounded weights.  m is a running reference: it
 // follows the row's maximum only when that has grown by more than 8 (a factor
 // of 2^8, and P stays below 2^15), which leaves O untouched for most tiles.
+//
+// A block of 256 rows takes 5K clocks to set up, 13K to bring fp32 queries in,
+// 2.6K (16-bit rows) or 3.3K (fp32) a key tile and 7K to write; the MMAs alone
+// would take 1.3K and 2.6K a tile.  2 x 1999..2048 bf16 rows of 32 heads on 8
+// behind 4096..6143 tokens: 600 us, 0.41 TFLOP, 680 TFLOP/s, bound by the
+// softmax and the 3.5 blocks an SM.  8 x 512 fp32 rows of 32 heads: 110 us,
+// bound by what surrounds 2 to 8 key tiles of a block.
 // ---------------------------------------------------------------------------
 constexpr int kKvpThreads = 640, kKvpTile = 64;
 constexpr int kKvpQ = 128 * 128 * 2;        // a query operand: 128 rows of two 128-byte-wide halves
@@ -60,22 +67,12 @@ __device__ __forceinline__ uint32_t kvp_idesc(int n) {   // fp16 A and B (K-majo
 }
 // Loads and their wait are one instruction to the compiler: a register that a
 // load is still on its way to cannot be moved or spilled.
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
-        "tcgen05.wait::ld.sync.aligned;"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]),
-          "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]),
-          "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr)
-        : "memory");
-}
 __device__ __forceinline__ void tmem_ld64(uint32_t taddr, uint32_t (&x)[2][32]) {
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%64];\n\t"
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%65];\n\t"
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%64];\n\t"
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
+        "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%65];\n\t"
         "tcgen05.wait::ld.sync.aligned;"
         : "=r"(x[0][0]), "=r"(x[0][1]), "=r"(x[0][2]), "=r"(x[0][3]), "=r"(x[0][4]), "=r"(x[0][5]), "=r"(x[0][6]),
           "=r"(x[0][7]), "=r"(x[0][8]), "=r"(x[0][9]), "=r"(x[0][10]), "=r"(x[0][11]), "=r"(x[0][12]),
@@ -89,16 +86,6 @@ __device__ __forceinline__ void tmem_ld64(uint32_t taddr, uint32_t (&x)[2][32]) 
           "=r"(x[1][23]), "=r"(x[1][24]), "=r"(x[1][25]), "=r"(x[1][26]), "=r"(x[1][27]), "=r"(x[1][28]),
           "=r"(x[1][29]), "=r"(x[1][30]), "=r"(x[1][31])
         : "r"(taddr), "r"(taddr + 32)
-        : "memory");
-}
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
-        "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"r"(r[0]),
-        "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
-        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
-        "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
-        "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
         : "memory");
 }
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
