@@ -7,6 +7,8 @@
 #include <cuda_fp16.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace aion {
@@ -403,6 +405,33 @@ __device__ __forceinline__ void store4(T* p, bool vec, float4 x) {
     }
 }
 
+// Two fp32 values in one 64-bit register, for the packed fp32 instructions.
+__device__ __forceinline__ uint64_t f2_pack(float x, float y) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ float2 f2_unpack(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
 // The integer nearest to the exact x / s (ties to even), within +-127; s > 0.
 // The rounded quotient can only be off next to a border between two integers;
 // x - q s is exact there (a multiple of the smaller ulp, below 2^24 of them),
@@ -425,14 +454,16 @@ __device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d) {
 // those and tiny scales take the exact way.
 __device__ __forceinline__ uint32_t kv_quant4(float4 x, float s, float inv) {
     constexpr float kMagic = 12582912.0f;   // 1.5 2^23: the sum's low byte is the integer's
-    const float m0 = fmaf(x.x, inv, kMagic), m1 = fmaf(x.y, inv, kMagic), m2 = fmaf(x.z, inv, kMagic),
-                m3 = fmaf(x.w, inv, kMagic);
+    const uint64_t x01 = f2_pack(x.x, x.y), x23 = f2_pack(x.z, x.w), i2 = f2_pack(inv, inv), s2 = f2_pack(-s, -s);
+    const uint64_t up = f2_pack(kMagic, kMagic), down = f2_pack(-kMagic, -kMagic);
+    const uint64_t m01 = f2_fma(x01, i2, up), m23 = f2_fma(x23, i2, up);
+    const float2 r01 = f2_unpack(f2_fma(f2_add(m01, down), s2, x01)), r23 = f2_unpack(f2_fma(f2_add(m23, down), s2, x23));
     const float h = 0.5f * s;
-    const bool close = fabsf(fmaf(m0 - kMagic, -s, x.x)) >= h || fabsf(fmaf(m1 - kMagic, -s, x.y)) >= h ||
-                       fabsf(fmaf(m2 - kMagic, -s, x.z)) >= h || fabsf(fmaf(m3 - kMagic, -s, x.w)) >= h;
+    const bool close = fabsf(r01.x) >= h || fabsf(r01.y) >= h || fabsf(r23.x) >= h || fabsf(r23.y) >= h;
+    const float2 a = f2_unpack(m01), b = f2_unpack(m23);
     if (close || s < 1e-30f) return pack4(kv_quant(x.x, s), kv_quant(x.y, s), kv_quant(x.z, s), kv_quant(x.w, s));
-    return __byte_perm(__byte_perm(__float_as_uint(m0), __float_as_uint(m1), 0x0040),
-                       __byte_perm(__float_as_uint(m2), __float_as_uint(m3), 0x0040), 0x5410);
+    return __byte_perm(__byte_perm(__float_as_uint(a.x), __float_as_uint(a.y), 0x0040),
+                       __byte_perm(__float_as_uint(b.x), __float_as_uint(b.y), 0x0040), 0x5410);
 }
 // Largest magnitude so far, as bits: a NaN or an infinity stays the largest.
 __device__ __forceinline__ uint32_t kv_top4(uint32_t top, float4 x) {
@@ -497,18 +528,24 @@ __global__ void __launch_bounds__(kKvAppendThreads) k_kv_append(KvAppendArgs a) 
     const int rows = (int)(hi - lo), row0 = (int)(lo & (c.page - 1)), ppr = c.hd / 4, n = rows * ppr;   // pieces of a row
     float4 v[PIECES];
     uint32_t top = 0;
-    const int dr = kKvAppendThreads / ppr, dc = kKvAppendThreads - dr * ppr;
-    int row = threadIdx.x / ppr, col = threadIdx.x - row * ppr;
+    const int dr = kKvAppendThreads / ppr, dc = kKvAppendThreads - dr * ppr, first = threadIdx.x / ppr;
+    auto load = [&](auto vec) {
+        int col = threadIdx.x - first * ppr;
+        const T* p = x + first * stride + 4 * col;
+        const long long step = dr * stride + 4 * dc, wrap = stride - c.hd;
 #pragma unroll
-    for (int e = 0; e < PIECES; e++) {
-        v[e] = (int)threadIdx.x + e * kKvAppendThreads < n ? load4(x + row * stride + 4 * col, a.vec) : make_float4(0, 0, 0, 0);
-        row += dr;
-        col += dc;
-        if (col >= ppr) {
-            col -= ppr;
-            row++;
+        for (int e = 0; e < PIECES; e++) {
+            v[e] = (int)threadIdx.x + e * kKvAppendThreads < n ? load4(p, vec.value) : make_float4(0, 0, 0, 0);
+            p += step;
+            col += dc;
+            if (col >= ppr) {
+                col -= ppr;
+                p += wrap;
+            }
         }
-    }
+    };
+    if (a.vec) load(std::true_type{});
+    else load(std::false_type{});
     bool bad = slot < 0 || slot >= c.max_seqs;
     for (int j = threadIdx.x; j < s; j += kKvAppendThreads) bad = bad || a.r.seqs[j] == slot;
     const int page = slot >= 0 && slot < c.max_seqs && pg < c.max_pages ? c.tables[(size_t)slot * c.max_pages + pg] : -1;

@@ -4,8 +4,6 @@
 
 #include <stddef.h>
 
-#include <type_traits>
-
 #include "kv8.cuh"
 
 namespace aion {
