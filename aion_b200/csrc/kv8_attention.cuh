@@ -722,11 +722,13 @@ __global__ void __launch_bounds__(kKvaThreads, KvaShape<HDP, D, WIDE>::kBlocks) 
 // Units that blocks share.  Block b - 1 takes the border before block b: the
 // unit that lies across it, if this is the first border inside the unit.  The
 // records of the blocks from b - 1 on are read at once, lane i that of b - 1 + i.
-constexpr int kKvJoinThreads = 128;
+constexpr int kKvJoinThreads = 256;   // a warp a row: one trip after the other is what this costs
 template <typename T>
 __global__ void __launch_bounds__(kKvJoinThreads) k_kv_attention_join(const KvAttnArgs a, int blocks) {
+    static_assert(kKvJoinThreads / 32 >= kKvaRows, "a warp for each row");
+    const int b = blockIdx.x + 1, r = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (r >= 1 << a.unit_log) return;
     pdl_wait();
-    const int b = blockIdx.x + 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const KvPart* p0 = a.parts + 2 * (size_t)(b - 1);
     const KvPart* mine = p0 + 2 * (size_t)lane;
     const bool there = b - 1 + lane < blocks;
@@ -742,38 +744,35 @@ __global__ void __launch_bounds__(kKvJoinThreads) k_kv_attention_join(const KvAt
     int end = b - 1 + (other ? __ffs(other) - 1 : 32);
     if (!other)
         while (end < blocks && a.parts[2 * (size_t)end].valid && a.parts[2 * (size_t)end].begin == ubegin) end++;
-    const KvSeq q = kv_seq(a, s);
     const int np = end - (b - 1);
-    for (int r = warp; r < 1 << a.unit_log; r += kKvJoinThreads / 32) {
-        const KvRow row = kv_row(a, q, h, rg, r);
-        if (row.out < 0) break;
-        float mx = -INFINITY, ls = 0.0f;
-        float4 os = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (int base = 0; base < np; base += 32) {   // lane i weighs part base + i
-            const KvPart* p = base + lane == 0 ? head : p0 + 2 * (size_t)(base + lane);
-            const bool in = base + lane < np;
-            const float pm = in ? p->m[r] : -INFINITY, pl = in ? p->l[r] : 0.0f;
-            const float mn = fmaxf(mx, warp_max(pm)), wgt = pm == -INFINITY ? 0.0f : kv_exp2(pm - mn);
-            const float old = mx == -INFINITY ? 0.0f : kv_exp2(mx - mn);
-            mx = mn;
-            ls = ls * old + warp_sum(wgt * pl);
-            os = make_float4(os.x * old, os.y * old, os.z * old, os.w * old);
-            const int n = min(np - base, 32);
+    const KvRow row = kv_row(a, kv_seq(a, s), h, rg, r);
+    float mx = -INFINITY, ls = 0.0f;
+    float4 os = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    // the parts of a row that the unit does not have are not set: it is joined all the same, and not stored
+    for (int base = 0; base < np; base += 32) {   // lane i weighs part base + i
+        const KvPart* p = base + lane == 0 ? head : p0 + 2 * (size_t)(base + lane);
+        const bool in = base + lane < np;
+        const float pm = in ? p->m[r] : -INFINITY, pl = in ? p->l[r] : 0.0f;
+        const float mn = fmaxf(mx, warp_max(pm)), wgt = pm == -INFINITY ? 0.0f : kv_exp2(pm - mn);
+        const float old = mx == -INFINITY ? 0.0f : kv_exp2(mx - mn);
+        mx = mn;
+        ls = ls * old + warp_sum(wgt * pl);
+        os = make_float4(os.x * old, os.y * old, os.z * old, os.w * old);
+        const int n = min(np - base, 32);
 #pragma unroll 8
-            for (int i = 0; i < n; i++) {
-                const KvPart* pi = base + i == 0 ? head : p0 + 2 * (size_t)(base + i);
-                const float w = __shfl_sync(0xffffffffu, wgt, i);
-                const float4 x = *reinterpret_cast<const float4*>(&pi->o[r][4 * lane]);
-                os.x += w * x.x;
-                os.y += w * x.y;
-                os.z += w * x.z;
-                os.w += w * x.w;
-            }
+        for (int i = 0; i < n; i++) {
+            const KvPart* pi = base + i == 0 ? head : p0 + 2 * (size_t)(base + i);
+            const float w = __shfl_sync(0xffffffffu, wgt, i);
+            const float4 x = *reinterpret_cast<const float4*>(&pi->o[r][4 * lane]);
+            os.x += w * x.x;
+            os.y += w * x.y;
+            os.z += w * x.z;
+            os.w += w * x.w;
         }
-        const float inv = ls == 0.0f ? 0.0f : 1.0f / ls;
-        if (4 * lane < a.c.hd)
-            store4((T*)a.out + row.out + 4 * lane, a.vec_out, make_float4(os.x * inv, os.y * inv, os.z * inv, os.w * inv));
     }
+    const float inv = ls == 0.0f ? 0.0f : 1.0f / ls;
+    if (row.out >= 0 && 4 * lane < a.c.hd)
+        store4((T*)a.out + row.out + 4 * lane, a.vec_out, make_float4(os.x * inv, os.y * inv, os.z * inv, os.w * inv));
 }
 
 }  // namespace aion
