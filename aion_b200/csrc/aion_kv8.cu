@@ -297,10 +297,10 @@ static cudaError_t launch_append(const KvAppendArgs& a, cudaStream_t st) {
         return cudaGetLastError();
     }
     const unsigned grid = (unsigned)((int64_t)kv_places(true, a.r.n_seq, a.r.n_tok, a.c.page_log, 2) * a.c.nkv * 2);
-    if (a.c.page == 16) k_kv_append<T, 2><<<grid, kKvAppendThreads, 0, st>>>(a);
-    else if (a.c.page == 32) k_kv_append<T, 4><<<grid, kKvAppendThreads, 0, st>>>(a);
-    else if (a.c.page == 64) k_kv_append<T, 8><<<grid, kKvAppendThreads, 0, st>>>(a);
-    else k_kv_append<T, 16><<<grid, kKvAppendThreads, 0, st>>>(a);
+    if (a.c.page == 16) k_kv_append<T, 4, 128><<<grid, 128, 0, st>>>(a);
+    else if (a.c.page == 32) k_kv_append<T, 8, 128><<<grid, 128, 0, st>>>(a);
+    else if (a.c.page == 64) k_kv_append<T, 16, 128><<<grid, 128, 0, st>>>(a);
+    else k_kv_append<T, 16, 256><<<grid, 256, 0, st>>>(a);
     return cudaGetLastError();
 }
 

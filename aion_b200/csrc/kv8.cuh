@@ -500,14 +500,15 @@ struct KvAppendArgs {
 };
 // Block (place, K or V, head, heads fastest: neighbours read neighbouring
 // rows): the rows of one page and head, four values a thread and step, all of
-// them loaded before the scale is known and kept in registers (PIECES = page /
-// 8 steps at most).  Bound by memory: a row is read once and leaves as a
-// quarter (or half) of its bytes; 32 x 512 fp32 rows of 32 heads of 128 take
-// 156 us, 4.3 TB/s.
+// them loaded before the scale is known and kept in registers (PIECES = page hd
+// / (4 THREADS) steps at most).  Bound by memory, and by instructions next to
+// it, so warps are few and take many steps: with 256 threads a page of 64 took
+// 1.1 times as long.  32 x 512 fp32 rows of 32 heads of 128 take 138 us, 4.9
+// TB/s.
 constexpr int kKvAppendThreads = 256;
-template <typename T, int PIECES>
-__global__ void __launch_bounds__(kKvAppendThreads) k_kv_append(KvAppendArgs a) {
-    __shared__ uint32_t red[kKvAppendThreads / 32];
+template <typename T, int PIECES, int THREADS>
+__global__ void __launch_bounds__(THREADS) k_kv_append(KvAppendArgs a) {
+    __shared__ uint32_t red[THREADS / 32];
     const KvView& c = a.c;
     const int h = blockIdx.x % c.nkv, isv = (blockIdx.x / c.nkv) & 1;
     int idx;
@@ -528,14 +529,14 @@ __global__ void __launch_bounds__(kKvAppendThreads) k_kv_append(KvAppendArgs a) 
     const int rows = (int)(hi - lo), row0 = (int)(lo & (c.page - 1)), ppr = c.hd / 4, n = rows * ppr;   // pieces of a row
     float4 v[PIECES];
     uint32_t top = 0;
-    const int dr = kKvAppendThreads / ppr, dc = kKvAppendThreads - dr * ppr, first = threadIdx.x / ppr;
+    const int dr = THREADS / ppr, dc = THREADS - dr * ppr, first = threadIdx.x / ppr;
     auto load = [&](auto vec) {
         int col = threadIdx.x - first * ppr;
         const T* p = x + first * stride + 4 * col;
         const long long step = dr * stride + 4 * dc, wrap = stride - c.hd;
 #pragma unroll
         for (int e = 0; e < PIECES; e++) {
-            v[e] = (int)threadIdx.x + e * kKvAppendThreads < n ? load4(p, vec.value) : make_float4(0, 0, 0, 0);
+            v[e] = (int)threadIdx.x + e * THREADS < n ? load4(p, vec.value) : make_float4(0, 0, 0, 0);
             p += step;
             col += dc;
             if (col >= ppr) {
@@ -547,7 +548,7 @@ __global__ void __launch_bounds__(kKvAppendThreads) k_kv_append(KvAppendArgs a) 
     if (a.vec) load(std::true_type{});
     else load(std::false_type{});
     bool bad = slot < 0 || slot >= c.max_seqs;
-    for (int j = threadIdx.x; j < s; j += kKvAppendThreads) bad = bad || a.r.seqs[j] == slot;
+    for (int j = threadIdx.x; j < s; j += THREADS) bad = bad || a.r.seqs[j] == slot;
     const int page = slot >= 0 && slot < c.max_seqs && pg < c.max_pages ? c.tables[(size_t)slot * c.max_pages + pg] : -1;
     if (__syncthreads_or(bad)) {
         if (threadIdx.x == 0) kv_flag(c, KV_BAD_ARG);
@@ -566,15 +567,15 @@ __global__ void __launch_bounds__(kKvAppendThreads) k_kv_append(KvAppendArgs a) 
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = top;
     __syncthreads();   // every thread has the old scale, too
 #pragma unroll
-    for (int w = 0; w < kKvAppendThreads / 32; w++) top = max(top, red[w]);
+    for (int w = 0; w < THREADS / 32; w++) top = max(top, red[w]);
     const float sc = kv_scale_of(top, row0 != 0, old);
     if (threadIdx.x == 0) *scale = sc;
-    if (row0 && sc != old) kv_rescale(pool, row0 * ppr, threadIdx.x, kKvAppendThreads, old, sc);
+    if (row0 && sc != old) kv_rescale(pool, row0 * ppr, threadIdx.x, THREADS, old, sc);
     const float inv = __fdiv_rn(1.0f, sc);
     uint32_t* to = reinterpret_cast<uint32_t*>(pool) + row0 * ppr;
 #pragma unroll
     for (int e = 0; e < PIECES; e++) {
-        const int i = threadIdx.x + e * kKvAppendThreads;
+        const int i = threadIdx.x + e * THREADS;
         if (i < n) to[i] = sc > 0.0f ? kv_quant4(v[e], sc, inv) : 0u;
     }
 }
