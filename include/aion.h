@@ -461,8 +461,9 @@ AION_API aion_status aion_kv8_status(const aion_kv8* kv, void* stream);
  * of each sequence's last token.  Needs an int4 file and tp_size 1; W4A8
  * contexts run the same products.  AION_ERR_OOM when the cache has no room
  * for a sequence, AION_ERR_ARG when one would pass the checkpoint's seq_len:
- * every slot is then as long as before.  Waits for its own work; what other
- * streams do to the cache has to be complete before the call. */
+ * every slot is then as long as before.  What earlier calls left for
+ * aion_kv8_status is returned before anything grows.  Waits for its own work;
+ * what other streams do to the cache has to be complete before the call. */
 AION_API aion_status aion_extend(aion_ctx* ctx, const aion_kv8* kv, const int32_t* seqs, const int32_t* n_new,
                                  const int32_t* tokens, int32_t n_seq, float* logits_host);
 

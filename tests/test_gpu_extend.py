@@ -191,3 +191,17 @@ def test_extend_refuses_a_tensor_parallel_or_fp32_context(cuda, tiny_f32_path):
         with pytest.raises(A.AionError) as e:
             m.extend(pair(A, m, 16, 4)[0], [0], [[1]])
         assert e.value.code == "STATE"
+
+
+def test_extend_returns_what_earlier_calls_left_to_report(cuda, tiny_path):
+    import aion_b200 as A
+    with A.Model(tiny_path) as m:
+        c, _ = pair(A, m, 16, 4)
+        c.grow(cuda.tensor([0], dtype=cuda.int32, device="cuda"), cuda.tensor([65], dtype=cuda.int32, device="cuda"))
+        cuda.cuda.synchronize()
+        with pytest.raises(A.AionError) as e:
+            m.extend(c, [1], [[1, 2]])
+        assert e.value.code == "OOM" and c.lens.sum().item() == 0 and c.refs.sum().item() == 0
+        m.extend(c, [1], [[1, 2]])
+        assert c.lens[1].item() == 2
+        c.status()

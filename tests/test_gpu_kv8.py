@@ -497,6 +497,68 @@ def test_many_rows_captured_and_replayed(cuda):
         assert cuda.equal(first, out) and cuda.equal(eager, out)
 
 
+def test_many_rows_do_not_change_from_run_to_run_or_beside_another_stream(cuda):
+    p = Pair(cuda, 1, 80, 16, 128, 3, 20, 64, seed=6)
+    p.fill([700, 500], cuda.float32)
+    q = p.rows(400, 16, cuda.float32)
+    args = p.ints([0, 1]), p.ints([500, 300]), p.ints([0, 200, 400])
+    first = p.c.attention(0, q, *args)
+    streams = [cuda.cuda.Stream() for _ in range(3)]
+    cuda.cuda.synchronize()
+    got = [p.c.attention(0, q, *args, stream=streams[i % 3]) for i in range(9)]
+    cuda.cuda.synchronize()
+    assert all(cuda.equal(first, g) for g in got)
+    p.c.status()
+
+
+@pytest.mark.parametrize("with_cu", [True, False])
+def test_4096_sequences_in_one_call(cuda, with_cu):
+    p = Pair(cuda, 1, 9000, 1, 16, 4096, 2, 16, seed=8)
+    order = p.rng.permutation(4096)
+    for i in range(0, 4096, 1024):   # a page call takes 1024 entries
+        s = order[i:i + 1024].tolist()
+        p.grow(s, (1 + np.asarray(s) % 20).tolist())
+    lens = p.r.lens[order]
+    counts = np.where(order % 3 == 0, 0, np.minimum(lens, 2)) if with_cu else np.ones(4096, int)
+    pos0 = (lens - counts).tolist()
+    p.append(0, order.tolist(), [0] * 4096, lens.tolist(), cuda.float32)
+    p.append(0, order.tolist(), pos0, counts.tolist(), cuda.float32, with_cu=with_cu)
+    p.same()
+    check_attention(p, 0, p.rows(int(counts.sum()), 2, cuda.float32), order.tolist(), pos0, counts.tolist(), "f32", with_cu=with_cu)
+    p.c.status()
+
+
+def test_pages_behind_four_gigabytes(cuda):
+    """K and V of 5 GB each, the pages in use at their ends; a layer and a page copy behind 4 GB, too."""
+    import aion_b200 as A
+    n_pages, nkv, page, hd = 20000, 8, 128, 128
+    pool = (2, n_pages, nkv, page, hd)
+    k, v = (cuda.empty(pool, dtype=cuda.int8, device="cuda") for _ in range(2))
+    ks, vs = (cuda.empty(pool[:3], device="cuda") for _ in range(2))
+    refs = cuda.ones(n_pages, dtype=cuda.int32, device="cuda")
+    refs[-8:] = 0
+    big = A.KV8Cache.wrap(k, v, ks, vs, cuda.full((3, 6), -1, dtype=cuda.int32, device="cuda"),
+                          cuda.zeros(3, dtype=cuda.int32, device="cuda"), refs)
+    p = Pair(cuda, 2, 8, nkv, hd, 3, 6, page, seed=9)
+    x = [p.rows(300, nkv, cuda.float32) for _ in range(2)]
+    one, many = p.rows(1, 16, cuda.float32), p.rows(300, 16, cuda.float32)
+    got = []
+    for c in (p.c, big):
+        pos0 = c.grow(p.ints([1]), p.ints([300]))
+        c.append(1, x[0], x[1], p.ints([1]), pos0, p.ints([0, 300]))
+        c.fork(p.ints([1]), p.ints([2]))
+        at = c.grow(p.ints([2]), p.ints([1]))   # copies the last page
+        c.append(1, x[0][:1] * 2, x[1][:1] * 2, p.ints([2]), at)
+        got.append([c.read(1, p.ints([2]), p.ints([0]), 301, p.ints([0, 301])),
+                    c.attention(1, one, p.ints([2]), p.ints([300])),
+                    c.attention(1, many, p.ints([1]), p.ints([0]), p.ints([0, 300]))])
+        c.status()
+    assert big.tables[1, 0].item() == n_pages - 8 and big.tables[2, 2].item() == n_pages - 5
+    for a, b in zip(got[0][0], got[1][0]):
+        assert cuda.equal(a, b)
+    assert cuda.equal(got[0][1], got[1][1]) and cuda.equal(got[0][2], got[1][2])
+
+
 # ---------------------------------------------------------------------------
 # Entries that are refused on the device
 # ---------------------------------------------------------------------------
