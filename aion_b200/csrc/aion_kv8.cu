@@ -198,7 +198,7 @@ static cudaError_t launch_move(const aion_kv8* kv, int tables, cudaStream_t st) 
     // enough blocks to fill the card, and no more than a call could use
     const int64_t units = ((int64_t)kv->n_kv_heads * kv->page_tokens * kv->head_size + kKvCopyUnit - 1) / kKvCopyUnit;
     const int64_t most = units * kv->n_layers * 2 * kv->n_pages;
-    const int grid = (int)std::min<int64_t>(most, (int64_t)sm_count(kv->device) * 4);
+    const int grid = (int)std::min<int64_t>(most, (int64_t)sm_count(kv->device) * 6);
     return launch_pdl(k_kv_move, dim3(grid), dim3(kKvCopyThreads), 0, st, view_of(kv), tables);
 }
 

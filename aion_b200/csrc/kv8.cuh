@@ -666,7 +666,7 @@ __global__ void __launch_bounds__(kKvAppendThreads) k_kv_read_one(KvReadArgs a) 
 // Block (place of 64 rows, K or V, head, heads fastest): four values a thread
 // and step, eight steps in flight.  Bound by memory, the writes above all: 32 x
 // 512 fp32 rows of 32 heads of 128 take 127 us, 5.3 TB/s.
-constexpr int kKvReadThreads = 256, kKvReadLog = 6, kKvReadSteps = 8;
+constexpr int kKvReadThreads = 128, kKvReadLog = 6, kKvReadSteps = 8;
 template <typename T>
 __global__ void __launch_bounds__(kKvReadThreads) k_kv_read(KvReadArgs a) {
     __shared__ long long s_at[8];
