@@ -257,7 +257,7 @@ __global__ void __launch_bounds__(1024) k_kv_compact(KvView c, int32_t* n_used) 
 // values and scales; with `tables`, rewrites the page tables after a
 // compaction.  A unit is 16 KB of one plane of one page: four 16-byte loads in
 // flight a thread.  Bound by memory: 0.84 GB of pages (32 layers of 32 heads of
-// 128, 64 tokens a page) read and written in 310 us, 5.4 TB/s.
+// 128, 64 tokens a page) read and written in 288 us, 5.8 TB/s.
 constexpr int kKvCopyThreads = 256, kKvCopyUnit = 4 * 16 * kKvCopyThreads;
 __global__ void __launch_bounds__(kKvCopyThreads) k_kv_move(KvView c, int tables) {
     pdl_wait();
@@ -503,7 +503,7 @@ struct KvAppendArgs {
 // them loaded before the scale is known and kept in registers (PIECES = page hd
 // / (4 THREADS) steps at most).  Bound by memory, and by instructions next to
 // it, so warps are few and take many steps: with 256 threads a page of 64 took
-// 1.1 times as long.  32 x 512 fp32 rows of 32 heads of 128 take 138 us, 4.9
+// 1.1 times as long.  32 x 512 fp32 rows of 32 heads of 128 take 128 us, 5.2
 // TB/s.
 constexpr int kKvAppendThreads = 256;
 template <typename T, int PIECES, int THREADS>
@@ -665,7 +665,8 @@ __global__ void __launch_bounds__(kKvAppendThreads) k_kv_read_one(KvReadArgs a) 
 
 // Block (place of 64 rows, K or V, head, heads fastest): four values a thread
 // and step, eight steps in flight.  Bound by memory, the writes above all: 32 x
-// 512 fp32 rows of 32 heads of 128 take 127 us, 5.3 TB/s.
+// 512 fp32 rows of 32 heads of 128 take 115 us, 5.8 TB/s (127 us in blocks of
+// 256 with divisions for each piece).
 constexpr int kKvReadThreads = 128, kKvReadLog = 6, kKvReadSteps = 8;
 template <typename T>
 __global__ void __launch_bounds__(kKvReadThreads) k_kv_read(KvReadArgs a) {
@@ -706,24 +707,42 @@ __global__ void __launch_bounds__(kKvReadThreads) k_kv_read(KvReadArgs a) {
     const int8_t* pool = isv ? c.v : c.k;
     const int in = (int)(first & (c.page - 1));   // the first row's place in its page
     out += (long long)(t0 + i0) * stride + (long long)h * c.hd;
-    for (int base = 0; base < n; base += kKvReadSteps * kKvReadThreads) {
-        uint32_t w[kKvReadSteps];
+    const int dr = kKvReadThreads / ppr, dc = kKvReadThreads - dr * ppr;   // from a thread's piece to its next
+    int row = threadIdx.x / ppr, col = threadIdx.x - row * ppr;
+    auto copy = [&](auto vec) {
+#pragma unroll 1
+        for (int i0 = threadIdx.x; i0 < n; i0 += kKvReadSteps * kKvReadThreads) {
+            uint32_t w[kKvReadSteps];
+            float sc[kKvReadSteps];
+            const int row0 = row, col0 = col;
+            auto next = [&] {
+                row += dr;
+                col += dc;
+                if (col >= ppr) {
+                    col -= ppr;
+                    row++;
+                }
+            };
 #pragma unroll
-        for (int e = 0; e < kKvReadSteps; e++) {
-            const int i = base + e * kKvReadThreads + threadIdx.x, row = i / ppr, r = in + row;
-            const long long at = i < n ? s_at[r >> c.page_log] : -1;
-            w[e] = at >= 0 ? *reinterpret_cast<const uint32_t*>(pool + at + (r & (c.page - 1)) * c.hd + 4 * (i - row * ppr)) : 0u;
-        }
+            for (int e = 0; e < kKvReadSteps; e++, next()) {
+                const int r = in + row, pg = r >> c.page_log;
+                const bool there = i0 + e * kKvReadThreads < n;
+                const long long at = there ? s_at[pg] : -1;
+                w[e] = at >= 0 ? *reinterpret_cast<const uint32_t*>(pool + at + (r & (c.page - 1)) * c.hd + 4 * col) : 0u;
+                sc[e] = there ? s_scale[pg] : 0.0f;
+            }
+            row = row0;
+            col = col0;
 #pragma unroll
-        for (int e = 0; e < kKvReadSteps; e++) {
-            const int i = base + e * kKvReadThreads + threadIdx.x, row = i / ppr;
-            if (i >= n) break;
-            const float sc = s_scale[(in + row) >> c.page_log];
-            store4(out + row * stride + 4 * (i - row * ppr), a.vec,
-                   make_float4((float)(int8_t)w[e] * sc, (float)(int8_t)(w[e] >> 8) * sc, (float)(int8_t)(w[e] >> 16) * sc,
-                               (float)(int8_t)(w[e] >> 24) * sc));
+            for (int e = 0; e < kKvReadSteps; e++, next())
+                if (i0 + e * kKvReadThreads < n)
+                    store4(out + row * stride + 4 * col, vec.value,
+                           make_float4((float)(int8_t)w[e] * sc[e], (float)(int8_t)(w[e] >> 8) * sc[e],
+                                       (float)(int8_t)(w[e] >> 16) * sc[e], (float)(int8_t)(w[e] >> 24) * sc[e]));
         }
-    }
+    };
+    if (a.vec) copy(std::true_type{});
+    else copy(std::false_type{});
 }
 
 }  // namespace aion
