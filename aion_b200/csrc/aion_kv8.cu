@@ -383,7 +383,7 @@ extern "C" AION_API aion_status aion_kv8_read(const aion_kv8* kv, int32_t layer,
 //   fp32, 32 K/V heads, 4 x 4096 keys   16 rows 131 / 71, 32: 131 / 113, 64: 132 / 196
 //   bf16, 8 K/V heads, 16 x 4096 keys   16 rows 104 / 69, 32: 105 / 110, 64: 104 / 187
 //   bf16, 8 K/V heads, 1 x 32768 keys   256 rows 733 / 318, 512: 768 / 605, 1024: 770 / 1170
-// and within 4% of the better one from 4096 keys on over 90 such shapes (20% at 512 keys).
+// and within 4% of the better one from 4096 keys on over 147 such shapes (20% at 512 keys).
 constexpr int kTileUnits = 4;
 static bool attention_tiles(const aion_kv8* kv, int n_seq, int n_tok, int group) {
     const int64_t rows = ((int64_t)n_tok * group + n_seq - 1) / n_seq, lines = (int64_t)n_seq * kv->n_kv_heads;

@@ -503,8 +503,8 @@ struct KvAppendArgs {
 // them loaded before the scale is known and kept in registers (PIECES = page hd
 // / (4 THREADS) steps at most).  Bound by memory, and by instructions next to
 // it, so warps are few and take many steps: with 256 threads a page of 64 took
-// 1.1 times as long.  32 x 512 fp32 rows of 32 heads of 128 take 128 us, 5.2
-// TB/s.
+// 1.1 times as long (a page of 128 has 256, for the registers).  32 x 512 fp32
+// rows of 32 heads of 128 take 128 us, 5.2 TB/s.
 constexpr int kKvAppendThreads = 256;
 template <typename T, int PIECES, int THREADS>
 __global__ void __launch_bounds__(THREADS) k_kv_append(KvAppendArgs a) {
