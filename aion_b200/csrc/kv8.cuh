@@ -341,7 +341,8 @@ __device__ __forceinline__ int kv_warp_find(int n, long long u, First first) {
 // on, up to the next one's.  Its cnt = cu[i+1] - cu[i] rows need at most
 // (cnt >> log) + extra blocks, and floor(a + b) - floor(a) >= floor(b), so the
 // places suffice: extra 1 for blocks of rows, 2 for pages (the first page may
-// begin anywhere).  Returns the sequence of place u.
+// begin anywhere).  Returns the sequence of place u; *index < 0: the place lies
+// in front of cu[0], which need not be 0, and has nothing to do.
 __device__ __forceinline__ int kv_seq_of(const KvRows& r, int u, int log, int extra, int* index) {
     if (!r.cu) {
         *index = 0;
@@ -513,6 +514,7 @@ __global__ void __launch_bounds__(THREADS) k_kv_append(KvAppendArgs a) {
     const int h = blockIdx.x % c.nkv, isv = (blockIdx.x / c.nkv) & 1;
     int idx;
     const int s = kv_seq_of(a.r, blockIdx.x / (2 * c.nkv), c.page_log, 2, &idx);
+    if (idx < 0) return;
     const int t0 = a.r.begin(s), t1 = min(a.r.end(s), a.r.n_tok), p0 = a.r.pos0[s], slot = a.r.seqs[s];
     if (p0 < 0 || t1 <= t0) return;
     const int pg = (p0 >> c.page_log) + idx;                        // page of the slot
@@ -678,6 +680,7 @@ __global__ void __launch_bounds__(kKvReadThreads) k_kv_read(KvReadArgs a) {
     if (!out) return;
     int idx;
     const int s = kv_seq_of(a.r, blockIdx.x / (2 * c.nkv), kKvReadLog, 1, &idx);
+    if (idx < 0) return;
     const int t0 = a.r.begin(s), t1 = min(a.r.end(s), a.r.n_tok), p0 = a.r.pos0[s], slot = a.r.seqs[s];
     const int i0 = idx << kKvReadLog, rows = min(t1 - t0 - i0, 1 << kKvReadLog), ppr = c.hd / 4, n = rows * ppr;
     if (rows <= 0 || t0 < 0) return;

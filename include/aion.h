@@ -392,7 +392,7 @@ AION_API aion_status aion_kv8_compact(const aion_kv8* kv, int32_t* n_used, void*
 
 /* Writes the K and V rows of n_tok tokens of n_seq sequences into `layer`.
  * Sequence i has the rows cu[i] .. cu[i+1]-1 (cu NULL: one row each, n_tok =
- * n_seq) and they stand at positions pos0[i], pos0[i]+1, ... of slot seqs[i],
+ * n_seq; cu[0] need not be 0) and they stand at positions pos0[i], pos0[i]+1, ... of slot seqs[i],
  * which has pages for them (aion_kv8_grow); pos0[i] < 0 skips the sequence.
  * Rows are [n_kv_heads][head_size] of `type`, k_stride / v_stride elements
  * apart.  Per page and head the scale is
@@ -411,7 +411,8 @@ AION_API aion_status aion_kv8_append(const aion_kv8* kv, int32_t layer, const vo
 
 /* The K and V rows at those positions as the cache holds them, q * s rounded
  * to `type` (k or v may be NULL).  Rows of a skipped sequence or of a page
- * that is missing are zero; rows from cu[n_seq] on are left as they were. */
+ * that is missing are zero; rows in front of cu[0] and from cu[n_seq] on are
+ * left as they were. */
 AION_API aion_status aion_kv8_read(const aion_kv8* kv, int32_t layer, void* k, void* v, int32_t type,
                                    int64_t k_stride, int64_t v_stride, const int32_t* seqs, const int32_t* pos0,
                                    const int32_t* cu, int32_t n_seq, int32_t n_tok, void* stream);
@@ -422,8 +423,8 @@ AION_API aion_status aion_kv8_read(const aion_kv8* kv, int32_t layer, void* k, v
  * K/V head h / (n_heads / n_kv_heads).  q and out are [n_heads][head_size]
  * rows of `type`, q_stride / out_stride elements apart, and do not overlap.
  * scale 0: 1 / sqrt(head_size).  A sequence with pos0[i] < 0 gets zeros;
- * positions whose page is missing are left out; rows from cu[n_seq] on are
- * left as they were.  The products are exact, the softmax and the sums fp32,
+ * positions whose page is missing are left out; rows in front of cu[0] and
+ * from cu[n_seq] on are left as they were.  The products are exact, the softmax and the sums fp32,
  * and out is rounded once.  What is rounded before: where a K/V head has few
  * rows, queries and weights to fixed point (24 bits for fp32 rows, 16 for
  * 16-bit rows, relative to the largest of a row, or of 64 weights); where it
