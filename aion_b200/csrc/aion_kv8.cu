@@ -62,6 +62,12 @@ static aion_status check_shape(const aion_kv8* kv, const char* what) {
                           kv->n_layers, kv->n_pages, kv->n_kv_heads, kv->max_seqs, kKvMaxSeqs, kv->max_pages);
         return AION_ERR_SHAPE;
     }
+    // Each count is in range, but sizes in bytes and offsets are products of them in 64 bits.
+    if ((double)kv->n_layers * kv->n_pages * kv->n_kv_heads * kv->page_tokens * kv->head_size > 1152921504606846976.0) {   // 2^60
+        aion_thread_error("%s: %d layers of %d pages of %d x %d x %d values pass 2^60 bytes", what, kv->n_layers, kv->n_pages,
+                          kv->n_kv_heads, kv->page_tokens, kv->head_size);
+        return AION_ERR_SHAPE;
+    }
     return AION_OK;
 }
 

@@ -358,7 +358,8 @@ enum { AION_F32 = 0, AION_F16 = 1, AION_BF16 = 2 };
 
 /* Allocates a cache of the shape in *shape (its int32 fields; the pointers
  * are ignored) in one device allocation, empty, and fills *out.  Waits for
- * the device memory to be cleared. */
+ * the device memory to be cleared.  AION_ERR_SHAPE for K values past 2^60
+ * bytes, AION_ERR_OOM for what the device has no memory for. */
 AION_API aion_status aion_kv8_create(const aion_kv8* shape, aion_kv8* out);
 /* Frees a cache that aion_kv8_create made; clears *kv. */
 AION_API aion_status aion_kv8_destroy(aion_kv8* kv);
@@ -392,8 +393,9 @@ AION_API aion_status aion_kv8_compact(const aion_kv8* kv, int32_t* n_used, void*
 
 /* Writes the K and V rows of n_tok tokens of n_seq sequences into `layer`.
  * Sequence i has the rows cu[i] .. cu[i+1]-1 (cu NULL: one row each, n_tok =
- * n_seq; cu[0] need not be 0) and they stand at positions pos0[i], pos0[i]+1, ... of slot seqs[i],
- * which has pages for them (aion_kv8_grow); pos0[i] < 0 skips the sequence.
+ * n_seq; cu[0] need not be 0) and they stand at positions pos0[i],
+ * pos0[i]+1, ... of slot seqs[i], which has pages for them (aion_kv8_grow);
+ * pos0[i] < 0 skips the sequence.
  * Rows are [n_kv_heads][head_size] of `type`, k_stride / v_stride elements
  * apart.  Per page and head the scale is
  *   s = max|x| / 127                       for a page that starts here,
@@ -424,9 +426,9 @@ AION_API aion_status aion_kv8_read(const aion_kv8* kv, int32_t layer, void* k, v
  * rows of `type`, q_stride / out_stride elements apart, and do not overlap.
  * scale 0: 1 / sqrt(head_size).  A sequence with pos0[i] < 0 gets zeros;
  * positions whose page is missing are left out; rows in front of cu[0] and
- * from cu[n_seq] on are left as they were.  The products are exact, the softmax and the sums fp32,
- * and out is rounded once.  What is rounded before: where a K/V head has few
- * rows, queries and weights to fixed point (24 bits for fp32 rows, 16 for
+ * from cu[n_seq] on are left as they were.  The products are exact, the
+ * softmax and the sums fp32, and out is rounded once.  What is rounded before:
+ * where a K/V head has few rows, queries and weights to fixed point (24 bits for fp32 rows, 16 for
  * 16-bit rows, relative to the largest of a row, or of 64 weights); where it
  * has many, fp32 queries and weights to 22 bits, weights of 16-bit rows to
  * fp16.

@@ -174,3 +174,13 @@ def test_one_workspace_serves_every_call(built):
     assert len(sizes) == 1 and sizes.pop() > 0
     kv = view(page_tokens=64, max_pages=16)
     assert A.lib().aion_kv8_attention_workspace(ctypes.addressof(kv), 4, 2, 2) == 0
+
+
+@pytest.mark.parametrize("over,status", [
+    (dict(n_layers=65535, n_pages=1 << 24, n_kv_heads=65535, page_tokens=128, head_size=128), SHAPE),   # 2^70 bytes
+    (dict(n_layers=1 << 15, n_pages=1 << 24, n_kv_heads=1 << 13, page_tokens=32, head_size=128), SHAPE)])   # 2^64: 0 in 64 bits
+def test_sizes_past_64_bits_are_refused(built, over, status):
+    import aion_b200 as A
+    kv, out = view(**over), A.KV8()
+    assert A.lib().aion_kv8_create(ctypes.byref(kv), ctypes.byref(out)) == status
+    assert not out.k and append(kv) == status
