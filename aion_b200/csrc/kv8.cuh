@@ -40,37 +40,41 @@ __device__ __forceinline__ void kv_flag(const KvView& c, int bit) { atomicOr(c.w
 // ---------------------------------------------------------------------------
 
 // Exclusive scan over the block's 1024 threads; *total in every thread.
-__device__ __forceinline__ int block_scan_1024(int v, int* total, int* red) {
+template <typename V>
+__device__ __forceinline__ V block_scan_1024(V v, V* total, V* red) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int x = v;
+    V x = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        const V y = __shfl_up_sync(0xffffffffu, x, o);
         if (lane >= o) x += y;
     }
     __syncthreads();   // red may still be read from the last scan
     if (lane == 31) red[warp] = x;
     __syncthreads();
-    const int w = red[lane];
-    int s = w;
+    const V w = red[lane];
+    V s = w;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, s, o);
+        const V y = __shfl_up_sync(0xffffffffu, s, o);
         if (lane >= o) s += y;
     }
     *total = __shfl_sync(0xffffffffu, s, 31);
-    const int before = __shfl_sync(0xffffffffu, s - w, warp);
+    const V before = __shfl_sync(0xffffffffu, s - w, warp);
     return before + x - v;
 }
 
 // One block.  Thread i takes entry i: what it needs, then an inclusive scan of
 // the needs gives its place in the list of free pages; a sweep over refs in
-// tiles of 4096 pages builds that list and stops once it is long enough.
+// tiles of 4096 pages builds that list and stops once it is long enough.  The
+// needs add up past 32 bits (1024 entries of up to 2^26 pages), so they are
+// summed in 64; a sum past the number of pages is refused whatever it is.
 __global__ void __launch_bounds__(1024) k_kv_grow(KvView c, const int32_t* seqs, const int32_t* n_new, int n,
                                                   int32_t* pos0) {
     __shared__ int first[kKvMaxSeqs];
     __shared__ int s_upto[kKvMaxList], s_slot[kKvMaxList], s_have[kKvMaxList], s_last[kKvMaxList];
     __shared__ int red[32], s_moves;
+    __shared__ long long wide[32];
     const int i = threadIdx.x;
     for (int j = i; j < c.max_seqs; j += 1024) first[j] = 0x7FFFFFFF;
     if (i == 0) s_moves = 0;
@@ -99,8 +103,9 @@ __global__ void __launch_bounds__(1024) k_kv_grow(KvView c, const int32_t* seqs,
         }
     }
     if (i < n && !ok) kv_flag(c, KV_BAD_ARG);
-    int total;
-    const int upto = block_scan_1024(need, &total, red) + need;
+    long long asked;
+    const int upto = (int)min(block_scan_1024<long long>(need, &asked, wide) + need, c.n_pages + 1LL);
+    const int total = (int)min(asked, c.n_pages + 1LL);
     s_upto[i] = upto;
     s_slot[i] = slot;
     s_have[i] = have;

@@ -47,3 +47,23 @@ def test_attention_rows_in_front_of_the_first_sequence(cuda, first, n_kv, counts
     want, _ = p.r.attention(0, q[first:first + n].cpu().numpy(), [0, 1], [3, 3], [0, counts[0], n])
     assert np.abs(out[first:first + n].cpu().numpy() - want).max() < 1e-4
     p.c.status()
+
+
+# ---------------------------------------------------------------------------
+# Lists whose needs add up past 32 bits
+# ---------------------------------------------------------------------------
+def test_needs_past_32_bits_are_refused(cuda):
+    """600 entries of 2^22 pages each: the sum passes 2^31 in the middle of the list."""
+    import aion_b200 as A
+    n, pages = 600, 1 << 22
+    c = A.KV8Cache(1, 40, 1, 16, n + 2, pages, 16)
+    seqs = cuda.arange(n + 2, dtype=cuda.int32, device="cuda")
+    n_new = cuda.full((n + 2,), pages * 16, dtype=cuda.int32, device="cuda")
+    n_new[0], n_new[300], n_new[-1] = 33, 16, 0   # three pages; one page, but behind what is refused; none
+    pos0 = c.grow(seqs, n_new).tolist()
+    assert pos0 == [0] + [-1] * n + [0]
+    with pytest.raises(A.AionError) as e:
+        c.status()
+    assert e.value.code == "OOM"
+    assert c.lens.tolist() == [33] + [0] * (n + 1) and c.refs.tolist() == [1] * 3 + [0] * 37
+    assert c.tables[:, :4].tolist() == [[0, 1, 2, -1]] + [[-1] * 4] * (n + 1)
