@@ -7,6 +7,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <mutex>
 #include <utility>
 
 #include "kv8.h"
@@ -528,10 +529,19 @@ extern "C" AION_API aion_status aion_kv8_status(const aion_kv8* kv, void* stream
     if (s != AION_OK) return s;
     DeviceGuard dev(kv->device);
     KV_CUDA(dev.err);
+    const cudaStream_t st = (cudaStream_t)stream;
+    KV_CUDA(cudaStreamSynchronize(st));
+    // Calls on other streams may record something at any time, so the word is taken in one piece; one call at a time
+    // brings what it took to the host.
+    static std::mutex one;
     int32_t word = 0;
-    KV_CUDA(cudaMemcpyAsync(&word, kv->work, 4, cudaMemcpyDeviceToHost, (cudaStream_t)stream));
-    KV_CUDA(cudaMemsetAsync(kv->work, 0, 4, (cudaStream_t)stream));
-    KV_CUDA(cudaStreamSynchronize((cudaStream_t)stream));
+    {
+        const std::lock_guard<std::mutex> hold(one);
+        k_kv_take_status<<<1, 1, 0, st>>>(view_of(kv));
+        KV_CUDA(cudaGetLastError());
+        KV_CUDA(cudaMemcpyAsync(&word, kv->work + 3, 4, cudaMemcpyDeviceToHost, st));
+        KV_CUDA(cudaStreamSynchronize(st));
+    }
     if (!word) return AION_OK;
     aion_thread_error("%s:%s%s%s%s", what, word & KV_TIMEOUT ? " a bounded device-side wait gave up: its result is invalid;" : "",
                       word & KV_BAD_ARG ? " an entry was out of range or a slot appeared twice;" : "",

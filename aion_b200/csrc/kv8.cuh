@@ -27,7 +27,7 @@ struct KvView {
     int32_t *tables, *lens, *refs, *work;
     int n_layers, n_pages, nkv, page, page_log, hd, max_seqs, max_pages;
     __host__ __device__ long long plane() const { return (long long)n_pages * nkv * page * hd; }   // one layer, K or V
-    // work[]: 0 status, 1 moves, 2 pages in use, then three lists of n_pages
+    // work[]: 0 status, 1 moves, 2 pages in use, 3 status on its way to the host, then three lists of n_pages
     __device__ int32_t* list(int i) const { return work + 4 + (size_t)i * n_pages; }
 };
 
@@ -315,6 +315,8 @@ __global__ void k_kv_reset(KvView c) {
     for (long long i = i0; i < c.max_seqs; i += step) c.lens[i] = 0;
     if (i0 < 4) c.work[i0] = 0;
 }
+
+__global__ void k_kv_take_status(KvView c) { c.work[3] = atomicExch(c.work, 0); }
 
 // ---------------------------------------------------------------------------
 // Rows of a call: sequence i has rows cu[i]..cu[i+1]-1 at positions pos0[i]...

@@ -443,10 +443,11 @@ AION_API aion_status aion_kv8_attention(const aion_kv8* kv, int32_t layer, const
  * supported. */
 AION_API int64_t aion_kv8_attention_workspace(const aion_kv8* kv, int32_t n_heads, int32_t n_seq, int32_t n_tok);
 
-/* Waits for `stream`, then reports and clears what the calls enqueued before
- * it recorded: AION_ERR_TIMEOUT (a bounded wait inside an attention call
- * gave up: its result is invalid), AION_ERR_ARG (an entry was out of range or a slot appeared
- * twice), AION_ERR_STATE (a page was missing, or an append met a page that
+/* Waits for `stream`, then reports and clears what the cache's calls have
+ * recorded until then, on this stream and any other; what another stream
+ * records meanwhile is kept for the next call.  AION_ERR_TIMEOUT (a bounded
+ * wait inside an attention call gave up: its result is invalid), AION_ERR_ARG
+ * (an entry was out of range or a slot appeared twice), AION_ERR_STATE (a page was missing, or an append met a page that
  * several slots hold), AION_ERR_OOM (aion_kv8_grow refused an entry for want
  * of pages); the first of these that applies. */
 AION_API aion_status aion_kv8_status(const aion_kv8* kv, void* stream);

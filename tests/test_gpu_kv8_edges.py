@@ -67,3 +67,33 @@ def test_needs_past_32_bits_are_refused(cuda):
     assert e.value.code == "OOM"
     assert c.lens.tolist() == [33] + [0] * (n + 1) and c.refs.tolist() == [1] * 3 + [0] * 37
     assert c.tables[:, :4].tolist() == [[0, 1, 2, -1]] + [[-1] * 4] * (n + 1)
+
+
+# ---------------------------------------------------------------------------
+# Reports that other streams leave
+# ---------------------------------------------------------------------------
+def test_a_report_that_another_stream_leaves_meanwhile_is_not_lost(cuda):
+    """A read of a slot that does not exist runs on one stream while the other
+    asks for the status: one of the answers has it."""
+    import aion_b200 as A
+    p = Pair(cuda, 1, 4, 1, 16, 2, 2, 16)
+    slot, at = p.ints([9]), p.ints([0])
+    reader, asker = cuda.cuda.Stream(), cuda.cuda.Stream()
+    cuda.cuda.synchronize()
+
+    def asked():
+        try:
+            p.c.status(asker)
+        except A.AionError as e:
+            assert e.code == "ARG"
+            return 1
+        return 0
+
+    for i in range(1000):
+        with cuda.cuda.stream(reader):
+            cuda.cuda._sleep(97 * (i % 500))   # up to 25 us
+        p.c.read(0, slot, at, 1, stream=reader)
+        got = asked() + asked() + asked()
+        reader.synchronize()
+        assert got + asked() >= 1, i
+    assert asked() == 0
