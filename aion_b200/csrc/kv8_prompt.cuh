@@ -35,10 +35,14 @@ namespace aion {
 // Products of fp16 values are exact in the MMA and summed in fp32.
 // P = 2^(s - m) * 2^7 * vscale / vref in fp16 (fp32 rows: two terms, 22
 // bits), where vref is the largest V scale of the sequence's pages for this
-// head, so that pages of different scales add up in one accumulator; its sum
-// l is kept in fp32 from the unrounded weights.  m is a running reference: it
-// follows the row's maximum only when that has grown by more than 8 (a factor
-// of 2^8, and P stays below 2^15), which leaves O untouched for most tiles.
+// head, so that pages of different scales add up in one accumulator; the sum
+// l of 2^(s - m) is kept in fp32 from the unrounded weights.  m is a running
+// reference of s + log2(vscale / vref) over what the row sees, so that the
+// largest P of a row is 2^7 or more whatever the scales of pages that it does
+// not see, or hardly weighs.  (At -80 the logarithm is cut off, which bounds l
+// by 2^88 a key: only pages that much below another lose bits.)  m follows
+// the row's maximum only when that has grown by more than 8 (a factor of 2^8,
+// and P stays below 2^15), which leaves O untouched for most tiles.
 //
 // A block of 256 rows takes 5K clocks to set up, 13K to bring fp32 queries in,
 // 2.6K (16-bit rows) or 3.3K (fp32) a key tile and 7K to write; the MMAs alone
@@ -53,6 +57,7 @@ constexpr int kKvpStage = 64 * 128 * 2;     // a key tile's K (64 rows, two halv
 constexpr int kKvpRaw = 64 * 128;           // a key tile's K or V as the cache holds it
 constexpr int kKvpSmem = 2 * kKvpQ + 8 * kKvpStage + 4 * kKvpRaw + 1024;
 constexpr uint32_t kKvpWaitLimit = 20000;
+constexpr float kKvpLvMin = -80.0f;
 
 // Registers a thread, by warpgroup; at launch all have 96 (640 threads).
 constexpr int kKvpRegsSoft = 144, kKvpRegsConv = 72, kKvpRegsMma = 40;
@@ -142,8 +147,9 @@ __device__ __forceinline__ bool kvp_wait(uint64_t* bar, uint32_t parity, volatil
 
 // What the softmax needs to know of a key tile: for each 16 of its keys the
 // scales, and which of them have a page.
-struct KvpMeta {
+struct alignas(16) KvpMeta {
     float ks[4], fv[4];   // fv = 2^7 vscale / vref; ks is positive (1 where the page's values are 0 or NaN)
+    float lv[4];          // log2(vscale / vref), kKvpLvMin at least
     uint32_t live, nan;   // bit j: keys 16 j.. have a page; one of its scales is NaN
 };
 
@@ -355,7 +361,7 @@ __global__ void __launch_bounds__(kKvpThreads, 1) k_kv_prompt(const KvAttnArgs a
 #pragma unroll
                 for (int e = 1; e < 15; e += 2) mx = max3(mx, __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
                 mx = fmaxf(mx, __uint_as_float(v[15]));
-                mt = fmaxf(mt, mx * cs[g]);   // fmaxf leaves a NaN out: m is never one
+                mt = fmaxf(mt, fmaf(mx, cs[g], me.lv[g]));   // fmaxf leaves a NaN out: m is never one
             }
             // the reference follows the maximum in steps of more than 8
             const bool grow = mt > m + 8.0f;
@@ -418,11 +424,11 @@ __global__ void __launch_bounds__(kKvpThreads, 1) k_kv_prompt(const KvAttnArgs a
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_addr(&p_full[tile][j & 1]));
         }
-        // ---- out = O vref / (2^7 l)
+        // ---- out = O / (2^7 l) vref, in this order: vref may be near the end of the range
         if (ok && mine > 0) ok = wait_for(&o_full[tile], 0);
         tc_fence_after();
         if (ok && (tile < nq)) {
-            const float f = l == 0.0f ? 0.0f : vref * 0.0078125f / l;
+            const float f = l == 0.0f ? 0.0f : 0.0078125f / l;
             T* dst = (T*)a.out + (q.t0 + tok) * a.out_stride + (long long)head * c.hd;
             if (a.vec_out) {
                 // Through the place of the tile's queries, which no MMA reads any more, 16 bytes a piece: a store then
@@ -437,7 +443,7 @@ __global__ void __launch_bounds__(kKvpThreads, 1) k_kv_prompt(const KvAttnArgs a
                     float x[16];
                     if (mine > 0) tmem_ld16(to + b, x);
 #pragma unroll
-                    for (int e = 0; e < 16; e++) x[e] = l == 0.0f || mine == 0 ? 0.0f : x[e] * f;
+                    for (int e = 0; e < 16; e++) x[e] = l == 0.0f || mine == 0 ? 0.0f : x[e] * f * vref;
 #pragma unroll
                     for (int e = 0; e < 16 / PV; e++) {
                         T y[PV];
@@ -464,7 +470,7 @@ __global__ void __launch_bounds__(kKvpThreads, 1) k_kv_prompt(const KvAttnArgs a
                     float x[16];
                     if (mine > 0) tmem_ld16(to + b, x);
 #pragma unroll
-                    for (int e = 0; e < 16; e++) x[e] = l == 0.0f || mine == 0 ? 0.0f : x[e] * f;
+                    for (int e = 0; e < 16; e++) x[e] = l == 0.0f || mine == 0 ? 0.0f : x[e] * f * vref;
                     if (live_row) store16(dst + b, false, x);
                 }
             }
@@ -499,7 +505,8 @@ __global__ void __launch_bounds__(kKvpThreads, 1) k_kv_prompt(const KvAttnArgs a
             const bool in = 16 * kc < c.hd;
             const int8_t* src = c.k + a.layer * c.plane() + kr * c.hd + 16 * kc;
             const float* scales = ((lane & 4) ? c.v_scale : c.k_scale) + (long long)a.layer * c.n_pages * c.nkv;
-            const float vinv = vref > 0.0f ? 128.0f / vref : 0.0f;
+            // 1 / vref in two factors, since a small vref's is past fp32's range: 1 or 2^64, and what is left
+            const float vinv0 = vref < 1.0f ? 18446744073709551616.0f : 1.0f, vinv1 = vref > 0.0f ? 1.0f / (vref * vinv0) : 0.0f;
             unsigned char *mine = raw + 16 * id;   // the thread's pieces, 2 KB apart
             unsigned char *to0 = kst + kvp_piece(64, kr, 2 * kc), *to1 = kst + kvp_piece(64, kr, 2 * kc + 1);   // + 2 KB every 16 rows
             auto fetch = [&](int j, int page) {
@@ -546,7 +553,9 @@ __global__ void __launch_bounds__(kKvpThreads, 1) k_kv_prompt(const KvAttnArgs a
                     const unsigned nan = __ballot_sync(0xffffffffu, ks != ks || vs != vs);
                     if (lane < 4) {
                         me.ks[lane] = ks > 0.0f ? ks : 1.0f;
-                        me.fv[lane] = vs > 0.0f ? vs * vinv : 0.0f;
+                        const float part = vs > 0.0f ? vs * vinv0 * vinv1 : 0.0f;
+                        me.fv[lane] = 128.0f * part;
+                        me.lv[lane] = fmaxf(__log2f(part), kKvpLvMin);
                     }
                     if (lane == 0) {
                         me.live = live & 0xF;

@@ -4,7 +4,7 @@ from __future__ import annotations
 import numpy as np
 import pytest
 
-from test_gpu_kv8 import Pair
+from test_gpu_kv8 import TYPES, Pair, dtype_of
 
 pytestmark = pytest.mark.gpu
 
@@ -97,3 +97,88 @@ def test_a_report_that_another_stream_leaves_meanwhile_is_not_lost(cuda):
         reader.synchronize()
         assert got + asked() >= 1, i
     assert asked() == 0
+
+
+# ---------------------------------------------------------------------------
+# Pages whose scales are far apart, or near the end of fp32's range
+# ---------------------------------------------------------------------------
+def by_terms(p, q, seqs, pos0, counts, scale=None):
+    """(out, bound, score bound) of layer 0 in 64 bits.  bound[row][head] = sum of the
+    row's weights times 127 V scales, divided by the sum of the weights: what
+    relative errors of the terms are relative to, whatever the scales of pages
+    that the row does not see or hardly weighs."""
+    heads, hd = q.shape[1:]
+    group = heads // p.r.k.shape[2]
+    scale = 1 / np.sqrt(hd) if scale is None else scale
+    out, bound, score = np.zeros(q.shape), np.zeros(q.shape[:2]), np.zeros(q.shape[:2])
+    at = 0
+    for slot, p0, n in zip(seqs, pos0, counts):
+        k, v = p.r.rows(0, slot, p0 + n)
+        vs = p.r.v_scale[0][p.r.tables[slot, np.arange(p0 + n) // p.r.page]].astype(np.float64)
+        for h in range(heads):
+            x, g = q[at:at + n, h].astype(np.float64), h // group
+            s = x @ k[:, g].T * scale
+            s[np.arange(p0 + n)[None, :] > p0 + np.arange(n)[:, None]] = -np.inf
+            w = np.exp(s - s.max(1, keepdims=True))
+            w /= w.sum(1, keepdims=True)
+            out[at:at + n, h], bound[at:at + n, h] = w @ v[:, g], w @ vs[:, g] * 127
+            score[at:at + n, h] = abs(scale) * np.abs(x).max(1) * np.abs(k[:, g]).sum(1).max()
+        at += n
+    return out, bound, score
+
+
+def check_terms(p, q, seqs, pos0, counts, name, weight, with_cu=True, scale=None):
+    """Tolerance, relative to `bound`: twice the error of a score (queries to 22
+    bits or more, sums of the dot and its two factors in fp32: 2^-21 of the
+    largest query times the sum of a key, and 2^-21 for the exponential), the
+    rounding of the weights (`weight`), fp32 sums of groups of 64 (as in the
+    other tests); half a step of the result, infinite where it rounds to that; and, where scales are near the end
+    of fp32's range, half of its smallest step for each group's factor, which
+    meets up to 64 values of 127."""
+    cu = [0] + np.cumsum(counts).tolist()
+    got = p.c.attention(0, q, p.ints(seqs), p.ints(pos0), p.ints(cu) if with_cu else None, scale).float().cpu().numpy()
+    want, bound, score = by_terms(p, q.float().cpu().numpy(), seqs, pos0, counts, scale)
+    seen = np.concatenate([b + 1 + np.arange(n) for b, n in zip(pos0, counts)])[:, None]
+    tol = (2 * (score * 2.0 ** -21 + 2.0 ** -21) + weight + 2.0 ** -22 * (seen / 64 + 4)) * bound + seen * 2.0 ** -143
+    half = {"f32": 2.0 ** -24, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}[name]
+    least = {"f32": 2.0 ** -149, "f16": 2.0 ** -25, "bf16": 2.0 ** -134}[name]
+    tol = tol[..., None] + half * np.abs(want) + least
+    top = {"f32": 2.0 ** 128, "f16": 65520, "bf16": 2.0 ** 128}[name]   # rounds to infinity from here on
+    big = np.abs(want) > top + tol
+    assert (got[big] == np.copysign(np.inf, want[big])).all()
+    with np.errstate(invalid="ignore"):
+        got = np.where(np.abs(want) > top - tol, np.where(np.isinf(got), want, got), got)
+    assert np.isfinite(got).all()
+    err = np.abs(got.astype(np.float64) - want)
+    assert (err <= tol).all(), f"worst {float((err / tol).max())} of the tolerance"
+    p.c.status()
+
+
+def uneven(p, slot, base, ratio, light, heavy):
+    """V scales of a slot's pages: `base`, but 1 / ratio of it on page `heavy`
+    (which late rows see alone) and on page `light`, whose keys point away from
+    every query of positive channels, so that their weights are about 2^-60."""
+    table = p.r.tables[slot]
+    p.r.v_scale[0, table[table >= 0]] *= np.float32(base)
+    for page in (table[light], table[heavy]):
+        p.r.v_scale[0, page] = np.minimum(p.r.v_scale[0, page].astype(np.float64) / ratio, 2.0 ** 100)
+    p.r.k[0, table[light]] = -127
+    p.r.k_scale[0, table[light]] = 60 * np.log(2) / 127 / np.sqrt(p.r.k.shape[-1]) / 0.8   # 0.8: the mean of |q|
+    p.upload()
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("base,ratio", [(1e-37, 1.0), (1e-30, 1.0), (1.0, 2.0 ** -10), (1.0, 2.0 ** -20), (1e-20, 2.0 ** -40),
+                                        (1e-30, 2.0 ** -70)])
+def test_many_rows_over_pages_of_uneven_scales(cuda, name, page, base, ratio):
+    """Weights: two fp16 terms for fp32 rows (2^-22 of each), one for the others
+    (2^-11), and 2^-32 of the largest term for each key."""
+    if name == "f16" and base < 1e-10:
+        pytest.skip("results below fp16's range")
+    dt = dtype_of(cuda, name)
+    p = Pair(cuda, 1, 40, 16, 32, 2, 40, page, seed=page)
+    p.fill([320], dt)
+    uneven(p, 0, base, ratio, 0 if page == 16 else 1, 320 // page - 1)
+    q = p.rows(320, 16, dt).abs()
+    check_terms(p, q, [0], [0], [320], name, (2.0 ** -22 if name == "f32" else 2.0 ** -11) + 320 * 2.0 ** -32)
