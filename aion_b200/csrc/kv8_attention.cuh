@@ -24,23 +24,27 @@ struct KvAttnArgs {
 
 // ---------------------------------------------------------------------------
 // Arithmetic.  K and V stay the int8 values that the cache holds; the query
-// and the softmax weights become fixed-point numbers of D base-256 digits, so
-// that every product is an exact integer dot on the tensor cores
+// becomes a fixed-point number of 3 base-256 digits and the softmax weights of
+// D, so that every product is an exact integer dot on the tensor cores
 // (mma.sync.m16n8k32, s32 accumulators):
-//   q = rint(x 127 256^(D-1) / max|x|), digits in -128..127, per row;
-//   score = max|x| / (127 256^(D-1)) * K scale * sum_d 256^(D-1-d) (K . q_d);
+//   q = rint(x 127 256^2 / max|x|), digits in -128..127, per row;
+//   score = max|x| / (127 256^2) * K scale * sum_d 256^(2-d) (K . q_d);
 //   w = rint(2^(score - group max) (256^D - 1)), digits in 0..255;
 //   out += V scale * 2^(group max - running max) / (256^D - 1) * sum_d ....
-// D is 3 for fp32 rows (a step of 2^-23 of the largest value: fp32's own) and
-// 2 for 16-bit rows (2^-15, against the 2^-8 or 2^-11 of a rounded result).
-// Weights are relative to the largest of their 64 positions, so a position far
-// below its row's maximum keeps its share.  Sums run in fp32.
+// A query's step is 2^-23 of its largest value, fp32's own, for 16-bit rows
+// too: an error of a score is exponentiated, and with two digits (a step of
+// 2^-15) an fp16 row with one channel 256 times the others lost scores of 0.01.
+// D is 3 for fp32 rows and 2 for 16-bit rows, whose weights enter linearly: half
+// a step, 2^-17 of the largest of 64, against the 2^-9 or 2^-12 of a rounded
+// result.  Weights are relative to the largest of their 64 positions, so a
+// position far below its row's maximum keeps its share.  Sums run in fp32.
 //
 // Rows and digits are the columns of the MMAs (8 of them).  WIDE: 8 rows, an
 // MMA for each digit, which a lane joins by itself.  Else one MMA holds 4 rows
-// x 2 digits (lane t of a quad has both of row t) or 2 rows x 3 digits in fours
-// (two lanes have a row and swap halves), and half or less of the work around
-// the MMAs is left: one query head per K/V head, or few, as most models decode.
+// x 2 digits (lane t of a quad has both of row t; a query's third digit has an
+// MMA with every other column) or 2 rows x 3 digits in fours (two lanes have a
+// row and swap halves), and half or less of the work around the MMAs is left:
+// one query head per K/V head, or few, as most models decode.
 //
 // Work.  A unit is (sequence, K/V head, so many rows: tokens x query heads of
 // that K/V head); its keys come in groups of 64.  All groups of all units form
@@ -222,14 +226,40 @@ template <int HDP, int D, bool WIDE> struct KvaShape {
     static constexpr int kBlocks = 2 * (kTotal + 1024 + 128) <= 228 * 1024 ? 2 : 1;   // blocks an SM has room for
 };
 
+// The digits' dots of N accumulators, joined: values e < NV of a lane; `odd`: lane & 1.
+__device__ __forceinline__ float kva_three(int a, int b, int c) {
+    return fmaf((float)a, 65536.0f, fmaf((float)b, 256.0f, (float)c));
+}
+template <bool WIDE, int D, int N, int NV>
+__device__ __forceinline__ void kva_join(const int (&acc)[N][4], bool odd, float (&v)[NV]) {
+    if constexpr (WIDE) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            if constexpr (N == 3) v[e] = kva_three(acc[0][e], acc[1][e], acc[2][e]);
+            else v[e] = fmaf((float)acc[0][e], 256.0f, (float)acc[1][e]);
+        }
+    } else if constexpr (N == 2) {   // a query's digits 0 and 1 in one, 2 in the other
+        v[0] = kva_three(acc[0][0], acc[0][1], acc[1][0]);
+        v[1] = kva_three(acc[0][2], acc[0][3], acc[1][2]);
+    } else if constexpr (D == 2) {
+        v[0] = fmaf((float)acc[0][0], 256.0f, (float)acc[0][1]);
+        v[1] = fmaf((float)acc[0][2], 256.0f, (float)acc[0][3]);
+    } else {   // even lanes have digits 0 and 1, odd ones digit 2; even ones keep the first 8 of 16, odd ones the others
+        const float lo = odd ? (float)acc[0][0] : fmaf((float)acc[0][0], 65536.0f, (float)acc[0][1] * 256.0f);
+        const float hi = odd ? (float)acc[0][2] : fmaf((float)acc[0][2], 65536.0f, (float)acc[0][3] * 256.0f);
+        v[0] = (odd ? hi : lo) + __shfl_xor_sync(0xffffffffu, odd ? lo : hi, 1);
+    }
+}
+
 template <typename T, int HDP, int D, bool WIDE>
 __global__ void __launch_bounds__(kKvaThreads, KvaShape<HDP, D, WIDE>::kBlocks) k_kv_attention(const KvAttnArgs a) {
     using SH = KvaShape<HDP, D, WIDE>;
-    constexpr float kQ = D == 3 ? 127.0f * 65536.0f : 127.0f * 256.0f, kP = D == 3 ? 16777215.0f : 65535.0f;
+    constexpr float kQ = 127.0f * 65536.0f, kP = D == 3 ? 16777215.0f : 65535.0f;
     constexpr int KS = HDP / 32, MT = HDP / 16;   // k-steps of a score, 16-dimension tiles of a result
     constexpr int RL = WIDE ? 2 : 1;              // rows a lane has scores of
     constexpr int NV = WIDE ? 4 : D == 2 ? 2 : 1; // its scores of 16 positions
-    constexpr int ND = WIDE ? D : 1;              // MMAs for the digits
+    constexpr int NQ = WIDE ? 3 : D == 2 ? 2 : 1; // MMAs for the digits of a query
+    constexpr int ND = WIDE ? D : 1;              // and of the weights
     extern __shared__ __align__(16) unsigned char smem[];
     if (!a.whole) pdl_launch_dependents();   // the join's launch overlaps; it waits for this grid before it reads
     const KvView& c = a.c;
@@ -364,7 +394,7 @@ __global__ void __launch_bounds__(kKvaThreads, KvaShape<HDP, D, WIDE>::kBlocks) 
     auto my_row = [&](int e) { return WIDE ? 2 * t + e : D == 2 ? t : t >> 1; };   // rows a lane has scores of
     float o[MT][NV], m[RL], l[RL], rs[RL];
     int lim[RL];
-    uint32_t qd[ND][KS][2];
+    uint32_t qd[NQ][KS][2];
     // Lane (g, t) brings column g of the score MMAs: a row, or a digit of one; dimensions 32 k + 4 t..+3 and + 16.
     auto begin_unit = [&](const Item& it) {
 #pragma unroll
@@ -405,26 +435,27 @@ __global__ void __launch_bounds__(kKvaThreads, KvaShape<HDP, D, WIDE>::kBlocks) 
 #pragma unroll
             for (int i = 0; i < 2; i++) {
                 const float* w = reinterpret_cast<const float*>(&v[k][i]);
-                int dg[D][4];
+                int dg[3][4];
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     int z = bad ? 0 : __float2int_rn(w[e] * up * f);
 #pragma unroll
-                    for (int d = D - 1; d >= 0; d--) {
+                    for (int d = 2; d >= 0; d--) {
                         dg[d][e] = (int8_t)z;
                         z = (z - dg[d][e]) >> 8;
                     }
                 }
-                uint32_t pk[D];
+                uint32_t pk[3];
 #pragma unroll
-                for (int d = 0; d < D; d++) pk[d] = pack4(dg[d][0], dg[d][1], dg[d][2], dg[d][3]);
+                for (int d = 0; d < 3; d++) pk[d] = pack4(dg[d][0], dg[d][1], dg[d][2], dg[d][3]);
                 if constexpr (WIDE) {
 #pragma unroll
-                    for (int d = 0; d < D; d++) qd[d][k][i] = pk[d];
+                    for (int d = 0; d < 3; d++) qd[d % NQ][k][i] = pk[d];
                 } else if constexpr (D == 2) {
                     qd[0][k][i] = g & 1 ? pk[1] : pk[0];
+                    qd[NQ - 1][k][i] = g & 1 ? 0u : pk[2];
                 } else {
-                    qd[0][k][i] = (g & 3) == 0 ? pk[0] : (g & 3) == 1 ? pk[1] : (g & 3) == 2 ? pk[D - 1] : 0u;
+                    qd[0][k][i] = (g & 3) == 0 ? pk[0] : (g & 3) == 1 ? pk[1] : (g & 3) == 2 ? pk[2] : 0u;
                 }
             }
         const float r = bad ? __int_as_float(0x7FC00000) : top / kQ * a.scale;
@@ -435,24 +466,6 @@ __global__ void __launch_bounds__(kKvaThreads, KvaShape<HDP, D, WIDE>::kBlocks) 
             lim[e] = __shfl_sync(0xffffffffu, row.lim, from);
             m[e] = -INFINITY;
             l[e] = 0.0f;
-        }
-    };
-    // The digits' dots of an accumulator, joined: values e < NV.
-    auto join = [&](const int (&acc)[ND][4], float (&v)[NV]) {
-        if constexpr (WIDE) {
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                if constexpr (D == 3) v[e] = fmaf((float)acc[0][e], 65536.0f, fmaf((float)acc[1][e], 256.0f, (float)acc[ND - 1][e]));
-                else v[e] = fmaf((float)acc[0][e], 256.0f, (float)acc[ND - 1][e]);
-            }
-        } else if constexpr (D == 2) {
-            v[0] = fmaf((float)acc[0][0], 256.0f, (float)acc[0][1]);
-            v[NV - 1] = fmaf((float)acc[0][2], 256.0f, (float)acc[0][3]);
-        } else {   // even lanes have digits 0 and 1, odd ones digit 2; even ones keep the first 8 of 16, odd ones the others
-            const bool odd = t & 1;
-            const float lo = odd ? (float)acc[0][0] : fmaf((float)acc[0][0], 65536.0f, (float)acc[0][1] * 256.0f);
-            const float hi = odd ? (float)acc[0][2] : fmaf((float)acc[0][2], 65536.0f, (float)acc[0][3] * 256.0f);
-            v[0] = (odd ? hi : lo) + __shfl_xor_sync(0xffffffffu, odd ? lo : hi, 1);
         }
     };
     auto sub = [&](int e) { return g + 8 * (WIDE ? e >> 1 : D == 2 ? e : t & 1); };   // of 16 positions, or dimensions
@@ -531,17 +544,17 @@ __global__ void __launch_bounds__(kKvaThreads, KvaShape<HDP, D, WIDE>::kBlocks) 
                 for (int e = 0; e < RL; e++) mg[e] = -INFINITY;
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
-                    int acc[ND][4];
+                    int acc[NQ][4];
 #pragma unroll
-                    for (int d = 0; d < ND; d++) acc[d][0] = acc[d][1] = acc[d][2] = acc[d][3] = 0;
+                    for (int d = 0; d < NQ; d++) acc[d][0] = acc[d][1] = acc[d][2] = acc[d][3] = 0;
 #pragma unroll
                     for (int k = 0; k < KS; k++) {
                         uint32_t f[4];
                         ldsm_rows(f, ks + 16 * j * HDP + place(lane & 15, 2 * k + (lane >> 4)));
 #pragma unroll
-                        for (int d = 0; d < ND; d++) mma_ss(acc[d], f, qd[d][k][0], qd[d][k][1]);
+                        for (int d = 0; d < NQ; d++) mma_ss(acc[d], f, qd[d][k][0], qd[d][k][1]);
                     }
-                    join(acc, p[j]);
+                    kva_join<WIDE, D>(acc, t & 1, p[j]);
 #pragma unroll
                     for (int e = 0; e < NV; e++) {
                         const int pos = ksc[j] == -1.0f ? 0x7FFFFFFF : key0 + 16 * j + sub(e);   // -1: no page
@@ -624,7 +637,7 @@ __global__ void __launch_bounds__(kKvaThreads, KvaShape<HDP, D, WIDE>::kBlocks) 
                         for (int d = 0; d < ND; d++) mma_su(acc[d], f, pd[d][2 * k], pd[d][2 * k + 1]);
                     }
                     float v[NV];
-                    join(acc, v);
+                    kva_join<WIDE, D>(acc, t & 1, v);
 #pragma unroll
                     for (int e = 0; e < NV; e++) o[mt][e] = fmaf(v[e], wt[e % RL], o[mt][e] * alpha[e % RL]);
                 }

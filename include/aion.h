@@ -428,12 +428,12 @@ AION_API aion_status aion_kv8_read(const aion_kv8* kv, int32_t layer, void* k, v
  * positions whose page is missing are left out; rows in front of cu[0] and
  * from cu[n_seq] on are left as they were.  The products are exact, the
  * softmax and the sums fp32, and out is rounded once.  What is rounded before:
- * where a K/V head has few rows, queries and weights to fixed point (24 bits
- * for fp32 rows, 16 for 16-bit rows, relative to the largest of a row, or of
- * 64 weights); where it has many, fp32 queries and weights to 22 bits, weights
- * of 16-bit rows to fp16, each relative to itself, or to 2^-32 of the row's
- * largest weight times V scale (2^80 times that where the V scales of a
- * sequence's pages are further apart than 2^80).
+ * where a K/V head has few rows, queries to fixed point of 24 bits, relative
+ * to the largest of a row, and weights to 24 bits (fp32 rows) or 16 (16-bit
+ * rows), relative to the largest of 64; where it has many, fp32 queries and
+ * weights to 22 bits and weights of 16-bit rows to fp16, each relative to
+ * itself, or to 2^-32 of the row's largest weight times V scale, for V scales
+ * within 2^80 of one another.
  * `workspace`: aion_kv8_attention_workspace bytes of device memory, 16-byte
  * aligned, that no other call in flight uses (NULL when that is 0). */
 AION_API aion_status aion_kv8_attention(const aion_kv8* kv, int32_t layer, const void* q, void* out, int32_t type,

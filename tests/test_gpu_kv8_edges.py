@@ -127,17 +127,18 @@ def by_terms(p, q, seqs, pos0, counts, scale=None):
     return out, bound, score
 
 
-def check_terms(p, q, seqs, pos0, counts, name, weight, with_cu=True, scale=None):
+def check_terms(p, q, seqs, pos0, counts, name, weight, with_cu=True, scale=None, largest=None):
     """Tolerance, relative to `bound`: twice the error of a score (queries to 22
     bits or more, sums of the dot and its two factors in fp32: 2^-21 of the
-    largest query times the sum of a key, and 2^-21 for the exponential), the
-    rounding of the weights (`weight`), fp32 sums of groups of 64 (as in the
+    largest query times the sum of a key, or, for queries that are held exactly,
+    of the `largest` score; and 2^-21 for the exponential), the rounding of the weights (`weight`), fp32 sums of groups of 64 (as in the
     other tests); half a step of the result, infinite where it rounds to that; and, where scales are near the end
     of fp32's range, half of its smallest step for each group's factor, which
     meets up to 64 values of 127."""
     cu = [0] + np.cumsum(counts).tolist()
     got = p.c.attention(0, q, p.ints(seqs), p.ints(pos0), p.ints(cu) if with_cu else None, scale).float().cpu().numpy()
     want, bound, score = by_terms(p, q.float().cpu().numpy(), seqs, pos0, counts, scale)
+    score = score if largest is None else largest
     seen = np.concatenate([b + 1 + np.arange(n) for b, n in zip(pos0, counts)])[:, None]
     tol = (2 * (score * 2.0 ** -21 + 2.0 ** -21) + weight + 2.0 ** -22 * (seen / 64 + 4)) * bound + seen * 2.0 ** -143
     half = {"f32": 2.0 ** -24, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}[name]
@@ -182,3 +183,30 @@ def test_many_rows_over_pages_of_uneven_scales(cuda, name, page, base, ratio):
     uneven(p, 0, base, ratio, 0 if page == 16 else 1, 320 // page - 1)
     q = p.rows(320, 16, dt).abs()
     check_terms(p, q, [0], [0], [320], name, (2.0 ** -22 if name == "f32" else 2.0 ** -11) + 320 * 2.0 ** -32)
+
+
+# ---------------------------------------------------------------------------
+# Queries with one large channel
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("n_kv,group,counts,before", [
+    (2, 1, [1, 1], [299, 130]), (2, 4, [1, 1], [299, 130]), (2, 4, [5, 3], [290, 128]), (16, 1, [320], [0])])   # four kernels
+def test_queries_with_one_large_channel(cuda, name, hd, n_kv, group, counts, before):
+    """One channel 2^21 times the others, where the keys are 0: the scores come
+    from the smallest digits.  508 = 127 2^16 u and 1..3 u (u = 2^-14) are held
+    exactly by 24-bit fixed point, by fp16 and by two fp16 terms, so a score is
+    off by its fp32 roundings only.  Weights: 64 half steps of 24 or 16 bits of a
+    group's largest, or, in tiles, those of the test above."""
+    dt = dtype_of(cuda, name)
+    p = Pair(cuda, 1, 40, n_kv, hd, 2, 40, 16, seed=hd)
+    p.fill([a + b for a, b in zip(counts, before)], dt)
+    p.r.k[:] = p.rng.integers(0, 128, p.r.k.shape[:-1])[..., None]
+    p.r.k[..., 5] = 0
+    p.upload()
+    q = cuda.from_numpy(p.rng.integers(1, 4, (sum(counts), n_kv * group, hd)).astype(np.float32) * 2.0 ** -14).to(dt).cuda()
+    q[..., 5] = 508
+    scale = 10 / (hd * 127 * 2.0 ** -13)
+    tiles = n_kv == 16
+    weight = {True: 2.0 ** -22 + 320 * 2.0 ** -32, False: 2.0 ** -19}[tiles] if name == "f32" else 2.0 ** -11
+    check_terms(p, q, list(range(len(counts))), before, counts, name, weight, with_cu=counts != [1, 1], scale=scale, largest=10 * 1.5 * 1.5)
