@@ -29,15 +29,20 @@ struct KvAttnArgs {
 // (mma.sync.m16n8k32, s32 accumulators):
 //   q = rint(x 127 256^2 / max|x|), digits in -128..127, per row;
 //   score = max|x| / (127 256^2) * K scale * sum_d 256^(2-d) (K . q_d);
-//   w = rint(2^(score - group max) (256^D - 1)), digits in 0..255;
-//   out += V scale * 2^(group max - running max) / (256^D - 1) * sum_d ....
+//   w = rint(2^(score - m) r (256^D - 1)), digits in 0..255;
+//   out += V * 2^(m - running m) / (256^D - 1) * sum_d ....
+// V is the largest V scale of a group of 64 positions and r a position's own,
+// relative to it; m is the group's largest score + log2 r that the row sees, so
+// the largest 2^(score - m) r is 1, whatever the scales of pages that the row
+// does not see, or hardly weighs (log2 r is cut off at -80, which bounds the sum
+// of 2^(score - m)).
 // A query's step is 2^-23 of its largest value, fp32's own, for 16-bit rows
 // too: an error of a score is exponentiated, and with two digits (a step of
 // 2^-15) an fp16 row with one channel 256 times the others lost scores of 0.01.
 // D is 3 for fp32 rows and 2 for 16-bit rows, whose weights enter linearly: half
 // a step, 2^-17 of the largest of 64, against the 2^-9 or 2^-12 of a rounded
-// result.  Weights are relative to the largest of their 64 positions, so a
-// position far below its row's maximum keeps its share.  Sums run in fp32.
+// result.  Weights are relative to the largest of their group, so a position
+// far below its row's maximum keeps its share.  Sums run in fp32.
 //
 // Rows and digits are the columns of the MMAs (8 of them).  WIDE: 8 rows, an
 // MMA for each digit, which a lane joins by itself.  Else one MMA holds 4 rows
@@ -539,6 +544,16 @@ __global__ void __launch_bounds__(kKvaThreads, KvaShape<HDP, D, WIDE>::kBlocks) 
                 const float4 vscale = *reinterpret_cast<const float4*>(q_scale + 8 * (i & 3) + 4);
                 const float ksc[4] = {kscale.x, kscale.y, kscale.z, kscale.w}, vs[4] = {vscale.x, vscale.y, vscale.z, vscale.w};
                 const uint32_t ks = smem_addr(ring + kslot * SH::kSlot);
+                const float vmax = fmaxf(0.0f, fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3])));   // without a NaN or a missing page
+                float part[4] = {kP, kP, kP, kP}, lv[4] = {0.0f, 0.0f, 0.0f, 0.0f};   // r (256^D - 1), log2 r
+                if (c.page < kKvaT) {
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        part[j] = vs[j] > 0.0f ? vs[j] / vmax : 0.0f;
+                        lv[j] = fmaxf(__log2f(part[j]), -80.0f);
+                        part[j] *= kP;
+                    }
+                }
                 float p[4][NV], mg[RL];
 #pragma unroll
                 for (int e = 0; e < RL; e++) mg[e] = -INFINITY;
@@ -559,11 +574,10 @@ __global__ void __launch_bounds__(kKvaThreads, KvaShape<HDP, D, WIDE>::kBlocks) 
                     for (int e = 0; e < NV; e++) {
                         const int pos = ksc[j] == -1.0f ? 0x7FFFFFFF : key0 + 16 * j + sub(e);   // -1: no page
                         p[j][e] = pos <= lim[e % RL] ? p[j][e] * (rs[e % RL] * ksc[j]) : -INFINITY;
-                        mg[e % RL] = fmaxf(mg[e % RL], p[j][e]);
+                        mg[e % RL] = fmaxf(mg[e % RL], p[j][e] + lv[j]);
                     }
                 }
                 // ---- weights relative to the group's largest
-                const float vmax = fmaxf(0.0f, fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3])));   // without a NaN or a missing page
 #pragma unroll
                 for (int e = 0; e < RL; e++) {
                     if (kLow == 1) mg[e] = fmaxf(mg[e], __shfl_xor_sync(0xffffffffu, mg[e], 1));
@@ -581,13 +595,12 @@ __global__ void __launch_bounds__(kKvaThreads, KvaShape<HDP, D, WIDE>::kBlocks) 
                 float sum[RL] = {};
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
-                    const float ratio = kP * (c.page >= kKvaT ? 1.0f : vmax > 0.0f ? vs[j] / vmax : 0.0f);
 #pragma unroll
                     for (int e = 0; e < NV; e++) {
                         const float w = kv_exp2(p[j][e] - mg[e % RL]);
                         sum[e % RL] += w;
                         if (vs[j] != vs[j] && p[j][e] != -INFINITY) sum[e % RL] = vs[j];   // a NaN scale reaches the rows that see it
-                        const uint32_t z = __float2uint_rn(w * ratio);
+                        const uint32_t z = __float2uint_rn(fminf(w * part[j], kP));   // lv is rounded
                         const int at = 16 * j + sub(e);
                         if constexpr (D == 2 && !WIDE) reinterpret_cast<uint16_t*>(fx + my_row(0) * SH::kWords)[at] = (uint16_t)z;
                         else fx[my_row(e % RL) * SH::kWords + at] = z;

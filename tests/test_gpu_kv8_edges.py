@@ -185,6 +185,25 @@ def test_many_rows_over_pages_of_uneven_scales(cuda, name, page, base, ratio):
     check_terms(p, q, [0], [0], [320], name, (2.0 ** -22 if name == "f32" else 2.0 ** -11) + 320 * 2.0 ** -32)
 
 
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("page", [16, 32, 64])
+@pytest.mark.parametrize("group,counts,before", [(1, [1, 1], [300, 304]), (4, [1, 1], [319, 100]), (4, [6, 3], [300, 301]),
+                                                 (2, [40], [250])])
+@pytest.mark.parametrize("base,ratio", [(1.0, 2.0 ** -8), (1.0, 2.0 ** -10), (2.0 ** -10, 2.0 ** -20), (1e-20, 2.0 ** -40)])
+def test_few_rows_over_pages_of_uneven_scales(cuda, name, page, group, counts, before, base, ratio):
+    """Weights: for each of 64 keys half a step of 24 or 16 bits of a group's largest term."""
+    if name == "f16" and base < 1e-10:
+        pytest.skip("results below fp16's range")
+    dt = dtype_of(cuda, name)
+    p = Pair(cuda, 1, 60, 2, 32, 2, 40, page, seed=page)
+    p.fill([320] * len(counts), dt)
+    for slot in range(len(counts)):
+        uneven(p, slot, base, ratio, 0 if page == 16 else 1, 320 // page - 1)
+    q = p.rows(sum(counts), 2 * group, dt).abs()
+    check_terms(p, q, list(range(len(counts))), before, counts, name, 2.0 ** -19 if name == "f32" else 2.0 ** -11,
+                with_cu=max(counts) > 1)
+
+
 # ---------------------------------------------------------------------------
 # Queries with one large channel
 # ---------------------------------------------------------------------------
