@@ -260,6 +260,7 @@ template <typename T, int HDP, int D, bool WIDE>
 __global__ void __launch_bounds__(kKvaThreads, KvaShape<HDP, D, WIDE>::kBlocks) k_kv_attention(const KvAttnArgs a) {
     using SH = KvaShape<HDP, D, WIDE>;
     constexpr float kQ = 127.0f * 65536.0f, kP = D == 3 ? 16777215.0f : 65535.0f;
+    constexpr float kUp = D == 3 ? 16777216.0f : 65536.0f;   // keeps the factor of a small V scale a normal number
     constexpr int KS = HDP / 32, MT = HDP / 16;   // k-steps of a score, 16-dimension tiles of a result
     constexpr int RL = WIDE ? 2 : 1;              // rows a lane has scores of
     constexpr int NV = WIDE ? 4 : D == 2 ? 2 : 1; // its scores of 16 positions
@@ -609,7 +610,7 @@ __global__ void __launch_bounds__(kKvaThreads, KvaShape<HDP, D, WIDE>::kBlocks) 
 #pragma unroll
                 for (int e = 0; e < RL; e++) {
                     l[e] = l[e] * alpha[e] + wt[e] * sum[e];
-                    wt[e] *= vmax * (1.0f / kP);
+                    wt[e] *= vmax * (kUp / kP);
                 }
                 __syncwarp();
 #pragma unroll
@@ -652,7 +653,7 @@ __global__ void __launch_bounds__(kKvaThreads, KvaShape<HDP, D, WIDE>::kBlocks) 
                     float v[NV];
                     kva_join<WIDE, D>(acc, t & 1, v);
 #pragma unroll
-                    for (int e = 0; e < NV; e++) o[mt][e] = fmaf(v[e], wt[e % RL], o[mt][e] * alpha[e % RL]);
+                    for (int e = 0; e < NV; e++) o[mt][e] = fmaf(v[e] * (1.0f / kUp), wt[e % RL], o[mt][e] * alpha[e % RL]);
                 }
                 __syncwarp();
                 if (i0.g < 0 || i + 1 == n) {   // the unit's last group, or the stretch's

@@ -204,6 +204,21 @@ def test_few_rows_over_pages_of_uneven_scales(cuda, name, page, group, counts, b
                 with_cu=max(counts) > 1)
 
 
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+@pytest.mark.parametrize("page", [32, 64])
+@pytest.mark.parametrize("group,counts,before", [(1, [1, 1], [300, 304]), (4, [1, 1], [319, 100]), (4, [6, 3], [300, 301])])
+@pytest.mark.parametrize("base", [1e-30, 1e-37, 1e30])
+def test_few_rows_over_scales_near_the_ends_of_the_range(cuda, name, page, group, counts, before, base):
+    dt = dtype_of(cuda, name)
+    p = Pair(cuda, 1, 60, 2, 32, 2, 40, page, seed=page)
+    p.fill([320] * len(counts), dt)
+    for slot in range(len(counts)):
+        uneven(p, slot, base, 1.0, 1, 320 // page - 1)
+    q = p.rows(sum(counts), 2 * group, dt).abs()
+    check_terms(p, q, list(range(len(counts))), before, counts, name, 2.0 ** -19 if name == "f32" else 2.0 ** -11,
+                with_cu=max(counts) > 1)
+
+
 # ---------------------------------------------------------------------------
 # Queries with one large channel
 # ---------------------------------------------------------------------------
