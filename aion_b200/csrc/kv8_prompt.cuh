@@ -322,7 +322,7 @@ __global__ void __launch_bounds__(kKvpThreads, 1) k_kv_prompt(const KvAttnArgs a
 
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
         const uint32_t to = tmem + lanes + 256 + 128 * tile;   // O
-        float m = -INFINITY, l = bad ? __int_as_float(0x7FC00000) : 0.0f;   // a NaN in l stays and reaches the result
+        float m = -INFINITY, l = 0.0f;   // a NaN in l stays and reaches the result
         const int mine = nt[tile];
         bool ok = true;
         auto wait_for = [&](uint64_t* bar, int parity) { return (bool)__all_sync(0xffffffffu, kvp_wait(bar, parity & 1, &s_fail)); };
@@ -424,6 +424,7 @@ __global__ void __launch_bounds__(kKvpThreads, 1) k_kv_prompt(const KvAttnArgs a
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_addr(&p_full[tile][j & 1]));
         }
+        if (bad && l != 0.0f) l = __int_as_float(0x7FC00000);   // a query that is not finite, unless it sees nothing
         // ---- out = O / (2^7 l) vref, in this order: vref may be near the end of the range
         if (ok && mine > 0) ok = wait_for(&o_full[tile], 0);
         tc_fence_after();

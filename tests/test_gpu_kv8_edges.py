@@ -244,3 +244,24 @@ def test_queries_with_one_large_channel(cuda, name, hd, n_kv, group, counts, bef
     tiles = n_kv == 16
     weight = {True: 2.0 ** -22 + 320 * 2.0 ** -32, False: 2.0 ** -19}[tiles] if name == "f32" else 2.0 ** -11
     check_terms(p, q, list(range(len(counts))), before, counts, name, weight, with_cu=counts != [1, 1], scale=scale, largest=10 * 1.5 * 1.5)
+
+
+# ---------------------------------------------------------------------------
+# Rows that see nothing
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("n_kv,rows", [(2, 3), (16, 320)])   # streams of keys; tiles of rows
+def test_rows_that_see_nothing_are_zero_whatever_their_query(cuda, name, n_kv, rows):
+    """Slot 0's first 32 positions have no pages; queries that are not finite there and behind."""
+    import aion_b200 as A
+    p = Pair(cuda, 1, 40, n_kv, 32, 2, 40, 16, seed=rows)
+    p.fill([rows + 30], cuda.float32)
+    p.c.tables[0, :2] = -1
+    q = p.rows(rows, n_kv, dtype_of(cuda, name))
+    q[0, 0, 3], q[1, 1, 4], q[-1, 0, 2] = float("nan"), float("inf"), float("nan")
+    out = p.c.attention(0, q, p.ints([0]), p.ints([30]), p.ints([0, rows])).float()   # rows 0 and 1: positions 30 and 31
+    with pytest.raises(A.AionError) as e:
+        p.c.status()
+    assert e.value.code == "STATE"
+    assert (out[:2] == 0).all()
+    assert cuda.isnan(out[-1, 0]).all() and cuda.isfinite(out[-1, 1:]).all() and cuda.isfinite(out[2:-1]).all()
