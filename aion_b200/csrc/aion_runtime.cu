@@ -1454,20 +1454,28 @@ extern "C" AION_API aion_status aion_prefill(aion_ctx* c, const int32_t* tokens,
 // ---------------------------------------------------------------------------
 // New tokens of several sequences against an 8-bit paged cache (aion_kv8)
 // ---------------------------------------------------------------------------
-// Gives back what aion_kv8_grow granted: every granted slot to its length before.
-static void extend_undo(aion_ctx* c, const aion_kv8* kv, const int32_t* seqs, const std::vector<int32_t>& pos0) {
-    std::vector<int32_t> list, keep;
+// Gives back what aion_kv8_grow granted: every granted slot to its length
+// before.  `list` has two words a sequence and nothing is allocated here, so
+// that a call that is out of host memory can be undone, too; the error that
+// the caller reports stays.
+static void extend_undo(aion_ctx* c, const aion_kv8* kv, const int32_t* seqs, const std::vector<int32_t>& pos0,
+                        std::vector<int32_t>& list) {
+    std::string err, thread_err;
+    err.swap(c->err);
+    thread_err.swap(g_thread_err);
+    size_t n = 0, at = 0;
+    for (const int32_t p : pos0) n += p >= 0;
     for (size_t i = 0; i < pos0.size(); i++)
         if (pos0[i] >= 0) {
-            list.push_back(seqs[i]);
-            keep.push_back(pos0[i]);
+            list[at] = seqs[i];
+            list[n + at++] = pos0[i];
         }
-    const size_t n = list.size();
-    list.insert(list.end(), keep.begin(), keep.end());
-    if (n && cudaMemcpyAsync(c->pf.seq, list.data(), list.size() * 4, cudaMemcpyHostToDevice, c->stream) == cudaSuccess)
+    if (n && cudaMemcpyAsync(c->pf.seq, list.data(), 2 * n * 4, cudaMemcpyHostToDevice, c->stream) == cudaSuccess)
         aion_kv8_trim(kv, c->pf.seq, c->pf.seq + n, (int32_t)n, c->stream);
     cudaStreamSynchronize(c->stream);
-    aion_kv8_status(kv, c->stream);   // the refusal is this call's to report
+    aion_kv8_status(kv, c->stream);   // what went wrong is this call's to report
+    err.swap(c->err);
+    thread_err.swap(g_thread_err);
 }
 
 static aion_status extend(aion_ctx* c, const aion_kv8* kv, const int32_t* seqs, const int32_t* n_new,
@@ -1516,6 +1524,8 @@ static aion_status extend(aion_ctx* c, const aion_kv8* kv, const int32_t* seqs, 
     CK_RET(&c->err, cudaSetDevice(c->dev));
     const long long dim = c->dim, hid = c->hidden, kvd = c->kv_dim, mpad = round_up(mrows, kGemmBM);
     const long long kpd = round_up(dim, kGemmBK), kph = round_up(hid, kGemmBK), mcls = round_up(n_seq, kGemmBM);
+    // Host memory for all that follows, before anything grows.
+    std::vector<int32_t> pos0(n_seq), pos((size_t)mrows), map(n_seq), undo(2 * (size_t)n_seq);
     // What earlier calls have left to report is reported before anything grows.
     aion_status st = aion_kv8_status(kv, c->stream);
     if (st != AION_OK) return kv_fail(st);
@@ -1532,10 +1542,8 @@ static aion_status extend(aion_ctx* c, const aion_kv8* kv, const int32_t* seqs, 
     CK_RET(&c->err, cudaMemcpyAsync(pf.tok, tokens, (size_t)mrows * 4, cudaMemcpyHostToDevice, sm));
     st = aion_kv8_grow(kv, d_seqs, d_new, n_seq, d_pos0, sm);
     if (st != AION_OK) return kv_fail(st);
-    std::vector<int32_t> pos0(n_seq);
     CK_RET(&c->err, cudaMemcpyAsync(pos0.data(), d_pos0, n_seq * 4, cudaMemcpyDeviceToHost, sm));
     CK_RET(&c->err, cudaStreamSynchronize(sm));
-    std::vector<int32_t> pos((size_t)mrows), map(n_seq);
     for (int i = 0; i < n_seq; i++) {
         if (pos0[i] < 0 || (long long)pos0[i] + n_new[i] > c->seq) {
             const bool full = pos0[i] < 0;
@@ -1544,56 +1552,65 @@ static aion_status extend(aion_ctx* c, const aion_kv8* kv, const int32_t* seqs, 
             else
                 set_err(&c->err, "aion_extend: sequence %d would reach position %lld of %lld", i, (long long)pos0[i] + n_new[i],
                         (long long)c->seq);
-            extend_undo(c, kv, seqs, pos0);
+            extend_undo(c, kv, seqs, pos0, undo);
             return full ? AION_ERR_OOM : AION_ERR_ARG;
         }
         for (int t = 0; t < n_new[i]; t++) pos[(size_t)cu[i] + t] = pos0[i] + t;
         map[i] = cu[i + 1] - 1;
     }
-    CK_RET(&c->err, cudaMemcpyAsync(d_pos, pos.data(), (size_t)mrows * 4, cudaMemcpyHostToDevice, sm));
-    CK_RET(&c->err, cudaMemcpyAsync(pf.map, map.data(), n_seq * 4, cudaMemcpyHostToDevice, sm));
+    auto run = [&]() -> aion_status {
+        CK_RET(&c->err, cudaMemcpyAsync(d_pos, pos.data(), (size_t)mrows * 4, cudaMemcpyHostToDevice, sm));
+        CK_RET(&c->err, cudaMemcpyAsync(pf.map, map.data(), n_seq * 4, cudaMemcpyHostToDevice, sm));
 
-    const unsigned rows = (unsigned)mrows, padded = (unsigned)mpad;
-    k_pf_embed<<<rows, 256, 0, sm>>>(pf.tok, (int)mrows, c->emb, (int)dim, pf.x);
-    CK_RET(&c->err, cudaGetLastError());
-    for (int l = 0; l < (int)c->L; l++) {
-        long long np = 0;
-        k_pf_norm_split<<<padded, 256, 0, sm>>>(pf.x, nullptr, (int)mrows, (int)dim, (int)kpd, c->rms_att + l * dim, pf.a);
-        st = pf_matmul(c, c->qkv[l], mpad, kpd, &np);
-        if (st != AION_OK) return st;
-        k_pf_rope_rows<<<rows, 256, 0, sm>>>(pf.c, (int)np, (int)mrows, d_pos, (int)dim, (int)kvd, (int)c->hs, c->freq_re,
-                                            c->freq_im);
+        const unsigned rows = (unsigned)mrows, padded = (unsigned)mpad;
+        k_pf_embed<<<rows, 256, 0, sm>>>(pf.tok, (int)mrows, c->emb, (int)dim, pf.x);
         CK_RET(&c->err, cudaGetLastError());
-        st = aion_kv8_append(kv, l, pf.c + dim, pf.c + dim + kvd, AION_F32, np, np, d_seqs, d_pos0, d_cu, n_seq,
-                             (int32_t)mrows, sm);
-        if (st == AION_OK)
-            st = aion_kv8_attention(kv, l, pf.c, pf.q, AION_F32, (int32_t)c->nh, np, dim, 0.0f, d_seqs, d_pos0, d_cu, n_seq,
-                                    (int32_t)mrows, pf.ws, ws, sm);
+        for (int l = 0; l < (int)c->L; l++) {
+            long long np = 0;
+            k_pf_norm_split<<<padded, 256, 0, sm>>>(pf.x, nullptr, (int)mrows, (int)dim, (int)kpd, c->rms_att + l * dim, pf.a);
+            st = pf_matmul(c, c->qkv[l], mpad, kpd, &np);
+            if (st != AION_OK) return st;
+            k_pf_rope_rows<<<rows, 256, 0, sm>>>(pf.c, (int)np, (int)mrows, d_pos, (int)dim, (int)kvd, (int)c->hs, c->freq_re,
+                                                c->freq_im);
+            CK_RET(&c->err, cudaGetLastError());
+            st = aion_kv8_append(kv, l, pf.c + dim, pf.c + dim + kvd, AION_F32, np, np, d_seqs, d_pos0, d_cu, n_seq,
+                                 (int32_t)mrows, sm);
+            if (st == AION_OK)
+                st = aion_kv8_attention(kv, l, pf.c, pf.q, AION_F32, (int32_t)c->nh, np, dim, 0.0f, d_seqs, d_pos0, d_cu, n_seq,
+                                        (int32_t)mrows, pf.ws, ws, sm);
+            if (st != AION_OK) return kv_fail(st);
+            k_pf_split<<<padded, 256, 0, sm>>>(pf.q, (int)mrows, (int)dim, (int)kpd, pf.a);
+            st = pf_matmul(c, c->wo[l], mpad, kpd, &np);
+            if (st != AION_OK) return st;
+            k_pf_residual<<<rows, 256, 0, sm>>>(pf.x, pf.c, (int)np, (int)mrows, (int)dim);
+            k_pf_norm_split<<<padded, 256, 0, sm>>>(pf.x, nullptr, (int)mrows, (int)dim, (int)kpd, c->rms_ffn + l * dim, pf.a);
+            st = pf_matmul(c, c->w13[l], mpad, kpd, &np);
+            if (st != AION_OK) return st;
+            k_pf_swiglu_split<<<padded, 256, 0, sm>>>(pf.c, (int)np, (int)mrows, (int)hid, (int)kph, pf.a);
+            st = pf_matmul(c, c->w2[l], mpad, kph, &np);
+            if (st != AION_OK) return st;
+            k_pf_residual<<<rows, 256, 0, sm>>>(pf.x, pf.c, (int)np, (int)mrows, (int)dim);
+            CK_RET(&c->err, cudaGetLastError());
+        }
+        if (logits_host) {
+            k_pf_norm_split<<<(unsigned)mcls, 256, 0, sm>>>(pf.x, pf.map, n_seq, (int)dim, (int)kpd, c->rms_final, pf.a);
+            long long np = 0;
+            st = pf_matmul(c, c->emb, mcls, kpd, &np);
+            if (st != AION_OK) return st;
+            CK_RET(&c->err, cudaMemcpy2DAsync(logits_host, (size_t)c->vocab * 4, pf.c, (size_t)np * 4, (size_t)c->vocab * 4,
+                                              (size_t)n_seq, cudaMemcpyDeviceToHost, sm));
+        }
+        st = aion_kv8_status(kv, sm);
         if (st != AION_OK) return kv_fail(st);
-        k_pf_split<<<padded, 256, 0, sm>>>(pf.q, (int)mrows, (int)dim, (int)kpd, pf.a);
-        st = pf_matmul(c, c->wo[l], mpad, kpd, &np);
-        if (st != AION_OK) return st;
-        k_pf_residual<<<rows, 256, 0, sm>>>(pf.x, pf.c, (int)np, (int)mrows, (int)dim);
-        k_pf_norm_split<<<padded, 256, 0, sm>>>(pf.x, nullptr, (int)mrows, (int)dim, (int)kpd, c->rms_ffn + l * dim, pf.a);
-        st = pf_matmul(c, c->w13[l], mpad, kpd, &np);
-        if (st != AION_OK) return st;
-        k_pf_swiglu_split<<<padded, 256, 0, sm>>>(pf.c, (int)np, (int)mrows, (int)hid, (int)kph, pf.a);
-        st = pf_matmul(c, c->w2[l], mpad, kph, &np);
-        if (st != AION_OK) return st;
-        k_pf_residual<<<rows, 256, 0, sm>>>(pf.x, pf.c, (int)np, (int)mrows, (int)dim);
-        CK_RET(&c->err, cudaGetLastError());
+        return check_device_error(c);
+    };
+    try {
+        st = run();
+    } catch (const std::bad_alloc&) {   // of an error's text
+        st = AION_ERR_OOM;
     }
-    if (logits_host) {
-        k_pf_norm_split<<<(unsigned)mcls, 256, 0, sm>>>(pf.x, pf.map, n_seq, (int)dim, (int)kpd, c->rms_final, pf.a);
-        long long np = 0;
-        st = pf_matmul(c, c->emb, mcls, kpd, &np);
-        if (st != AION_OK) return st;
-        CK_RET(&c->err, cudaMemcpy2DAsync(logits_host, (size_t)c->vocab * 4, pf.c, (size_t)np * 4, (size_t)c->vocab * 4,
-                                          (size_t)n_seq, cudaMemcpyDeviceToHost, sm));
-    }
-    st = aion_kv8_status(kv, sm);
-    if (st != AION_OK) return kv_fail(st);
-    return check_device_error(c);
+    if (st != AION_OK) extend_undo(c, kv, seqs, pos0, undo);
+    return st;
 }
 
 extern "C" AION_API aion_status aion_extend(aion_ctx* c, const aion_kv8* kv, const int32_t* seqs, const int32_t* n_new,

@@ -468,8 +468,13 @@ AION_API aion_status aion_kv8_status(const aion_kv8* kv, void* stream);
  * contexts run the same products.  AION_ERR_OOM when the cache has no room
  * for a sequence, AION_ERR_ARG when one would pass the checkpoint's seq_len:
  * every slot is then as long as before.  What earlier calls left for
- * aion_kv8_status is returned before anything grows.  Waits for its own work;
- * what other streams do to the cache has to be complete before the call. */
+ * aion_kv8_status is returned before anything grows.  After any other error
+ * (AION_ERR_STATE: an append met a page that is not its slot's alone;
+ * AION_ERR_TIMEOUT; AION_ERR_CUDA) the slots are put back to their lengths,
+ * too, as long as the device answers; a last page that was not full may then
+ * be rounded to the scale of rows that are gone, or lost to rows that were not
+ * finite.  Waits for its own work; what other streams do to the cache has to
+ * be complete before the call. */
 AION_API aion_status aion_extend(aion_ctx* ctx, const aion_kv8* kv, const int32_t* seqs, const int32_t* n_new,
                                  const int32_t* tokens, int32_t n_seq, float* logits_host);
 

@@ -205,3 +205,28 @@ def test_extend_returns_what_earlier_calls_left_to_report(cuda, tiny_path):
         m.extend(c, [1], [[1, 2]])
         assert c.lens[1].item() == 2
         c.status()
+
+
+def test_a_failure_behind_the_growth_is_undone(cuda, tiny_path):
+    """A damaged count of holders: slot 0's last page is not its alone to the append.
+    Slot 1, which has grown in the same call, gives its page back."""
+    import aion_b200 as A
+    with A.Model(tiny_path) as m:
+        c, _ = pair(A, m, 16, 8)
+        m.extend(c, [1], [[1] * 20])
+        m.extend(c, [0], [[1] * 20])
+        c.trim(cuda.tensor([1], dtype=cuda.int32, device="cuda"))
+        last = c.tables[0, 1].item()
+        c.refs[last] = 0
+        cuda.cuda.synchronize()
+        before = c.tables.clone(), c.lens.clone(), c.refs.clone()
+        with pytest.raises(A.AionError) as e:
+            m.extend(c, [1, 0], [[1] * 16, [1]])
+        assert e.value.code == "STATE" and "page" in str(e.value)
+        for a, b in zip(before, (c.tables, c.lens, c.refs)):
+            assert cuda.equal(a, b)
+        c.status()
+        c.refs[last] = 1
+        cuda.cuda.synchronize()
+        m.extend(c, [1, 0], [[1] * 16, [1]])
+        assert c.lens.tolist()[:2] == [21, 16]
