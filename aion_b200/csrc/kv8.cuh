@@ -328,6 +328,16 @@ struct KvRows {
     __device__ __forceinline__ int end(int i) const { return cu ? cu[i + 1] : i + 1; }
 };
 
+// Records row offsets that fall, are negative or pass the rows of the call:
+// thread `i0` of `step` of one block.
+__device__ __forceinline__ void kv_vet_rows(const KvView& c, const KvRows& r, int i0, int step) {
+    if (!r.cu) return;
+    for (int i = i0; i < r.n_seq; i += step) {
+        const int b = r.cu[i], e = r.cu[i + 1];
+        if (r.pos0[i] >= 0 && (b < 0 || e < b || e > r.n_tok)) kv_flag(c, KV_BAD_ARG);
+    }
+}
+
 // The last i < n with first(i) <= u, where first does not fall and first(0) <=
 // u: by a converged warp, 32 places at a time, since one after the other each
 // would be a trip to memory.
@@ -519,19 +529,16 @@ __global__ void __launch_bounds__(THREADS) k_kv_append(KvAppendArgs a) {
     __shared__ uint32_t red[THREADS / 32];
     const KvView& c = a.c;
     const int h = blockIdx.x % c.nkv, isv = (blockIdx.x / c.nkv) & 1;
+    if (blockIdx.x == 0) kv_vet_rows(c, a.r, threadIdx.x, THREADS);
     int idx;
     const int s = kv_seq_of(a.r, blockIdx.x / (2 * c.nkv), c.page_log, 2, &idx);
     if (idx < 0) return;
     const int t0 = a.r.begin(s), t1 = min(a.r.end(s), a.r.n_tok), p0 = a.r.pos0[s], slot = a.r.seqs[s];
-    if (p0 < 0 || t1 <= t0) return;
+    if (p0 < 0 || t1 <= t0 || t0 < 0) return;
     const int pg = (p0 >> c.page_log) + idx;                        // page of the slot
     const long long lo = max((long long)p0, (long long)pg << c.page_log);
     const long long hi = min((long long)p0 + (t1 - t0), (long long)(pg + 1) << c.page_log);
     if (lo >= hi) return;
-    if (t0 < 0) {
-        if (threadIdx.x == 0) kv_flag(c, KV_BAD_ARG);
-        return;
-    }
     // the rows are on their way while the page is looked up and checked
     const long long stride = isv ? a.v_stride : a.k_stride;
     const T* x = (isv ? (const T*)a.v : (const T*)a.k) + (t0 + (lo - p0)) * stride + (long long)h * c.hd;
@@ -684,6 +691,7 @@ __global__ void __launch_bounds__(kKvReadThreads) k_kv_read(KvReadArgs a) {
     const KvView& c = a.c;
     const int h = blockIdx.x % c.nkv, isv = (blockIdx.x / c.nkv) & 1;
     T* out = isv ? (T*)a.v : (T*)a.k;
+    if (blockIdx.x == 0) kv_vet_rows(c, a.r, threadIdx.x, kKvReadThreads);
     if (!out) return;
     int idx;
     const int s = kv_seq_of(a.r, blockIdx.x / (2 * c.nkv), kKvReadLog, 1, &idx);

@@ -277,6 +277,7 @@ __global__ void __launch_bounds__(kKvaThreads, KvaShape<HDP, D, WIDE>::kBlocks) 
     typename SH::Info* info = reinterpret_cast<typename SH::Info*>(smem + SH::kInfo);
     long long *s_red = reinterpret_cast<long long*>(smem + SH::kSums), *s_range = s_red + kKvaWarps;
 
+    if (blockIdx.x == 0) kv_vet_rows(c, a.r, threadIdx.x, kKvaThreads);
     // ---- the line: prefix sums of the sequences' groups (in the ring's memory), the block's and the warp's stretch
     long long* pre = reinterpret_cast<long long*>(smem);
     const int per = (a.r.n_seq + kKvaThreads - 1) / kKvaThreads, sa = min((int)threadIdx.x * per, a.r.n_seq),

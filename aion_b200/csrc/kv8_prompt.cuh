@@ -184,7 +184,10 @@ __global__ void __launch_bounds__(kKvpThreads, 1) k_kv_prompt(const KvAttnArgs a
     }
     const KvSeq q = kv_seq(a, s);
     const long long total = (long long)q.cnt * a.group;
-    if (blk < 0 || (long long)blk * ROWS >= total) return;
+    if (blk < 0 || (long long)blk * ROWS >= total) {
+        if (blockIdx.x == 0) kv_vet_rows(c, a.r, threadIdx.x, kKvpThreads);
+        return;
+    }
     const int row0 = blk * ROWS;
     const int rows = (int)min((long long)ROWS, total - row0);
     const int nq = rows > 128 ? 2 : 1;
@@ -672,6 +675,8 @@ __global__ void __launch_bounds__(kKvpThreads, 1) k_kv_prompt(const KvAttnArgs a
                 umma_commit_warp(smem_addr(&k_empty[(j + 2) % ST]));
             }
             umma_commit_warp(smem_addr(&done_bar));
+        } else if (blockIdx.x == 0) {
+            kv_vet_rows(c, a.r, threadIdx.x - 32 * (16 + NQ), 32 * (4 - NQ));
         }
     }
     tc_fence_before();

@@ -334,7 +334,8 @@ AION_API aion_status aion_quantize_activations(const float* x_dev, int8_t* qx_de
  * What the host cannot see in them is checked on the device: an entry whose
  * slot or count is out of range, or whose slot a changing call has met
  * earlier in its list, is skipped (the first one counts), as is a row whose
- * page is missing, and the cache's status word records it for
+ * page is missing or that row offsets (cu) put behind n_tok, and a sequence
+ * whose offsets are negative or fall; the cache's status word records it for
  * aion_kv8_status.  Nothing out of bounds is read or written.
  * ------------------------------------------------------------------------- */
 typedef struct aion_kv8 {

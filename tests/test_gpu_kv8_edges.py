@@ -49,6 +49,30 @@ def test_attention_rows_in_front_of_the_first_sequence(cuda, first, n_kv, counts
     p.c.status()
 
 
+@pytest.mark.parametrize("cu", [[0, 20, 15, 40], [0, 30, 60, 61], [-3, 10, 20, 40], [0, 40, 10, 39]])
+def test_row_offsets_out_of_range_are_reported(cuda, cu):
+    """They fall, pass the 40 rows of the call or are negative: every call that takes
+    them says so, and touches no row outside."""
+    import aion_b200 as A
+    for n_kv, group in ((2, 1), (40, 4)):   # streams of keys; tiles of rows
+        p = Pair(cuda, 1, 40, n_kv, 32, 4, 8, 16)
+        p.fill([60, 60, 60], cuda.float32)
+        rows, q, slots, at = p.rows(40, n_kv, cuda.float32), p.rows(40, n_kv * group, cuda.float32), p.ints([0, 1, 2]), p.ints([0, 0, 0])
+        k, v, wide = (cuda.full((60, h, 32), 7.0, device="cuda") for h in (n_kv, n_kv, n_kv * group))
+        for call in (lambda: p.c.append(0, rows, rows, slots, at, p.ints(cu)),
+                     lambda: p.c.read(0, slots, at, 40, p.ints(cu), out=(k[10:50], v[10:50])),
+                     lambda: p.c.attention(0, q, slots, at, p.ints(cu), out=wide[10:50])):
+            call()
+            with pytest.raises(A.AionError) as e:
+                p.c.status()
+            assert e.value.code == "ARG"
+        for t in (k, v, wide):
+            assert (t[:10] == 7).all() and (t[50:] == 7).all() and cuda.isfinite(t).all()
+        # of skipped sequences there is nothing to say
+        p.c.attention(0, q, slots, p.ints([0, -1, -1]), p.ints([0, 40, 39, 100]), out=wide[10:50])
+        p.c.status()
+
+
 # ---------------------------------------------------------------------------
 # Lists whose needs add up past 32 bits
 # ---------------------------------------------------------------------------
