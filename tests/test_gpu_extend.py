@@ -230,3 +230,16 @@ def test_a_failure_behind_the_growth_is_undone(cuda, tiny_path):
         cuda.cuda.synchronize()
         m.extend(c, [1, 0], [[1] * 16, [1]])
         assert c.lens.tolist()[:2] == [21, 16]
+
+
+def test_extend_reports_a_wait_that_gave_up_before_it_grows(cuda, tiny_path):
+    import aion_b200 as A
+    with A.Model(tiny_path) as m:
+        c, _ = pair(A, m, 16, 4)
+        c.work[0] = 8   # as an attention call before it would have left it
+        cuda.cuda.synchronize()
+        with pytest.raises(A.AionError) as e:
+            m.extend(c, [1], [[1, 2]])
+        assert e.value.code == "TIMEOUT" and c.lens.sum().item() == 0 and c.refs.sum().item() == 0
+        m.extend(c, [1], [[1, 2]])
+        assert c.lens[1].item() == 2

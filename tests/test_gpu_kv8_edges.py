@@ -289,3 +289,44 @@ def test_rows_that_see_nothing_are_zero_whatever_their_query(cuda, name, n_kv, r
     assert e.value.code == "STATE"
     assert (out[:2] == 0).all()
     assert cuda.isnan(out[-1, 0]).all() and cuda.isfinite(out[-1, 1:]).all() and cuda.isfinite(out[2:-1]).all()
+
+
+def test_rows_of_a_slot_without_pages_are_zero_and_reported(cuda):
+    """Beside rows that have their pages, which come out whole."""
+    import aion_b200 as A
+    p = Pair(cuda, 1, 20, 1, 16, 4, 3, 16)
+    p.fill([20, 20], cuda.float32)
+    k, v = p.c.read(0, p.ints([0, 3]), p.ints([19, 0]), 4, p.ints([0, 3, 4]))
+    with pytest.raises(A.AionError) as e:
+        p.c.status()
+    assert e.value.code == "STATE"
+    for got, want in zip((k, v), p.r.rows(0, 0, 22)):   # positions 20 and 21: in slot 0's last page, behind its length
+        assert np.array_equal(got[:3].cpu().numpy(), want[19:].astype(np.float32)) and (got[3] == 0).all()
+
+
+@pytest.mark.parametrize("bits,code", [(8, "TIMEOUT"), (15, "TIMEOUT"), (7, "ARG"), (5, "STATE"), (1, "OOM")])
+def test_status_reports_the_first_that_applies_once(cuda, bits, code):
+    """The word that kernels set, among it what an attention call sets when a
+    bounded wait gives up."""
+    import aion_b200 as A
+    p = Pair(cuda, 1, 4, 1, 16, 2, 2, 16)
+    p.c.work[0] = bits
+    with pytest.raises(A.AionError) as e:
+        p.c.status()
+    assert e.value.code == code
+    p.c.status()
+
+
+# ---------------------------------------------------------------------------
+# fp32 rows, as close as their bits are
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("n_kv,group,hd,page,counts,before", [
+    (6, 1, 48, 16, [1, 1, 1], [500, 0, 77]), (2, 4, 128, 64, [1, 1], [300, 17]), (2, 2, 96, 32, [5, 9], [3, 260]),   # streams
+    (16, 1, 64, 16, [90, 1, 130, 77], [0, 40, 7, 100]), (8, 4, 48, 32, [37, 64, 129, 1], [0, 3, 70, 11])])           # tiles
+def test_fp32_rows_to_their_last_bits(cuda, n_kv, group, hd, page, counts, before):
+    p = Pair(cuda, 1, 120, n_kv, hd, 5, 64, page, seed=hd)
+    p.fill([a + b for a, b in zip(counts, before)], cuda.float32)
+    q = p.rows(sum(counts), n_kv * group, cuda.float32)
+    tiles = sum(counts) > 100
+    check_terms(p, q, list(range(len(counts))), before, counts, "f32", 2.0 ** -22 + 230 * 2.0 ** -32 if tiles else 2.0 ** -19,
+                with_cu=max(counts) > 1)
