@@ -17,10 +17,13 @@
 
 using namespace aion;
 
+// A failed call leaves its error behind for cudaGetLastError, too: taken here,
+// or the next launch that is checked would seem to have failed.
 #define KV_CUDA(call)                                                                                       \
     do {                                                                                                    \
         cudaError_t e_ = (call);                                                                            \
         if (e_ != cudaSuccess) {                                                                            \
+            (void)cudaGetLastError();                                                                       \
             aion_thread_error("%s: CUDA error %s (%s)", what, cudaGetErrorName(e_), cudaGetErrorString(e_)); \
             return e_ == cudaErrorMemoryAllocation ? AION_ERR_OOM : AION_ERR_CUDA;                          \
         }                                                                                                   \
@@ -110,7 +113,10 @@ static int sm_count(int dev) {
     if (dev < 0 || dev >= 64) return 148;
     if (!sms[dev]) {
         int v = 0;
-        if (cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || v <= 0) v = 148;
+        if (cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
+            (void)cudaGetLastError();
+            return 148;
+        }
         sms[dev] = v;
     }
     return sms[dev];

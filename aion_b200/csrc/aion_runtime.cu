@@ -64,10 +64,13 @@ static aion_status cuda_status(cudaError_t e) {
     return e == cudaErrorMemoryAllocation ? AION_ERR_OOM : AION_ERR_CUDA;
 }
 
+// A failed call leaves its error behind for cudaGetLastError, too: taken here,
+// or the next launch that is checked would seem to have failed.
 #define CK_RET(errp, call)                                                                          \
     do {                                                                                            \
         cudaError_t e_ = (call);                                                                    \
         if (e_ != cudaSuccess) {                                                                    \
+            (void)cudaGetLastError();                                                               \
             set_err(errp, "CUDA error %s (%s) at %s:%d", cudaGetErrorName(e_), cudaGetErrorString(e_), \
                     __FILE__, __LINE__);                                                            \
             return cuda_status(e_);                                                                 \

@@ -243,3 +243,17 @@ def test_extend_reports_a_wait_that_gave_up_before_it_grows(cuda, tiny_path):
         assert e.value.code == "TIMEOUT" and c.lens.sum().item() == 0 and c.refs.sum().item() == 0
         m.extend(c, [1], [[1, 2]])
         assert c.lens[1].item() == 2
+
+
+def test_extend_without_device_memory_for_its_rows(cuda, tiny_path):
+    """2^24 tokens: their operands pass the device's memory.  The next call does not see that error."""
+    import aion_b200 as A
+    with A.Model(tiny_path) as m:
+        c, _ = pair(A, m, 16, 4)
+        many = np.ones(1 << 24, np.int32)
+        with pytest.raises(A.AionError) as e:
+            m.extend(c, [0], [many])
+        assert e.value.code == "OOM" and c.lens.sum().item() == 0
+        m.extend(c, [0], [[1] * 20])
+        assert c.lens[0].item() == 20
+        c.status()

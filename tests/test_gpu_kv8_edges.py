@@ -1,6 +1,8 @@
 """The 8-bit paged K/V cache on the GPU at the edges of what its calls allow."""
 from __future__ import annotations
 
+import ctypes
+
 import numpy as np
 import pytest
 
@@ -330,3 +332,23 @@ def test_fp32_rows_to_their_last_bits(cuda, n_kv, group, hd, page, counts, befor
     tiles = sum(counts) > 100
     check_terms(p, q, list(range(len(counts))), before, counts, "f32", 2.0 ** -22 + 230 * 2.0 ** -32 if tiles else 2.0 ** -19,
                 with_cu=max(counts) > 1)
+
+
+# ---------------------------------------------------------------------------
+# Behind a call that failed
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("over,status", [(dict(n_layers=1000, n_pages=1 << 20, n_kv_heads=8, page_tokens=128, head_size=128), 4),   # 2^47 bytes
+                                         (dict(device=99), 5)])
+def test_a_failed_create_leaves_nothing_for_the_next_call(cuda, over, status):
+    """No memory; no such device.  What runs next, here and in torch, does not see that error."""
+    import aion_b200 as A
+    shape = dict(device=0, n_layers=1, n_pages=4, n_kv_heads=1, page_tokens=16, head_size=16, max_seqs=2, max_pages=2)
+    shape.update(over)
+    p = Pair(cuda, 1, 4, 1, 16, 2, 2, 16)
+    big, out = A.KV8(**shape), A.KV8()
+    cuda.cuda.synchronize()
+    assert A.lib().aion_kv8_create(ctypes.byref(big), ctypes.byref(out)) == status and not out.k
+    assert p.grow([0], [20]) == [0]
+    assert A.lib().aion_kv8_create(ctypes.byref(big), ctypes.byref(out)) == status
+    assert (cuda.ones(8, device="cuda") * 2).sum().item() == 16
+    p.c.status()
