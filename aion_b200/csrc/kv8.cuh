@@ -326,6 +326,8 @@ struct KvRows {
     int n_seq, n_tok;
     __device__ __forceinline__ int begin(int i) const { return cu ? cu[i] : i; }
     __device__ __forceinline__ int end(int i) const { return cu ? cu[i + 1] : i + 1; }
+    // entry i writes slot `s`; entries that are skipped (padding) or have no rows do not
+    __device__ __forceinline__ bool writes(int i, int s) const { return seqs[i] == s && pos0[i] >= 0 && end(i) > begin(i); }
 };
 
 // Records row offsets that fall, are negative or pass the rows of the call:
@@ -564,7 +566,7 @@ __global__ void __launch_bounds__(THREADS) k_kv_append(KvAppendArgs a) {
     if (a.vec) load(std::true_type{});
     else load(std::false_type{});
     bool bad = slot < 0 || slot >= c.max_seqs;
-    for (int j = threadIdx.x; j < s; j += THREADS) bad = bad || a.r.seqs[j] == slot;
+    for (int j = threadIdx.x; j < s; j += THREADS) bad = bad || a.r.writes(j, slot);
     const int page = slot >= 0 && slot < c.max_seqs && pg < c.max_pages ? c.tables[(size_t)slot * c.max_pages + pg] : -1;
     if (__syncthreads_or(bad)) {
         if (threadIdx.x == 0) kv_flag(c, KV_BAD_ARG);
@@ -610,7 +612,7 @@ __global__ void __launch_bounds__(kKvAppendThreads) k_kv_append_one(KvAppendArgs
     const T* x = isv ? (const T*)a.v + s * a.v_stride : (const T*)a.k + s * a.k_stride;
     const float4 v = 4 * lane < c.hd ? load4(x + (long long)h * c.hd + 4 * lane, a.vec) : make_float4(0, 0, 0, 0);
     bool twice = false;
-    for (int j = lane; j < s; j += 32) twice = twice || a.r.seqs[j] == slot;
+    for (int j = lane; j < s; j += 32) twice = twice || a.r.writes(j, slot);
     if (p0 < 0) return;
     if (__any_sync(0xffffffffu, twice) || slot < 0 || slot >= c.max_seqs) {
         if (lane == 0) kv_flag(c, KV_BAD_ARG);

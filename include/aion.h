@@ -396,7 +396,7 @@ AION_API aion_status aion_kv8_compact(const aion_kv8* kv, int32_t* n_used, void*
  * Sequence i has the rows cu[i] .. cu[i+1]-1 (cu NULL: one row each, n_tok =
  * n_seq; cu[0] need not be 0) and they stand at positions pos0[i],
  * pos0[i]+1, ... of slot seqs[i], which has pages for them (aion_kv8_grow);
- * pos0[i] < 0 skips the sequence.
+ * pos0[i] < 0 skips the sequence, which may then name any slot (padding).
  * Rows are [n_kv_heads][head_size] of `type`, k_stride / v_stride elements
  * apart.  Per page and head the scale is
  *   s = max|x| / 127                       for a page that starts here,

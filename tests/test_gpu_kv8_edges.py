@@ -6,7 +6,7 @@ import ctypes
 import numpy as np
 import pytest
 
-from test_gpu_kv8 import TYPES, Pair, dtype_of
+from test_gpu_kv8 import TYPES, Pair, check_attention, dtype_of
 
 pytestmark = pytest.mark.gpu
 
@@ -351,4 +351,21 @@ def test_a_failed_create_leaves_nothing_for_the_next_call(cuda, over, status):
     assert p.grow([0], [20]) == [0]
     assert A.lib().aion_kv8_create(ctypes.byref(big), ctypes.byref(out)) == status
     assert (cuda.ones(8, device="cuda") * 2).sum().item() == 16
+    p.c.status()
+
+
+# ---------------------------------------------------------------------------
+# Padding
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("counts,with_cu", [([1, 1, 1, 1, 1], False), ([1, 1, 1, 1, 1], True), ([3, 0, 20, 2, 5], True)])
+def test_padding_in_front_does_not_hide_a_sequence(cuda, counts, with_cu):
+    """Entries that are skipped, or have no rows, name slots that are written behind them."""
+    p = Pair(cuda, 1, 20, 2, 32, 4, 4, 16)
+    p.fill([17, 33], cuda.float32)
+    p.grow([0, 1], [20, 20])
+    p.append(0, [0, 1, 0, 1, 9], [-1, -1, 17, 33, -1], counts, cuda.float32, with_cu=with_cu)
+    p.same()
+    if not with_cu or counts[1]:
+        q = p.rows(5, 2, cuda.float32)
+        check_attention(p, 0, q, [0, 1, 0, 1, 9], [-1, -1, 17, 33, -1], counts, "f32", with_cu=with_cu)
     p.c.status()
