@@ -47,8 +47,11 @@ static void set_err(std::string* dst, const char* fmt, ...) {
     va_start(ap, fmt);
     vsnprintf(buf, sizeof(buf), fmt, ap);
     va_end(ap);
-    if (dst) *dst = buf;
-    g_thread_err = buf;
+    try {
+        if (dst) *dst = buf;
+        g_thread_err = buf;
+    } catch (const std::bad_alloc&) {   // the status says what it can
+    }
 }
 
 void aion_thread_error(const char* fmt, ...) {
@@ -57,7 +60,10 @@ void aion_thread_error(const char* fmt, ...) {
     va_start(ap, fmt);
     vsnprintf(buf, sizeof(buf), fmt, ap);
     va_end(ap);
-    g_thread_err = buf;
+    try {
+        g_thread_err = buf;
+    } catch (const std::bad_alloc&) {
+    }
 }
 
 static aion_status cuda_status(cudaError_t e) {
