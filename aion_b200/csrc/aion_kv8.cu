@@ -393,10 +393,12 @@ extern "C" AION_API aion_status aion_kv8_read(const aion_kv8* kv, int32_t layer,
 // the SM about 0.4 us a unit of 8 rows, the second 1.3 to 2.2 us a block of
 // 256, whatever there is in it, so the tiles win from about 4 units an SM and
 // wave of blocks on.  Measured, us of tiles / of streams, hd 128, page 64:
-//   fp32, 32 K/V heads, 4 x 4096 keys   16 rows 131 / 71, 32: 131 / 113, 64: 132 / 196
-//   bf16, 8 K/V heads, 16 x 4096 keys   16 rows 104 / 69, 32: 105 / 110, 64: 104 / 187
-//   bf16, 8 K/V heads, 1 x 32768 keys   256 rows 733 / 318, 512: 768 / 605, 1024: 770 / 1170
-// and within 4% of the better one from 4096 keys on over 147 such shapes (20% at 512 keys).
+//   fp32, 32 K/V heads, 4 x 4096 keys   16 rows 127 / 75, 32: 127 / 118, 64: 135 / 212
+//   bf16, 8 K/V heads, 16 x 4096 keys   16 rows 100 / 75, 32: 99 / 113, 64: 100 / 200
+//   bf16, 8 K/V heads, 1 x 32768 keys   256 rows 713 / 335, 512: 744 / 641, 1024: 748 / 1254
+// and within 5% (32768 keys), 14% (4096) and 18% (512) of the better one over 147 such shapes, of equally many rows
+// and keys a sequence.  The host knows a call's rows and sequences, not which sequence has how many: a call that mixes
+// a long chunk with single rows has one kernel for both, by the average.
 constexpr int kTileUnits = 4;
 static bool attention_tiles(const aion_kv8* kv, int n_seq, int n_tok, int group) {
     const int64_t rows = ((int64_t)n_tok * group + n_seq - 1) / n_seq, lines = (int64_t)n_seq * kv->n_kv_heads;
@@ -444,10 +446,10 @@ static cudaError_t launch_attention(KvAttnArgs a, int dev, cudaStream_t st) {
 template <typename T, int D>
 static cudaError_t launch_attention_of(const KvAttnArgs& a, int rows, int dev, cudaStream_t st) {
     // Units of 8 rows, or of 4 (16-bit rows) or 2 (fp32), whose turns are shorter but which read the keys anew.
-    // us, wide / narrow, 8 K/V heads, 1 x 32768 keys and 16 x 2048: bf16 4 rows 38.6 / 36.3 and 35.8 / 32.0, 8 rows
-    // 44.0 / 39.9 and 38.8 / 39.9, 12 rows 47.0 / 48.1 and 46.1 / 44.0, 16 rows 47.9 / 50.2 and 47.7 / 53.0; fp32
-    // 2 rows 39.8 / 35.9 and 35.5 / 31.9, 3 rows 39.9 / 39.9 and 35.8 / 39.1, 8 rows 45.9 / 50.5 and 39.4 / 52.4.
-    const bool wide = rows > (D == 2 ? 8 : 2);
+    // us, wide / narrow, 8 K/V heads, 1 x 32768 keys and 16 x 2048: bf16 4 rows 37.9 / 35.8 and 35.8 / 33.8, 5 rows
+    // 38.3 / 40.0 and 37.9 / 39.9, 8 rows 37.9 / 39.6 and 37.6 / 39.9, 16 rows 44.0 / 52.2 and 46.1 / 55.0; fp32 2 rows
+    // 37.9 / 33.9 and 35.8 / 31.7, 3 rows 37.9 / 38.1 and 35.9 / 37.9, 8 rows 38.1 / 50.2 and 37.0 / 52.2.
+    const bool wide = rows > (D == 2 ? 4 : 2);
     if (a.c.hd > 64) return wide ? launch_attention<T, 128, D, true>(a, dev, st) : launch_attention<T, 128, D, false>(a, dev, st);
     return wide ? launch_attention<T, 64, D, true>(a, dev, st) : launch_attention<T, 64, D, false>(a, dev, st);
 }
