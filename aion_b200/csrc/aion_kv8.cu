@@ -398,7 +398,8 @@ extern "C" AION_API aion_status aion_kv8_read(const aion_kv8* kv, int32_t layer,
 //   bf16, 8 K/V heads, 1 x 32768 keys   256 rows 713 / 335, 512: 744 / 641, 1024: 748 / 1254
 // and within 5% (32768 keys), 14% (4096) and 18% (512) of the better one over 147 such shapes, of equally many rows
 // and keys a sequence.  The host knows a call's rows and sequences, not which sequence has how many: a call that mixes
-// a long chunk with single rows has one kernel for both, by the average.
+// a long chunk with single rows has one kernel for both, by the average: bf16, 8 K/V heads, 31 rows over 8192 keys and
+// a chunk of 512 take 525 us, in calls of their own 116 and 217.
 constexpr int kTileUnits = 4;
 static bool attention_tiles(const aion_kv8* kv, int n_seq, int n_tok, int group) {
     const int64_t rows = ((int64_t)n_tok * group + n_seq - 1) / n_seq, lines = (int64_t)n_seq * kv->n_kv_heads;

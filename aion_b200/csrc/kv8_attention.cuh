@@ -72,11 +72,12 @@ struct KvAttnArgs {
 // zero): each branch keeps the MMAs around it from overlapping.
 //
 // Bound by memory where sequences are long: 16 x 8193..32767 bf16 tokens, 32
-// query heads on 8, take 120 us (672 MB, 5.6 TB/s), one of 131072 fp16 tokens
-// 60 us (269 MB, 4.5 TB/s).  32 x 512..639 fp32 tokens of 32 heads take 37 us
-// (153 MB): there the start (the line, the first pages, the first rows: about
-// 8 us) and the joins weigh.  8 x 3..5 drafted fp32 rows of 40 heads on
-// 251..1777 tokens take 40 us (85 MB), with 4 or 5 turns a warp.
+// query heads on 8, take 120 to 125 us (672 MB, 5.4 to 5.6 TB/s), one of 131072
+// fp16 tokens 60 us (269 MB, 4.5 TB/s).  32 x 512..639 fp32 tokens of 32 heads
+// take 37 us (153 MB) in a cache of at most 1024 tokens a sequence: there the
+// start (the line, the first pages, the first rows: about 8 us) and the joins
+// weigh, and a wider table adds the join's launch.  8 x 3..5 drafted fp32 rows
+// of 40 heads on 251..1777 tokens take 41 us (85 MB), with 4 or 5 turns a warp.
 // ---------------------------------------------------------------------------
 constexpr int kKvaWarps = 8, kKvaThreads = 32 * kKvaWarps, kKvaT = 64, kKvaRows = 8;
 

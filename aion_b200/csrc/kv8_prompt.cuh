@@ -34,7 +34,8 @@ namespace aion {
 // ones are split into two fp16 terms (22 bits), each with its own MMA.
 // Products of fp16 values are exact in the MMA and summed in fp32.
 // P = 2^(s - m) * 2^7 * vscale / vref in fp16 (fp32 rows: two terms, 22
-// bits), where vref is the largest V scale of the sequence's pages for this
+// bits; 16-bit rows: one, off by 2^-11 of itself at most, which is half a step
+// of an fp16 result and an eighth of one of bf16), where vref is the largest V scale of the sequence's pages for this
 // head, so that pages of different scales add up in one accumulator; the sum
 // l of 2^(s - m) is kept in fp32 from the unrounded weights.  m is a running
 // reference of s + log2(vscale / vref) over what the row sees, so that the
@@ -47,9 +48,10 @@ namespace aion {
 // A block of 256 rows takes 5K clocks to set up, 13K to bring fp32 queries in,
 // 2.6K (16-bit rows) or 3.3K (fp32) a key tile and 7K to write; the MMAs alone
 // would take 1.3K and 2.6K a tile.  2 x 1999..2048 bf16 rows of 32 heads on 8
-// behind 4096..6143 tokens: 600 us, 0.41 TFLOP, 680 TFLOP/s, bound by the
+// behind 4096..6143 tokens: 588 us, 0.41 TFLOP, 690 TFLOP/s, bound by the
 // softmax and the 3.5 blocks an SM.  8 x 512 fp32 rows of 32 heads: 110 us,
-// bound by what surrounds 2 to 8 key tiles of a block.
+// bound by what surrounds 2 to 8 key tiles of a block (its form spills 28 bytes
+// a thread around the loop).
 // ---------------------------------------------------------------------------
 constexpr int kKvpThreads = 640, kKvpTile = 64;
 constexpr int kKvpQ = 128 * 128 * 2;        // a query operand: 128 rows of two 128-byte-wide halves

@@ -461,12 +461,13 @@ AION_API aion_status aion_kv8_status(const aion_kv8* kv, void* stream);
  * continues slot seqs[i] with n_new[i] >= 1 tokens; `tokens` holds all of
  * them, sequence by sequence (all host memory).  Equivalent to transformer()
  * (src/kernel_simd.c:1014) for each token at the slot's next position, with
- * K and V rows held in 8 bits: prompts in chunks, single steps and drafts of
- * sequences of different lengths in one call, on prefixes that
- * aion_kv8_fork shares.  Products as in aion_prefill.  The slots grow by
- * their tokens; logits_host[n_seq][vocab] (may be NULL) receives the logits
- * of each sequence's last token.  Needs an int4 file and tp_size 1; W4A8
- * contexts run the same products.  AION_ERR_OOM when the cache has no room
+ * K and V rows held in 8 bits: prompts in chunks and single steps of
+ * sequences of different lengths in one call, on prefixes that aion_kv8_fork
+ * shares.  Products as in aion_prefill, which read every weight anew in each
+ * call: many tokens a call are what it is for.  The slots grow by their
+ * tokens; logits_host[n_seq][vocab] (may be NULL) receives the logits of each
+ * sequence's last token, and of no other.  Needs an int4 file and tp_size 1;
+ * W4A8 contexts run the same products.  AION_ERR_OOM when the cache has no room
  * for a sequence, AION_ERR_ARG when one would pass the checkpoint's seq_len:
  * every slot is then as long as before.  What earlier calls left for
  * aion_kv8_status is returned before anything grows.  After any other error
