@@ -150,7 +150,7 @@ __device__ __forceinline__ bool kvp_wait(uint64_t* bar, uint32_t parity, volatil
 // What the softmax needs to know of a key tile: for each 16 of its keys the
 // scales, and which of them have a page.
 struct alignas(16) KvpMeta {
-    float ks[4], fv[4];   // fv = 2^7 vscale / vref; ks is positive (1 where the page's values are 0 or NaN)
+    float ks[4], fv[4];   // fv = 2^7 vscale / vref; ks is not negative (1 where it is NaN or there is no page)
     float lv[4];          // log2(vscale / vref), kKvpLvMin at least
     uint32_t live, nan;   // bit j: keys 16 j.. have a page; one of its scales is NaN
 };
@@ -558,7 +558,7 @@ __global__ void __launch_bounds__(kKvpThreads, 1) k_kv_prompt(const KvAttnArgs a
                     const unsigned live = __ballot_sync(0xffffffffu, ks != -1.0f);
                     const unsigned nan = __ballot_sync(0xffffffffu, ks != ks || vs != vs);
                     if (lane < 4) {
-                        me.ks[lane] = ks > 0.0f ? ks : 1.0f;
+                        me.ks[lane] = ks >= 0.0f ? ks : 1.0f;
                         const float part = vs > 0.0f ? vs * vinv0 * vinv1 : 0.0f;
                         me.fv[lane] = 128.0f * part;
                         me.lv[lane] = fmaxf(__log2f(part), kKvpLvMin);

@@ -340,7 +340,7 @@ AION_API aion_status aion_quantize_activations(const float* x_dev, int8_t* qx_de
  * ------------------------------------------------------------------------- */
 typedef struct aion_kv8 {
     int8_t *k, *v;             /* [n_layers][n_pages][n_kv_heads][page_tokens][head_size], 16-byte aligned */
-    float *k_scale, *v_scale;  /* [n_layers][n_pages][n_kv_heads]                                          */
+    float *k_scale, *v_scale;  /* [n_layers][n_pages][n_kv_heads]: finite and not negative, or NaN         */
     int32_t* tables;           /* [max_seqs][max_pages] page ids; entries behind a slot's last page: -1    */
     int32_t* lens;             /* [max_seqs] tokens of each slot                                           */
     int32_t* refs;             /* [n_pages] slots that hold the page; 0: free                              */

@@ -245,6 +245,28 @@ def test_few_rows_over_scales_near_the_ends_of_the_range(cuda, name, page, group
                 with_cu=max(counts) > 1)
 
 
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("n_kv,counts,before", [(2, [1, 1], [300, 9]), (2, [5, 3], [60, 0]), (16, [320], [0])])
+def test_pages_of_zeros(cuda, name, page, n_kv, counts, before):
+    """K or V of a page all zero: rows that see V of no other are zero, and the page's keys weigh as they are."""
+    dt = dtype_of(cuda, name)
+    p = Pair(cuda, 1, 60, n_kv, 32, 2, 40, page, seed=page)
+    p.fill([a + b for a, b in zip(counts, before)], dt)
+    for slot in range(len(counts)):
+        t = p.r.tables[slot]
+        p.r.v_scale[0, t[0]] = 0
+        if t[2] >= 0:
+            p.r.k_scale[0, t[2]] = 0
+        if t[3] >= 0:
+            p.r.v_scale[0, t[3], 1:] = 0
+    p.upload()
+    q = p.rows(sum(counts), n_kv * 2, dt)
+    tiles = n_kv == 16
+    weight = {True: 2.0 ** -22 + 320 * 2.0 ** -32, False: 2.0 ** -19}[tiles] if name == "f32" else 2.0 ** -11
+    check_terms(p, q, list(range(len(counts))), before, counts, name, weight, with_cu=max(counts) > 1)
+
+
 # ---------------------------------------------------------------------------
 # Queries with one large channel
 # ---------------------------------------------------------------------------
